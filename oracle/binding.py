@@ -148,7 +148,7 @@ def build(which="all"):
     targets = []
     if which in ("all", "port"):
         targets.append("port")
-    if which in ("all", "ref") and os.path.isdir(os.environ.get("SFB_REFERENCE", "/root/reference")):
+    if which in ("all", "ref") and os.path.isdir(os.path.join(os.environ.get("SFB_REFERENCE", "/root/reference"), "src")):
         targets.append("ref")
     for target in targets:
         subprocess.run(["make", "-C", HERE, target, "-j8",
