@@ -322,6 +322,173 @@ sfb_status sfb_k_paged_kv_gather(const void* k_pool, const void* v_pool, void* k
                                  int head_dim, int head_dim_value, int block_tokens,
                                  int max_blocks, sfb_dtype dtype, sfb_stream stream);
 
+/* ---- serving operators over the paged cache (no counterpart in the reference) ---------------------------------
+ * They share the pool layout and the bound checks of sfb_k_attention_decode_paged: a context_len[b] below 0 or beyond
+ * what the tables and max_context cover is cut to that range, a block id outside [0, num_blocks) is skipped (its
+ * positions count as masked); either sets bit 0x200 of sfb_device_status.  bf16 or float32, head dimensions up to 256
+ * of either kind, any block size and any number of query heads per K/V head.  A sequence with nothing to attend to
+ * gives zeros.  Positions behind the live ones (the rest of a block, rows of dead nodes) may hold anything, NaN
+ * included.  `workspace`: device memory of at least the bytes the function beside it reports for the same arguments, 16-byte
+ * aligned, contents irrelevant before and after; calls that can overlap on the GPU need separate ones.  `splits` <= 0
+ * lets the library choose; `scale` <= 0 means 1/sqrt(head_dim).  Kernels are chosen by type, head dimension and
+ * alignment only, so the same arguments give the same bits every time. */
+
+/* Attention of a tree of drafted tokens over the cache (verification step of speculative decoding).  Every sequence
+ * brings `nodes` drafted tokens, of which the first node_count[b] are live; node i hangs below node parents[i] < i, or
+ * below the last committed token if parents[i] is -1.  Query (head, i) attends to the context_len[b] committed
+ * positions of its K/V head, to node i and to the ancestors of i:
+ *   out[b,h,i,:] = softmax over those of (scale * q . k) . v
+ * The drafted tokens' keys and values are passed as the layer produced them and are not in the cache;
+ * sfb_k_paged_kv_accept appends the accepted ones.  Rows of dead nodes are left as they were.  A parent outside
+ * [-1, i) counts as -1, a node_count outside [0, nodes] is cut, both set bit 0x200.  Values of live nodes must be
+ * finite: a NaN in one reaches every row of its tree.  nodes <= SFB_MAX_TREE_NODES, else SFB_UNSUPPORTED. */
+#define SFB_MAX_TREE_NODES 256
+typedef struct sfb_tree_args {
+    const void* q;           /* [batch, q_heads, nodes, head_dim]                                    */
+    const void* k_pool;
+    const void* v_pool;
+    const int* block_table;  /* int32 [batch, max_blocks]                                            */
+    const int* context_len;  /* int32 [batch], committed tokens, 0 allowed                           */
+    const void* draft_k;     /* [batch, kv_heads, nodes, head_dim]                                   */
+    const void* draft_v;     /* [batch, kv_heads, nodes, head_dim_value]                             */
+    const int* parents;      /* int32 [batch, nodes]                                                 */
+    const int* node_count;   /* int32 [batch]; NULL: every sequence has `nodes`                      */
+    void* out;               /* [batch, q_heads, nodes, head_dim_value], or, with token_major != 0,  */
+                             /* [batch, nodes, q_heads * head_dim_value]                             */
+    void* workspace;
+    int batch, q_heads, kv_heads, nodes, head_dim, head_dim_value;
+    int block_tokens, max_blocks, num_blocks;
+    int max_context;         /* upper bound of context_len, sizes the split count                    */
+    int splits;
+    float scale;
+    int token_major;
+    int dtype;
+} sfb_tree_args;
+size_t sfb_attention_tree_workspace(const sfb_tree_args* args);
+sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* args, sfb_stream stream);
+
+/* Appends the accepted path of a verified tree: for t < path_len[b] the K/V rows of node path[b, t] go to position
+ * start_len[b] + t, and new_len[b] = start_len[b] + path_len[b] (new_len may be NULL; it must not be start_len).
+ * path_len outside [0, max_path] is cut; a node outside [0, nodes) or a position past the table is skipped; both set
+ * bit 0x200. */
+typedef struct sfb_accept_args {
+    const void* draft_k;     /* [batch, kv_heads, nodes, head_dim]       */
+    const void* draft_v;     /* [batch, kv_heads, nodes, head_dim_value] */
+    void* k_pool;
+    void* v_pool;
+    const int* block_table;  /* int32 [batch, max_blocks] */
+    const int* start_len;    /* int32 [batch]             */
+    const int* path;         /* int32 [batch, max_path]   */
+    const int* path_len;     /* int32 [batch]             */
+    int* new_len;            /* int32 [batch] or NULL     */
+    int batch, kv_heads, nodes, max_path, head_dim, head_dim_value;
+    int block_tokens, max_blocks, num_blocks;
+    int dtype;
+} sfb_accept_args;
+sfb_status sfb_k_paged_kv_accept(const sfb_accept_args* args, sfb_stream stream);
+
+/* Key bounds of the cache's blocks, for sfb_k_attention_decode_sparse: bounds[block][kv_head][0][d] is the smallest and
+ * [1][d] the largest key element d among the block's live positions (NaN ignored), in the pool's type.  Recomputes
+ * every block that holds one of the positions [start_len[b], end_len[b]), over its positions below end_len[b]; other
+ * blocks keep theirs.  max_tokens: an upper bound of end_len - start_len, sizes the launch only. */
+typedef struct sfb_bounds_args {
+    const void* k_pool;
+    void* bounds;            /* [num_blocks][kv_heads][2][head_dim] */
+    const int* block_table;  /* int32 [batch, max_blocks] */
+    const int* start_len;    /* int32 [batch] */
+    const int* end_len;      /* int32 [batch] */
+    int batch, kv_heads, head_dim, max_tokens;
+    int block_tokens, max_blocks, num_blocks;
+    int dtype;
+} sfb_bounds_args;
+sfb_status sfb_k_paged_kv_bounds(const sfb_bounds_args* args, sfb_stream stream);
+
+/* Decode attention of one query token per sequence over the blocks that matter to it.  For each (sequence, K/V head)
+ * every live block gets a score that no logit of the block exceeds (before scaling),
+ *   score = max over the K/V head's query heads of sum_d max(q_d * low_d, q_d * high_d),  accumulated in 64 bits,
+ * and min(budget_blocks, live blocks) blocks are kept: the first sink_blocks, the last recent_blocks, and of the others those with the
+ * highest scores (ties: the lower index; a NaN score ranks last).  selected[b, kv_head, :] lists the kept logical
+ * block indices in ascending order, -1 behind them.  out is the softmax attention over the live positions of the
+ * kept blocks.  budget_blocks >= 1, sink_blocks + recent_blocks <= budget_blocks. */
+typedef struct sfb_sparse_args {
+    const void* q;           /* [batch, q_heads, head_dim]          */
+    const void* k_pool;
+    const void* v_pool;
+    const void* bounds;      /* sfb_k_paged_kv_bounds               */
+    const int* block_table;  /* int32 [batch, max_blocks]           */
+    const int* context_len;  /* int32 [batch]                       */
+    void* out;               /* [batch, q_heads, head_dim_value]    */
+    int* selected;           /* int32 [batch, kv_heads, budget_blocks] */
+    void* workspace;
+    int batch, q_heads, kv_heads, head_dim, head_dim_value;
+    int block_tokens, max_blocks, num_blocks;
+    int max_context;         /* upper bound of context_len          */
+    int budget_blocks, sink_blocks, recent_blocks;
+    int splits;
+    float scale;
+    int dtype;
+} sfb_sparse_args;
+size_t sfb_attention_sparse_workspace(const sfb_sparse_args* args);
+sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* args, sfb_stream stream);
+
+/* Decode attention of one query token per sequence that also accumulates its softmax weights: with p[h, t] the weight
+ * of position t in query head h,
+ *   weights_out[b, kv_head, t] = weights[b, kv_head, t] + sum over the K/V head's query heads of p[h, t]
+ * for t < context_len[b] (float32; entries behind it are left as they were).  weights NULL counts as zeros;
+ * weights_out may be weights itself.  positions != NULL: positions[b, kv_head, context_len[b] - 1] =
+ * query_position[b], the text position of the newest token, for sfb_k_paged_kv_evict. */
+typedef struct sfb_weights_args {
+    const void* q;           /* [batch, q_heads, head_dim]          */
+    const void* k_pool;
+    const void* v_pool;
+    const int* block_table;  /* int32 [batch, max_blocks]           */
+    const int* context_len;  /* int32 [batch]                       */
+    void* out;               /* [batch, q_heads, head_dim_value]    */
+    const float* weights;    /* [batch, kv_heads, weight_stride]    */
+    float* weights_out;
+    int* positions;          /* int32 [batch, kv_heads, weight_stride] or NULL */
+    const int* query_position; /* int32 [batch], with positions     */
+    void* workspace;
+    int batch, q_heads, kv_heads, head_dim, head_dim_value;
+    int block_tokens, max_blocks, num_blocks;
+    int max_context;         /* upper bound of context_len          */
+    int weight_stride;       /* >= max_context                      */
+    int splits;
+    float scale;
+    int dtype;
+} sfb_weights_args;
+size_t sfb_attention_weights_workspace(const sfb_weights_args* args);
+sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* args, sfb_stream stream);
+
+/* Cuts every (sequence, K/V head) to min(context_len[b], budget) cached positions.  Kept are those with a text position
+ * below sink_tokens, those among the recent_tokens newest text positions (> newest - recent_tokens) and of the others
+ * those with the largest weights (ties: the lower slot; NaN ranks last).  Kept rows in slots at or behind the new
+ * length move into the freed slots before it, both taken in ascending order; nothing else moves, so slots are no longer in text
+ * order and `positions` says which token each holds.  weights_out / positions_out receive the entries of the kept
+ * rows, 0 and -1 in slots [new length, context_len), and are left as they were behind that; each may be its input.
+ * new_len[b] = min(context_len[b], budget); it may be context_len.  Rows of K and V behind the new length stay as
+ * they were.  (Block bounds have to be recomputed over the new length.) */
+typedef struct sfb_evict_args {
+    void* k_pool;
+    void* v_pool;
+    const int* block_table;  /* int32 [batch, max_blocks]                    */
+    const int* context_len;  /* int32 [batch]                                */
+    const float* weights;    /* [batch, kv_heads, weight_stride]             */
+    float* weights_out;
+    const int* positions;    /* int32 [batch, kv_heads, weight_stride]       */
+    int* positions_out;
+    int* new_len;            /* int32 [batch]                                */
+    void* workspace;
+    int batch, kv_heads, head_dim, head_dim_value;
+    int block_tokens, max_blocks, num_blocks;
+    int max_context;         /* upper bound of context_len                   */
+    int weight_stride;       /* >= max_context                               */
+    int budget, sink_tokens, recent_tokens;
+    int dtype;
+} sfb_evict_args;
+size_t sfb_paged_kv_evict_workspace(const sfb_evict_args* args);
+sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* args, sfb_stream stream);
+
 /* Router: logits[t,e] = sum_f x[t,f]*router[f,e] accumulated sequentially in float32
  * (multiply rounded, then add rounded, f ascending) + optional bias[e]; softmax
  * numerators p = exp(logit - max); top-k by descending p (ties: lower expert id);

@@ -1,0 +1,371 @@
+// Single-token attention over a paged cache, CUDA-core form: any type, head dimension up to 256, block size and group.
+//
+// One CTA handles one (sequence, K/V head, up to eight query heads, split).  A key row is read by LPR lanes, eight
+// elements each, so that a warp has 32 / LPR rows in flight, four times over; every lane group runs its own online
+// softmax over the rows it meets (no synchronisation while streaming), and the groups, warps and splits are joined by
+// the log-sum-exp rule.  All heads of the CTA share each K and V byte.  Memory-bound for small groups; the K/V bytes
+// are read once per eight query heads.
+#include "cache_ops.cuh"
+
+namespace sfb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kRows = 4;  // rows in flight per lane group
+
+template <class T> struct Raw8;
+template <> struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const float4*>(p);
+        b = *reinterpret_cast<const float4*>(p + 4);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.0F, 0.0F, 0.0F, 0.0F); }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+};
+template <> struct Raw8<bf16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+// Eight elements of a row: lane `sub` of LPR owns [8 * sub, 8 * sub + 8) (VEC: dim % 8 == 0 and 16-byte aligned rows),
+// or every LPR-th element.
+template <class T, int LPR, bool VEC>
+struct Piece {
+    Raw8<T> raw;
+    float f[8];
+    __device__ __forceinline__ void load(const T* row, int sub, int dim, bool live) {
+        if constexpr (VEC) {
+            if (live && 8 * sub < dim) raw.load(row + 8 * sub);
+            else raw.zero();
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = sub + LPR * i;
+                f[i] = live && d < dim ? to_float(row[d]) : 0.0F;
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (VEC) raw.get(v);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = f[i];
+        }
+    }
+};
+
+template <class T, int LPR, int G, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32)
+step_kernel(const __grid_constant__ StepParams p) {
+    constexpr int RPW = 32 / LPR;
+    extern __shared__ float merge_smem[];  // [kWarps][G][dim_v + 2]
+    const PagedView& kv = p.kv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPR, rg = lane / LPR;
+    const int group = p.q_heads / kv.kv_heads;
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int chunks = (group + G - 1) / G;
+    const int kvh = blockIdx.y / chunks, head0 = kvh * group + (blockIdx.y % chunks) * G;
+    const int heads = min(G, (kvh + 1) * group - head0);
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int ctx = kv.length(b);
+    const int* list = p.selected ? p.selected + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.budget : nullptr;
+    const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
+    const int entries = list ? min(p.budget, blocks) : blocks;
+    const int e0 = min(entries, split * p.chunk_blocks), e1 = min(entries, e0 + p.chunk_blocks);
+    const int rows = (e1 - e0) * kv.block_tokens;
+
+    float q[G][8], o[G][8], m[G], l[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        Piece<T, LPR, VEC> piece;
+        piece.load(static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + head0 + (g < heads ? g : 0)) * kv.dim, sub, kv.dim, g < heads);
+        piece.get(q[g]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { q[g][i] *= p.scale_log2; o[g][i] = 0.0F; }
+        m[g] = -INFINITY;
+        l[g] = 0.0F;
+    }
+    for (int base = warp * RPW * kRows; base < rows; base += kWarps * RPW * kRows) {
+        Piece<T, LPR, VEC> kp[kRows], vp[kRows];
+        int position[kRows];
+        bool live[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int r = base + u * RPW + rg;
+            live[u] = r < rows;
+            int64_t at = -1;
+            position[u] = 0;
+            if (live[u]) {
+                const int e = kv.block_of(r);
+                int logical = list ? list[e0 + e] : e0 + e;
+                // (a list entry of -1 ends the list; it cannot be met before `entries`, but is not followed either)
+                position[u] = logical * kv.block_tokens + (r - e * kv.block_tokens);
+                live[u] = logical >= 0 && position[u] < ctx;
+                if (live[u]) at = kv.row(b, kvh, position[u]);
+            }
+            const bool there = at >= 0;
+            kp[u].load(static_cast<const T*>(kv.k_pool) + (there ? at : 0) * kv.dim, sub, kv.dim, there);
+            vp[u].load(static_cast<const T*>(kv.v_pool) + (there ? at : 0) * kv.dim_v, sub, kv.dim_v, there);
+            if (live[u] && !there && p.logits && sub < heads)   // a position whose block is missing weighs nothing
+                p.logits[(static_cast<size_t>(b) * p.q_heads + head0 + sub) * p.logit_stride + position[u]] = -INFINITY;
+            live[u] = there;
+        }
+        float x[kRows][G];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            float f[8];
+            kp[u].get(f);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float s = 0.0F;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fmaf(q[g][i], f[i], s);
+                x[u][g] = s;
+            }
+        }
+#pragma unroll
+        for (int w = 1; w < LPR; w <<= 1)
+#pragma unroll
+            for (int u = 0; u < kRows; ++u)
+#pragma unroll
+                for (int g = 0; g < G; ++g) x[u][g] += __shfl_xor_sync(0xffffffffu, x[u][g], w);
+        if (p.logits) {
+#pragma unroll
+            for (int u = 0; u < kRows; ++u)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (live[u] && sub == g % LPR && g < heads)
+                        p.logits[(static_cast<size_t>(b) * p.q_heads + head0 + g) * p.logit_stride + position[u]] = x[u][g];
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float top = m[g];
+#pragma unroll
+            for (int u = 0; u < kRows; ++u)
+                if (live[u]) top = fmaxf(top, x[u][g]);
+            const float alpha = top == -INFINITY ? 1.0F : exp2f(m[g] - top);
+            m[g] = top;
+            l[g] *= alpha;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[g][i] *= alpha;
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) {
+                x[u][g] = live[u] && x[u][g] != -INFINITY ? exp2f(x[u][g] - top) : 0.0F;
+                l[g] += x[u][g];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            float f[8];
+            vp[u].get(f);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[g][i] = fmaf(x[u][g], f[i], o[g][i]);
+        }
+    }
+    // lane groups of the warp
+#pragma unroll
+    for (int w = LPR; w < 32; w <<= 1)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float other = __shfl_xor_sync(0xffffffffu, m[g], w);
+            const float top = fmaxf(m[g], other);
+            const float mine = m[g] == -INFINITY ? 0.0F : exp2f(m[g] - top);
+            l[g] = l[g] * mine;
+            l[g] += __shfl_xor_sync(0xffffffffu, l[g], w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                o[g][i] *= mine;
+                o[g][i] += __shfl_xor_sync(0xffffffffu, o[g][i], w);
+            }
+            m[g] = top;
+        }
+    const int record = kv.dim_v + 2;
+    if (rg == 0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float* rec = merge_smem + (warp * G + g) * record;
+            if (sub == 0) { rec[0] = m[g]; rec[1] = l[g]; }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = VEC ? 8 * sub + i : sub + LPR * i;
+                if (d < kv.dim_v) rec[2 + d] = o[g][i];
+            }
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < heads * record; idx += kWarps * 32) {
+        const int g = idx / record, c = idx % record;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge_smem[(w * G + g) * record]);
+        float sum = 0.0F, value = 0.0F;
+        if (top != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float* rec = merge_smem + (w * G + g) * record;
+                const float f = rec[0] == -INFINITY ? 0.0F : exp2f(rec[0] - top);
+                sum += rec[1] * f;
+                value += rec[c] * f;
+            }
+        }
+        const size_t row = static_cast<size_t>(b) * p.q_heads + head0 + g;
+        if (p.splits == 1 && !p.logits) {
+            if (c >= 2) static_cast<T*>(p.out)[row * kv.dim_v + c - 2] = from_float<T>(sum > 0.0F ? value / sum : value);
+        } else {
+            p.partials[(row * p.splits + split) * record + c] = c == 0 ? top : c == 1 ? sum : value;
+        }
+    }
+}
+
+template <class T, int LPR, bool VEC>
+sfb_status launch_step(const StepParams& p, cudaStream_t stream) {
+    const int group = p.q_heads / p.kv.kv_heads;
+    const auto go = [&](auto kernel, int g) -> sfb_status {
+        const size_t smem = sizeof(float) * kWarps * g * (p.kv.dim_v + 2);
+        const dim3 grid(p.splits, p.kv.kv_heads * ceil_div(group, g), p.batch);
+        SFB_CUDA(launch_dependent(kernel, grid, dim3(kWarps * 32), smem, stream, p));
+        return check_launch("attention_step");
+    };
+    if (group == 1) return go(step_kernel<T, LPR, 1, VEC>, 1);
+    if (group == 2) return go(step_kernel<T, LPR, 2, VEC>, 2);
+    if (group <= 4) return go(step_kernel<T, LPR, 4, VEC>, 4);
+    return go(step_kernel<T, LPR, 8, VEC>, 8);
+}
+
+template <class T>
+sfb_status step_typed(const StepParams& p, cudaStream_t stream) {
+    const PagedView& kv = p.kv;
+    const bool vec = kv.dim % 8 == 0 && kv.dim_v % 8 == 0 && aligned16(p.q) && aligned16(kv.k_pool) && aligned16(kv.v_pool);
+    const int widest = kv.dim > kv.dim_v ? kv.dim : kv.dim_v;
+    if (!vec) return launch_step<T, 32, false>(p, stream);
+    if (widest <= 64) return launch_step<T, 8, true>(p, stream);
+    if (widest <= 128) return launch_step<T, 16, true>(p, stream);
+    return launch_step<T, 32, true>(p, stream);
+}
+
+// One CTA per output row; thread = output element (strided).
+template <class T>
+__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ MergeParams p) {
+    __shared__ float weight[128];
+    const int row = blockIdx.x;
+    const int node = row % p.nodes, head = (row / p.nodes) % p.q_heads, b = row / p.nodes / p.q_heads;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    if (p.node_count && node >= p.node_count[b]) return;
+    const int record = p.dim_v + 2;
+    const float* rec = p.partials + static_cast<size_t>(row) * p.splits * record;
+    if (threadIdx.x < 32) {
+        float m[4], top = -INFINITY, sum = 0.0F;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = threadIdx.x + 32 * i;
+            m[i] = s < p.splits ? rec[static_cast<size_t>(s) * record] : -INFINITY;
+            top = fmaxf(top, m[i]);
+        }
+        top = warp_max(top);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = threadIdx.x + 32 * i;
+            m[i] = m[i] == -INFINITY ? 0.0F : exp2f(m[i] - top);
+            if (s < p.splits) sum += rec[static_cast<size_t>(s) * record + 1] * m[i];
+        }
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = threadIdx.x + 32 * i;
+            if (s < p.splits) weight[s] = sum > 0.0F ? m[i] / sum : 0.0F;
+        }
+    }
+    __syncthreads();
+    T* dst = static_cast<T*>(p.out) + (p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
+                                                     : static_cast<size_t>(row)) * p.dim_v;
+    for (int d = threadIdx.x; d < p.dim_v; d += 128) {
+        float a = 0.0F;
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {
+            const float w = weight[s];
+            if (w != 0.0F) a = fmaf(w, rec[static_cast<size_t>(s) * record + 2 + d], a);
+        }
+        dst[d] = from_float<T>(a);
+    }
+}
+
+}  // namespace
+
+sfb_status check_cache(const void* k_pool, const void* v_pool, const int* table, int batch, int kv_heads, int dim, int dim_v,
+                       int block_tokens, int max_blocks, int num_blocks, int dtype, const char* what) {
+    const std::string name(what);
+    SFB_REQUIRE(k_pool && v_pool && table, name + ": null tensor");
+    SFB_REQUIRE(batch > 0 && kv_heads > 0 && dim > 0 && dim_v > 0 && block_tokens > 0 && max_blocks > 0 && num_blocks > 0,
+                name + ": invalid cache shape");
+    SFB_REQUIRE(dtype == SFB_F32 || dtype == SFB_BF16, name + ": unknown dtype");
+    if (dim > 256 || dim_v > 256) return fail(SFB_UNSUPPORTED, name + ": head dimension > 256");
+    if (batch > 65535 || kv_heads > 4096) return fail(SFB_UNSUPPORTED, name + ": more than 65535 sequences or 4096 K/V heads");
+    if (static_cast<int64_t>(max_blocks) * block_tokens > (int64_t{1} << 30))
+        return fail(SFB_UNSUPPORTED, name + ": more than 2^30 positions in a block table");
+    return SFB_OK;
+}
+
+PagedView make_view(const void* k_pool, const void* v_pool, const int* table, const int* lens, int kv_heads, int dim, int dim_v,
+                    int block_tokens, int max_blocks, int num_blocks, int max_context) {
+    PagedView kv{};
+    kv.k_pool = k_pool; kv.v_pool = v_pool; kv.table = table; kv.lens = lens;
+    kv.kv_heads = kv_heads; kv.dim = dim; kv.dim_v = dim_v; kv.block_tokens = block_tokens;
+    kv.block_shift = shift_of(block_tokens);
+    kv.max_blocks = max_blocks; kv.num_blocks = num_blocks;
+    const int covered = max_blocks * block_tokens;
+    kv.limit = max_context < covered ? max_context : covered;
+    kv.status = device_status_word();
+    return kv;
+}
+
+// Splits of `tokens` positions: whole blocks, at most 128 splits (the merge keeps one weight per split in shared
+// memory), as long as the CTAs still fill the GPU (two to four per SM).  Long splits stream better (the ramp of a CTA
+// is paid once), short ones fill the GPU when there are few sequences; 64 positions is the least worth a CTA.
+int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wanted, int* chunk_blocks) {
+    const int blocks = tokens > 0 ? ceil_div(tokens, block_tokens) : 1;
+    int splits = wanted;
+    if (splits <= 0) {
+        int chunk = 2048;
+        splits = ceil_div(tokens, chunk);
+        while (static_cast<int64_t>(batch) * kv_heads * splits < 4LL * sm_count() && chunk > 64) {
+            chunk /= 2;
+            splits = ceil_div(tokens, chunk);
+        }
+    }
+    if (splits > 128) splits = 128;
+    if (splits > blocks) splits = blocks;
+    if (splits < 1) splits = 1;
+    *chunk_blocks = ceil_div(blocks, splits);
+    return ceil_div(blocks, *chunk_blocks);
+}
+
+sfb_status step_attention(const StepParams& p, int dtype, cudaStream_t stream) {
+    return dtype == SFB_F32 ? step_typed<float>(p, stream) : step_typed<bf16>(p, stream);
+}
+
+sfb_status merge_partials(const MergeParams& p, int dtype, cudaStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.nodes;
+    const dim3 grid(static_cast<unsigned>(rows));
+    if (dtype == SFB_F32) SFB_CUDA(launch_dependent(merge_kernel<float>, grid, dim3(128), 0, stream, p));
+    else SFB_CUDA(launch_dependent(merge_kernel<bf16>, grid, dim3(128), 0, stream, p));
+    return check_launch("attention_merge");
+}
+
+}  // namespace sfb

@@ -1,0 +1,60 @@
+// Parameters and the ancestor table shared by the tree-attention kernels.
+#pragma once
+
+#include "cache_ops.cuh"
+
+namespace sfb {
+
+struct TreeParams {
+    PagedView kv;
+    const void *q, *draft_k, *draft_v;
+    const int *parents, *node_count;
+    void* out;
+    float* partials;
+    int batch, q_heads, nodes, token_major, splits, chunk, vec;
+    float scale_log2;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int tree_node_count(const TreeParams& p, int b) {
+    if (!p.node_count) return p.nodes;
+    int n = p.node_count[b];
+    if (n < 0 || n > p.nodes) {
+        n = n < 0 ? 0 : p.nodes;
+        if (threadIdx.x == 0) atomicOr(p.kv.status, kCodeDecodeBounds);
+    }
+    return n;
+}
+
+__device__ __forceinline__ size_t tree_out_row(const TreeParams& p, int b, int head, int node) {
+    return p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
+                         : (static_cast<size_t>(b) * p.q_heads + head) * p.nodes + node;
+}
+
+// seen[8 * i + w]: bit j % 32 of word j / 32 says that node i sees node j (itself and its ancestors).  Parents are
+// smaller than their children, so every walk ends.  All threads of the CTA call it; seen is ready after their next
+// __syncthreads().
+__device__ __forceinline__ void tree_ancestors(const TreeParams& p, int b, int count, int* parent, uint32_t* seen) {
+    for (int i = threadIdx.x; i < p.nodes; i += blockDim.x) {
+        int up = i < count ? p.parents[static_cast<size_t>(b) * p.nodes + i] : -1;
+        if (up < -1 || up >= i) {
+            up = -1;
+            atomicOr(p.kv.status, kCodeDecodeBounds);
+        }
+        parent[i] = up;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.nodes; i += blockDim.x) {
+        uint32_t words[8] = {};
+        for (int j = i < count ? i : -1; j >= 0; j = parent[j]) {
+#pragma unroll
+            for (int w = 0; w < 8; ++w)
+                if (w == j >> 5) words[w] |= 1u << (j & 31);
+        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w) seen[8 * i + w] = words[w];
+    }
+}
+#endif
+
+}  // namespace sfb

@@ -1,0 +1,377 @@
+// Accumulated attention weights, eviction by them, and the append of an accepted path.
+//
+// Weights: the decode kernel keeps every scaled logit (4 bytes per position and query head beside 4 * dim bytes of K and
+// V); once the splits are merged, exp2(logit - maximum) / sum of each head is added to the running sums.
+// Eviction: one CTA per (sequence, K/V head) finds the threshold of the kept weights and lists the kept rows that
+// lie behind the new length and the freed slots before it.  There are equally many, and no slot is in both lists, so the
+// rows can move in any order and with any parallelism.
+#include "cache_ops.cuh"
+#include "select.cuh"
+
+namespace sfb {
+namespace {
+
+// ---- weights ----------------------------------------------------------------------------------------------------
+
+struct AddParams {
+    PagedView kv;
+    const float *partials, *logits, *weights;
+    float* weights_out;
+    void* out;
+    int* positions;
+    const int* query_position;
+    int64_t logit_stride;
+    int q_heads, splits, stride;
+};
+
+constexpr int kAddThreads = 256;
+constexpr int kAddChunk = 1024;  // positions per CTA
+
+// CTA (chunk, K/V head, sequence): maxima and sums of the heads from the split records, then its share of the heads'
+// outputs, then its positions.
+template <class T>
+__global__ void __launch_bounds__(kAddThreads)
+add_weights_kernel(const __grid_constant__ AddParams p) {
+    extern __shared__ float stats[];  // [group] maximum, [group] 1 / sum
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = p.q_heads / kv.kv_heads, record = kv.dim_v + 2;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int ctx = kv.length(b);
+    const int first = blockIdx.x * kAddChunk;
+    const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
+    if (first >= ctx && blockIdx.x >= group) return;
+    for (int g = warp; g < group; g += kAddThreads / 32) {
+        const float* rec = p.partials + (row0 + g) * p.splits * record;
+        float top = -INFINITY, sum = 0.0F;
+        for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, rec[static_cast<size_t>(s) * record]);
+        top = warp_max(top);
+        for (int s = lane; s < p.splits; s += 32) {
+            const float m = rec[static_cast<size_t>(s) * record];
+            if (m != -INFINITY) sum += rec[static_cast<size_t>(s) * record + 1] * exp2f(m - top);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) {
+            stats[g] = top == -INFINITY ? 0.0F : top;
+            stats[group + g] = sum > 0.0F ? 1.0F / sum : 0.0F;
+        }
+    }
+    __syncthreads();
+    for (int g = blockIdx.x; g < group; g += gridDim.x) {
+        const float* rec = p.partials + (row0 + g) * p.splits * record;
+        T* dst = static_cast<T*>(p.out) + (row0 + g) * kv.dim_v;
+        for (int d = threadIdx.x; d < kv.dim_v; d += kAddThreads) {
+            float a = 0.0F;
+#pragma unroll 4
+            for (int s = 0; s < p.splits; ++s) {
+                const float m = rec[static_cast<size_t>(s) * record];
+                if (m != -INFINITY) a = fmaf(rec[static_cast<size_t>(s) * record + 2 + d], exp2f(m - stats[g]), a);
+            }
+            dst[d] = from_float<T>(a * stats[group + g]);
+        }
+    }
+    const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
+    const int end = min(ctx, first + kAddChunk);
+    for (int t = first + threadIdx.x; t < end; t += kAddThreads) {
+        float w = 0.0F;
+        for (int g = 0; g < group; ++g)
+            w = fmaf(exp2f(p.logits[(row0 + g) * p.logit_stride + t] - stats[g]), stats[group + g], w);
+        p.weights_out[wrow + t] = (p.weights ? p.weights[wrow + t] : 0.0F) + w;
+        if (p.positions && t == ctx - 1) p.positions[wrow + t] = p.query_position[b];
+    }
+}
+
+struct WeightsLayout {
+    int splits, chunk_blocks;
+    int64_t logit_stride;
+    size_t partials, total;
+};
+
+WeightsLayout weights_layout(const sfb_weights_args& a) {
+    WeightsLayout l{};
+    const int covered = a.max_blocks * a.block_tokens;
+    const int limit = a.max_context < covered ? a.max_context : covered;
+    l.splits = step_splits(a.batch, a.kv_heads, limit, a.block_tokens, a.splits, &l.chunk_blocks);
+    l.logit_stride = (limit + 3) & ~3;
+    l.partials = round_up16(sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.splits * (a.head_dim_value + 2));
+    l.total = l.partials + sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.logit_stride;
+    return l;
+}
+
+sfb_status check_weights(const sfb_weights_args* a) {
+    SFB_REQUIRE(a, "decode weights: null arguments");
+    SFB_TRY(check_cache(a->k_pool, a->v_pool, a->block_table, a->batch, a->kv_heads, a->head_dim, a->head_dim_value,
+                        a->block_tokens, a->max_blocks, a->num_blocks, a->dtype, "decode weights"));
+    SFB_REQUIRE(a->q_heads > 0 && a->q_heads % a->kv_heads == 0, "invalid grouped-query attention configuration");
+    SFB_REQUIRE(a->max_context > 0 && a->weight_stride >= a->max_context, "decode weights: weight_stride shorter than max_context");
+    return SFB_OK;
+}
+
+// ---- eviction ------------------------------------------------------------------------------------------------------
+
+struct EvictParams {
+    PagedView kv;
+    const float* weights;
+    float* weights_out;
+    const int* positions;
+    int* positions_out;
+    int* new_len;
+    int* moves;            // per (sequence, K/V head): count, then max_moves destinations, then max_moves sources
+    int max_moves, stride, budget, sink, recent;
+};
+
+constexpr int kEvictThreads = 1024;
+
+__global__ void __launch_bounds__(kEvictThreads)
+evict_select_kernel(const __grid_constant__ EvictParams p) {
+    __shared__ SelectShared sh;
+    __shared__ int newest_of[32];
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int n = kv.length(b), k = min(n, p.budget);
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    const float* weights = p.weights + row * p.stride;
+    const int* positions = p.positions + row * p.stride;
+    float* weights_out = p.weights_out + row * p.stride;
+    int* positions_out = p.positions_out + row * p.stride;
+    int* to = p.moves + row * (1 + 2 * static_cast<size_t>(p.max_moves)) + 1;
+    int* since = to + p.max_moves;
+    if (k == n) {
+        if (threadIdx.x == 0) to[-1] = 0;
+        for (int i = threadIdx.x; i < n; i += kEvictThreads) {
+            weights_out[i] = weights[i];
+            positions_out[i] = positions[i];
+        }
+        return;
+    }
+    int newest = -1;
+    for (int i = threadIdx.x; i < n; i += kEvictThreads) newest = max(newest, positions[i]);
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) newest_of[warp] = newest;
+    __syncthreads();
+    newest = __reduce_max_sync(0xffffffffu, newest_of[lane]);
+    const int64_t recent_from = static_cast<int64_t>(newest) - p.recent;
+    const int sink = p.sink;
+    const auto key = [&](int i) -> uint64_t {
+        const int at = positions[i];
+        return at < sink || at > recent_from ? ~0ull : order_key(weights[i]);
+    };
+    const Threshold t = select_threshold<kEvictThreads>(sh, n, k, key);
+    int ties = 0, holes = 0, tails = 0;
+    for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
+        const int i = i0 + threadIdx.x;
+        const uint64_t v = i < n ? key(i) : 0;
+        const bool tie = i < n && t.cut != 0 && v == t.low;
+        int tie_rank, unused, tie_total, unused_total;
+        flag_ranks<kEvictThreads>(sh.scan, tie, false, tie_rank, unused, tie_total, unused_total);
+        const bool kept = i < n && (tie ? tie_rank < t.cut - ties : (t.cut != 0 ? v > t.low : v >= t.low));
+        ties += tie_total;
+        const bool hole = i < k && !kept, tail = i >= k && kept;
+        int hole_rank, tail_rank, hole_total, tail_total;
+        flag_ranks<kEvictThreads>(sh.scan, hole, tail, hole_rank, tail_rank, hole_total, tail_total);
+        if (hole) to[holes + hole_rank] = i;
+        if (tail) since[tails + tail_rank] = i;
+        holes += hole_total;
+        tails += tail_total;
+        if (i < k && kept) {
+            weights_out[i] = weights[i];
+            positions_out[i] = positions[i];
+        }
+    }
+    __syncthreads();  // the lists, and every read of weights and positions that an aliased output may overwrite
+    for (int j = threadIdx.x; j < holes; j += kEvictThreads) {
+        weights_out[to[j]] = weights[since[j]];
+        positions_out[to[j]] = positions[since[j]];
+    }
+    __syncthreads();
+    for (int i = k + threadIdx.x; i < n; i += kEvictThreads) {
+        weights_out[i] = 0.0F;
+        positions_out[i] = -1;
+    }
+    if (threadIdx.x == 0) to[-1] = holes;
+}
+
+// One warp per moved row; new_len is written here, after every reader of context_len (it may be the same array).
+template <class V>
+__global__ void __launch_bounds__(256)
+evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_units) {
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int* to = p.moves + (static_cast<size_t>(b) * kv.kv_heads + kvh) * (1 + 2 * static_cast<size_t>(p.max_moves)) + 1;
+    const int* since = to + p.max_moves;
+    const int count = to[-1];
+    V* keys = static_cast<V*>(const_cast<void*>(kv.k_pool));
+    V* values = static_cast<V*>(const_cast<void*>(kv.v_pool));
+    for (int j = blockIdx.x * 8 + warp; j < count; j += gridDim.x * 8) {
+        const int64_t src = kv.row(b, kvh, since[j]), dst = kv.row(b, kvh, to[j]);
+        if (src < 0 || dst < 0) continue;
+        for (int i = lane; i < k_units; i += 32) keys[dst * k_units + i] = keys[src * k_units + i];
+        for (int i = lane; i < v_units; i += 32) values[dst * v_units + i] = values[src * v_units + i];
+    }
+    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) p.new_len[b] = min(max(kv.lens[b], 0), min(p.budget, kv.limit));
+}
+
+int evict_max_moves(const sfb_evict_args& a) {
+    const int covered = a.max_blocks * a.block_tokens;
+    const int limit = a.max_context < covered ? a.max_context : covered;
+    const int beyond = limit - a.budget;
+    return beyond <= 0 ? 0 : (beyond < a.budget ? beyond : a.budget);
+}
+
+sfb_status check_evict(const sfb_evict_args* a) {
+    SFB_REQUIRE(a, "evict: null arguments");
+    SFB_TRY(check_cache(a->k_pool, a->v_pool, a->block_table, a->batch, a->kv_heads, a->head_dim, a->head_dim_value,
+                        a->block_tokens, a->max_blocks, a->num_blocks, a->dtype, "evict"));
+    SFB_REQUIRE(a->max_context > 0 && a->weight_stride >= a->max_context, "evict: weight_stride shorter than max_context");
+    SFB_REQUIRE(a->budget > 0 && a->sink_tokens >= 0 && a->recent_tokens >= 0 &&
+                    static_cast<int64_t>(a->sink_tokens) + a->recent_tokens <= a->budget,
+                "evict: the sink and recent tokens have to fit into the budget");
+    return SFB_OK;
+}
+
+// ---- accepted path ---------------------------------------------------------------------------------------------------
+
+struct AcceptParams {
+    PagedView kv;
+    const void *draft_k, *draft_v;
+    const int *path, *path_len;
+    int* new_len;
+    int nodes, max_path;
+};
+
+// One warp per appended row.
+template <class V>
+__global__ void __launch_bounds__(256)
+accept_kernel(const __grid_constant__ AcceptParams p, int k_units, int v_units) {
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int start = kv.lens[b];
+    int count = p.path_len[b];
+    if (count < 0 || count > p.max_path) {
+        count = count < 0 ? 0 : p.max_path;
+        if (threadIdx.x == 0) atomicOr(kv.status, kCodeDecodeBounds);
+    }
+    if (p.new_len && blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) p.new_len[b] = start + count;
+    const V* draft_k = static_cast<const V*>(p.draft_k) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * k_units;
+    const V* draft_v = static_cast<const V*>(p.draft_v) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * v_units;
+    V* keys = static_cast<V*>(const_cast<void*>(kv.k_pool));
+    V* values = static_cast<V*>(const_cast<void*>(kv.v_pool));
+    for (int t = blockIdx.x * 8 + warp; t < count; t += gridDim.x * 8) {
+        const int node = p.path[static_cast<size_t>(b) * p.max_path + t];
+        const int64_t position = static_cast<int64_t>(start) + t;
+        if (node < 0 || node >= p.nodes || position < 0 || position >= kv.limit) {
+            atomicOr(kv.status, kCodeDecodeBounds);
+            continue;
+        }
+        const int64_t dst = kv.row(b, kvh, static_cast<int>(position));
+        if (dst < 0) continue;
+        for (int i = lane; i < k_units; i += 32) keys[dst * k_units + i] = draft_k[static_cast<size_t>(node) * k_units + i];
+        for (int i = lane; i < v_units; i += 32) values[dst * v_units + i] = draft_v[static_cast<size_t>(node) * v_units + i];
+    }
+}
+
+// Rows are copied in units of 16 bytes where every row starts and ends on one, else in elements.
+bool wide_rows(int dim, int dim_v, int dtype) {
+    return dim * dtype_size(dtype) % 16 == 0 && dim_v * dtype_size(dtype) % 16 == 0;
+}
+
+}  // namespace
+}  // namespace sfb
+
+using namespace sfb;
+
+extern "C" {
+
+size_t sfb_attention_weights_workspace(const sfb_weights_args* a) {
+    if (check_weights(a) != SFB_OK) return 0;
+    return weights_layout(*a).total;
+}
+
+sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream stream) {
+    SFB_TRY(check_weights(a));
+    SFB_REQUIRE(a->q && a->context_len && a->out && a->weights_out && a->workspace, "decode weights: null tensor");
+    SFB_REQUIRE(!a->positions || a->query_position, "decode weights: positions without query_position");
+    SFB_REQUIRE(aligned16(a->workspace), "decode weights: the workspace has to be 16-byte aligned");
+    const WeightsLayout l = weights_layout(*a);
+    cudaStream_t s = as_stream(stream);
+    StepParams p{};
+    p.kv = make_view(a->k_pool, a->v_pool, a->block_table, a->context_len, a->kv_heads, a->head_dim, a->head_dim_value,
+                     a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
+    p.q = a->q; p.out = a->out;
+    p.partials = static_cast<float*>(a->workspace);
+    p.logits = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + l.partials);
+    p.logit_stride = l.logit_stride;
+    p.batch = a->batch; p.q_heads = a->q_heads; p.splits = l.splits; p.chunk_blocks = l.chunk_blocks;
+    p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
+    SFB_TRY(step_attention(p, a->dtype, s));
+    const AddParams add{p.kv, p.partials, p.logits, a->weights, a->weights_out, a->out, a->positions, a->query_position,
+                        l.logit_stride, a->q_heads, l.splits, a->weight_stride};
+    const int group = a->q_heads / a->kv_heads;
+    const dim3 grid(ceil_div(p.kv.limit, kAddChunk), a->kv_heads, a->batch);
+    const size_t smem = sizeof(float) * 2 * group;
+    if (smem > 48 * 1024) return fail(SFB_UNSUPPORTED, "decode weights: more than 6144 query heads per K/V head");
+    if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(add_weights_kernel<float>, grid, dim3(kAddThreads), smem, s, add));
+    else SFB_CUDA(launch_dependent(add_weights_kernel<bf16>, grid, dim3(kAddThreads), smem, s, add));
+    return check_launch("decode_weights_add");
+}
+
+size_t sfb_paged_kv_evict_workspace(const sfb_evict_args* a) {
+    if (check_evict(a) != SFB_OK) return 0;
+    return sizeof(int) * static_cast<size_t>(a->batch) * a->kv_heads * (1 + 2 * static_cast<size_t>(evict_max_moves(*a)));
+}
+
+sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
+    SFB_TRY(check_evict(a));
+    SFB_REQUIRE(a->context_len && a->weights && a->weights_out && a->positions && a->positions_out && a->new_len && a->workspace,
+                "evict: null tensor");
+    SFB_REQUIRE(aligned16(a->workspace), "evict: the workspace has to be 16-byte aligned");
+    cudaStream_t s = as_stream(stream);
+    EvictParams p{};
+    p.kv = make_view(a->k_pool, a->v_pool, a->block_table, a->context_len, a->kv_heads, a->head_dim, a->head_dim_value,
+                     a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
+    p.weights = a->weights; p.weights_out = a->weights_out; p.positions = a->positions; p.positions_out = a->positions_out;
+    p.new_len = a->new_len; p.moves = static_cast<int*>(a->workspace); p.max_moves = evict_max_moves(*a);
+    p.stride = a->weight_stride; p.budget = a->budget; p.sink = a->sink_tokens; p.recent = a->recent_tokens;
+    SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), 0, s, p));
+    SFB_TRY(check_launch("evict_select"));
+    const dim3 grid(p.max_moves > 0 ? (p.max_moves > 64 * 8 ? 64 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
+    const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool);
+    const int per = wide ? 16 / static_cast<int>(dtype_size(a->dtype)) : 1;
+    const int ku = a->head_dim / per, vu = a->head_dim_value / per;
+    if (wide) SFB_CUDA(launch_dependent(evict_move_kernel<uint4>, grid, dim3(256), 0, s, p, ku, vu));
+    else if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(evict_move_kernel<uint32_t>, grid, dim3(256), 0, s, p, ku, vu));
+    else SFB_CUDA(launch_dependent(evict_move_kernel<uint16_t>, grid, dim3(256), 0, s, p, ku, vu));
+    return check_launch("evict_move");
+}
+
+sfb_status sfb_k_paged_kv_accept(const sfb_accept_args* a, sfb_stream stream) {
+    SFB_REQUIRE(a && a->draft_k && a->draft_v && a->start_len && a->path && a->path_len, "accept: null tensor");
+    SFB_TRY(check_cache(a->k_pool, a->v_pool, a->block_table, a->batch, a->kv_heads, a->head_dim, a->head_dim_value,
+                        a->block_tokens, a->max_blocks, a->num_blocks, a->dtype, "accept"));
+    SFB_REQUIRE(a->nodes > 0 && a->max_path > 0, "accept: no nodes or no path");
+    SFB_REQUIRE(a->new_len != a->start_len, "accept: new_len must not be start_len");
+    cudaStream_t s = as_stream(stream);
+    AcceptParams p{};
+    p.kv = make_view(a->k_pool, a->v_pool, a->block_table, a->start_len, a->kv_heads, a->head_dim, a->head_dim_value,
+                     a->block_tokens, a->max_blocks, a->num_blocks, a->max_blocks * a->block_tokens);
+    p.draft_k = a->draft_k; p.draft_v = a->draft_v; p.path = a->path; p.path_len = a->path_len; p.new_len = a->new_len;
+    p.nodes = a->nodes; p.max_path = a->max_path;
+    const dim3 grid(ceil_div(a->max_path, 8), a->kv_heads, a->batch);
+    const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool) &&
+                      aligned16(a->draft_k) && aligned16(a->draft_v);
+    const int per = wide ? 16 / static_cast<int>(dtype_size(a->dtype)) : 1;
+    const int ku = a->head_dim / per, vu = a->head_dim_value / per;
+    if (wide) SFB_CUDA(launch_dependent(accept_kernel<uint4>, grid, dim3(256), 0, s, p, ku, vu));
+    else if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(accept_kernel<uint32_t>, grid, dim3(256), 0, s, p, ku, vu));
+    else SFB_CUDA(launch_dependent(accept_kernel<uint16_t>, grid, dim3(256), 0, s, p, ku, vu));
+    return check_launch("paged_kv_accept");
+}
+
+}  // extern "C"

@@ -54,6 +54,55 @@ class DecodeArgs(C.Structure):
                [("scale", C.c_float), ("dtype", C.c_int), ("uniform_context", C.c_int)]
 
 
+class TreeArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k_pool", "v_pool", "block_table", "context_len", "draft_k", "draft_v", "parents",
+                                  "node_count", "out", "workspace")] + \
+               [(n, C.c_int) for n in ("batch", "q_heads", "kv_heads", "nodes", "head_dim", "head_dim_value",
+                                       "block_tokens", "max_blocks", "num_blocks", "max_context", "splits")] + \
+               [("scale", C.c_float), ("token_major", C.c_int), ("dtype", C.c_int)]
+
+
+class AcceptArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("draft_k", "draft_v", "k_pool", "v_pool", "block_table", "start_len", "path", "path_len",
+                                  "new_len")] + \
+               [(n, C.c_int) for n in ("batch", "kv_heads", "nodes", "max_path", "head_dim", "head_dim_value",
+                                       "block_tokens", "max_blocks", "num_blocks", "dtype")]
+
+
+class BoundsArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("k_pool", "bounds", "block_table", "start_len", "end_len")] + \
+               [(n, C.c_int) for n in ("batch", "kv_heads", "head_dim", "max_tokens", "block_tokens", "max_blocks",
+                                       "num_blocks", "dtype")]
+
+
+class SparseArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k_pool", "v_pool", "bounds", "block_table", "context_len", "out", "selected",
+                                  "workspace")] + \
+               [(n, C.c_int) for n in ("batch", "q_heads", "kv_heads", "head_dim", "head_dim_value", "block_tokens",
+                                       "max_blocks", "num_blocks", "max_context", "budget_blocks", "sink_blocks",
+                                       "recent_blocks", "splits")] + \
+               [("scale", C.c_float), ("dtype", C.c_int)]
+
+
+class WeightsArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k_pool", "v_pool", "block_table", "context_len", "out", "weights", "weights_out",
+                                  "positions", "query_position", "workspace")] + \
+               [(n, C.c_int) for n in ("batch", "q_heads", "kv_heads", "head_dim", "head_dim_value", "block_tokens",
+                                       "max_blocks", "num_blocks", "max_context", "weight_stride", "splits")] + \
+               [("scale", C.c_float), ("dtype", C.c_int)]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("k_pool", "v_pool", "block_table", "context_len", "weights", "weights_out", "positions",
+                                  "positions_out", "new_len", "workspace")] + \
+               [(n, C.c_int) for n in ("batch", "kv_heads", "head_dim", "head_dim_value", "block_tokens", "max_blocks",
+                                       "num_blocks", "max_context", "weight_stride", "budget", "sink_tokens",
+                                       "recent_tokens", "dtype")]
+
+
+MAX_TREE_NODES = 256
+
+
 class DecoderConfig(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("batch", "sequence", "hidden", "intermediate", "query_heads",
                                        "kv_heads", "head_dim")] + \
@@ -153,6 +202,9 @@ EXPORTS = (
     "sfb_rope_table sfb_k_rope_split sfb_k_attention_prefill "
     "sfb_attention_decode_workspace sfb_attention_decode_default_splits sfb_k_attention_decode_paged "
     "sfb_k_paged_kv_append sfb_k_paged_kv_gather "
+    "sfb_attention_tree_workspace sfb_k_attention_tree_paged sfb_k_paged_kv_accept sfb_k_paged_kv_bounds "
+    "sfb_attention_sparse_workspace sfb_k_attention_decode_sparse sfb_attention_weights_workspace "
+    "sfb_k_attention_decode_weights sfb_paged_kv_evict_workspace sfb_k_paged_kv_evict "
     "sfb_k_moe_route sfb_k_moe_dispatch sfb_moe_dispatch_scratch_bytes sfb_k_moe_dispatch_static sfb_k_moe_combine "
     "sfb_import_stablehlo sfb_import_stablehlo_dump "
     "sfb_decoder_compile sfb_decoder_destroy sfb_decoder_execute sfb_decoder_execute_rows sfb_decoder_upload_input "
@@ -202,7 +254,8 @@ def load():
     lib.sfb_tiled_weight_elems.restype = C.c_int64
     lib.sfb_decoder_compile_milliseconds.restype = C.c_double
     lib.sfb_benchmark_decoder_profile.argtypes = [vp, C.c_char_p, vp, C.c_uint64, C.c_uint64, C.c_int, C.c_int, vp]
-    for name in ("sfb_attention_decode_workspace", "sfb_moe_dispatch_scratch_bytes",
+    for name in ("sfb_attention_tree_workspace", "sfb_attention_sparse_workspace", "sfb_attention_weights_workspace",
+                 "sfb_paged_kv_evict_workspace", "sfb_attention_decode_workspace", "sfb_moe_dispatch_scratch_bytes",
                  "sfb_decoder_workspace_bytes", "sfb_gemm_stream_workspace_bytes", "sfb_decoder_peer_bytes"):
         if hasattr(lib, name):
             getattr(lib, name).restype = C.c_size_t
