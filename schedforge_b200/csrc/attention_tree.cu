@@ -278,14 +278,18 @@ extern "C" {
 
 size_t sfb_attention_tree_workspace(const sfb_tree_args* a) {
     if (check_tree(a) != SFB_OK) return 0;
-    return tree_layout(*a).total;
+    const size_t simt = tree_layout(*a).total;
+    if (!tree_tcgen05_supported(*a)) return simt;
+    const size_t tensor = tree_tcgen05_workspace(*a);   // (pointers that are not 16-byte aligned take the other kernel)
+    return tensor > simt ? tensor : simt;
 }
 
 sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* a, sfb_stream stream) {
     SFB_TRY(check_tree(a));
     SFB_REQUIRE(a->q && a->context_len && a->draft_k && a->draft_v && a->parents && a->out, "tree attention: null tensor");
     const TreeLayout l = tree_layout(*a);
-    SFB_REQUIRE(l.total == 0 || (a->workspace && aligned16(a->workspace)), "tree attention: the workspace is missing or not 16-byte aligned");
+    const bool tensor = tree_tcgen05_supported(*a);
+    SFB_REQUIRE((l.total == 0 && !tensor) || (a->workspace && aligned16(a->workspace)), "tree attention: the workspace is missing or not 16-byte aligned");
     cudaStream_t s = as_stream(stream);
     TreeParams p{};
     p.kv = make_view(a->k_pool, a->v_pool, a->block_table, a->context_len, a->kv_heads, a->head_dim, a->head_dim_value,
@@ -296,6 +300,7 @@ sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* a, sfb_stream stream)
     p.splits = l.splits; p.chunk = l.chunk;
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
     p.vec = a->head_dim % 4 == 0 && a->head_dim_value % 4 == 0 && aligned16(a->q) && aligned16(a->k_pool) && aligned16(a->v_pool);
+    if (tensor) return tree_tcgen05(*a, p, s);
     SFB_TRY(a->dtype == SFB_F32 ? tree_simt<float>(p, s) : tree_simt<bf16>(p, s));
     if (l.splits == 1) return SFB_OK;
     return merge_partials({p.partials, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, l.splits, a->token_major},

@@ -15,6 +15,11 @@ struct TreeParams {
     float scale_log2;
 };
 
+// bf16, head_dim = head_dim_value = 128 or 64 (attention_tree_tcgen05.cu).
+bool tree_tcgen05_supported(const sfb_tree_args& a);
+size_t tree_tcgen05_workspace(const sfb_tree_args& a);
+sfb_status tree_tcgen05(const sfb_tree_args& a, const TreeParams& t, cudaStream_t stream);
+
 #ifdef __CUDACC__
 __device__ __forceinline__ int tree_node_count(const TreeParams& p, int b) {
     if (!p.node_count) return p.nodes;

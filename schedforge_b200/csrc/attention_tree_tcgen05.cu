@@ -1,0 +1,699 @@
+// Tree attention on the 5th-generation tensor cores (bf16, head_dim = head_dim_value = 128 or 64, blocks of a multiple
+// of eight tokens).
+//
+// The query rows of one (sequence, K/V head) - the group's heads times the nodes - are the M dimension: 128 rows fill
+// an MMA tile however few are live, which costs nothing while the K/V bytes bound the time (a 128-key tile of K and V
+// is 64 KB, 1.45 us of one SM's share of the HBM rate; its two products take 0.55 us of the tensor pipe).
+// Keys are walked in tiles of 128: the committed positions (gathered from the pool by TMA, one box per run of
+// tokens inside a block), then the drafted nodes (their own tensors; a row's ancestors as bits).
+//
+// Work is cut evenly: the tiles of all (sequence, K/V head, row group) pairs are laid end to end and every CTA takes
+// one equal range, so ragged contexts leave no SM idle.  A pair that lies in one CTA writes its output
+// directly; the pieces of a pair that was cut are kept as (maximum, sum, numerator) and joined by a second kernel.
+//
+// 384 threads, roles as in the prefill kernel: two softmax groups of 128 threads (thread = row = tensor-memory lane),
+// one copy warp, one MMA-issuing thread; S and P share tensor memory columns, P is the A operand of P.V.
+//   ROWS = 256: the two groups own two 128-row tiles and meet every key tile;
+//   ROWS = 128: both own the same rows and take alternate key tiles, each with its own running maximum and
+//               accumulator; the first group joins them at the end of a piece, out of tensor memory.
+// Positions past the context in a loaded block may hold anything: their scores are masked and their V rows are zeroed
+// in shared memory before the product (0 * NaN).  Warps without a live row skip the arithmetic.  Waits are bounded.
+#include "attention_tree.cuh"
+#include "ptx_sm100.cuh"
+
+namespace sfb {
+namespace {
+
+constexpr int KT = 128;
+constexpr int kThreads = 384;
+constexpr int kHalfBytes = KT * 64 * 2;
+constexpr uint32_t kTmemCols = 512;   // S_t (P_t over its first half) at t * 128, O_t at 256 + t * D
+constexpr uint32_t kOCol = 256;
+constexpr uint32_t kCodeTree = 0x80;
+constexpr float kRescaleThreshold = 8.0F;  // log2 units
+constexpr int kBadRing = 16;
+
+template <int D, int ROWS>
+struct Shape {
+    static constexpr int kHalves = D / 64;
+    static constexpr int kQTiles = ROWS / 128;
+    static constexpr int kQBytes = kHalves * kHalfBytes;   // one 128-row tile
+    static constexpr int kTileBytes = kHalves * kHalfBytes;
+    static constexpr int kStages = D == 64 ? 5 : (ROWS == 128 ? 3 : 2);
+    static constexpr int kParentBytes = 2 * SFB_MAX_TREE_NODES;
+    static constexpr int kSmemBytes = kQTiles * kQBytes + 2 * kStages * kTileBytes + kParentBytes + 128 * 8 + 512 + 1024;
+};
+
+struct TreeTcParams {
+    TreeParams t;
+    int rows_all, row_groups, box_rows;
+    int64_t pairs;
+    int pool_rows;
+    float* part_o;          // [grid + pairs][ROWS][D]
+    float2* part_ml;        // [grid + pairs][ROWS]
+    int2* pair_span;        // [pairs]: first and last CTA
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ int tiles_of(int ctx, int count) {
+    return count > 0 ? (ctx + KT - 1) / KT + (count + KT - 1) / KT : 0;
+}
+
+// Position of a role in the CTA's range of tiles.
+struct Walk {
+    int b, sub, x, ctx, count, tiles;  // sub = kvh * row_groups + row group
+    int64_t left;
+
+    __device__ __forceinline__ void read(const TreeTcParams& p) {
+        ctx = p.t.kv.length(b);
+        count = tree_node_count(p.t, b);
+        tiles = tiles_of(ctx, count);
+    }
+    __device__ __forceinline__ int take() const { return static_cast<int>(left < tiles - x ? left : tiles - x); }
+    __device__ __forceinline__ void advance(const TreeTcParams& p, int n) {
+        left -= n;
+        x += n;
+        if (x < tiles || left <= 0) return;
+        x = 0;
+        if (++sub < p.t.kv.kv_heads * p.row_groups) return;
+        sub = 0;
+        do {
+            if (++b >= p.t.batch) { left = 0; return; }
+            read(p);
+        } while (tiles == 0);
+    }
+};
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
+                    const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ TreeTcParams p) {
+    using Sh = Shape<D, ROWS>;
+    constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kTileBytes = Sh::kTileBytes;
+    constexpr bool kTwoTiles = ROWS == 256;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_smem = smem;
+    uint8_t* k_smem = q_smem + Sh::kQTiles * Sh::kQBytes;
+    uint8_t* v_smem = k_smem + kStages * kTileBytes;
+    uint8_t* parent_smem = v_smem + kStages * kTileBytes;                           // [2][256], 255 = no parent
+    float2* ml_smem = reinterpret_cast<float2*>(parent_smem + Sh::kParentBytes);    // [128]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ml_smem + 128);
+    uint64_t* q_full = bars;
+    uint64_t* q_empty = bars + 1;
+    uint64_t* s_full = bars + 2;     // [2]
+    uint64_t* p_full = bars + 4;     // [2]
+    uint64_t* o_full = bars + 6;     // [2]
+    uint64_t* par_full = bars + 8;   // [2]
+    uint64_t* ml_full = bars + 10;   // group 1's maxima and sums are in shared memory
+    uint64_t* o_free = bars + 11;    // group 0 has read group 1's accumulator
+    uint64_t* k_full = bars + 12;
+    uint64_t* k_empty = k_full + kStages;
+    uint64_t* v_full = k_empty + kStages;
+    uint64_t* v_empty = v_full + kStages;
+    uint32_t* words = reinterpret_cast<uint32_t*>(v_empty + kStages);
+    uint32_t* tmem_slot = words;
+    volatile uint32_t* abort_flag = words + 1;
+    int* start = reinterpret_cast<int*>(words + 2);   // b, sub, x, tiles in the range
+    volatile uint32_t* bad = words + 6;               // [kBadRing], runs of eight keys without a block
+    const TreeParams& t_ = p.t;
+    const PagedView& kv = t_.kv;
+    uint32_t* status = kv.status;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(ptx::smem_u32(q_full), 1);
+        ptx::mbar_init(ptx::smem_u32(q_empty), 1);
+        for (int t = 0; t < 2; ++t) {
+            ptx::mbar_init(ptx::smem_u32(&s_full[t]), 1);
+            ptx::mbar_init(ptx::smem_u32(&p_full[t]), 128);
+            ptx::mbar_init(ptx::smem_u32(&o_full[t]), 1);
+            ptx::mbar_init(ptx::smem_u32(&par_full[t]), 128);
+        }
+        ptx::mbar_init(ptx::smem_u32(ml_full), 128);
+        ptx::mbar_init(ptx::smem_u32(o_free), 128);
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&k_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&k_empty[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&v_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&v_empty[s]), 1);
+        }
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async();
+        ptx::prefetch_tensormap(&map_q);
+        ptx::prefetch_tensormap(&map_k);
+        ptx::prefetch_tensormap(&map_v);
+        ptx::prefetch_tensormap(&map_dk);
+        ptx::prefetch_tensormap(&map_dv);
+    }
+    if (warp == 9) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    if (warp == 10) {
+        // this CTA's range of the tile list
+        const int64_t subs = static_cast<int64_t>(kv.kv_heads) * p.row_groups;
+        int64_t total = 0;
+        for (int b0 = 0; b0 < t_.batch; b0 += 32) {
+            const int b = b0 + lane;
+            int n = b < t_.batch ? tiles_of(kv.length(b), tree_node_count(t_, b)) : 0;
+            total += __reduce_add_sync(0xffffffffu, n);
+        }
+        total *= subs;
+        int64_t per = (total + gridDim.x - 1) / gridDim.x;
+        if (per < 1) per = 1;
+        const int64_t first = blockIdx.x * per;
+        const int64_t mine = first < total ? (total - first < per ? total - first : per) : 0;
+        int64_t before = 0;
+        if (mine > 0) {
+            for (int b0 = 0; b0 < t_.batch; b0 += 32) {
+                const int b = b0 + lane;
+                const int n = b < t_.batch ? tiles_of(kv.length(b), tree_node_count(t_, b)) : 0;
+                int sum = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += v;
+                }
+                const int64_t end = before + sum * subs, begin = end - n * subs;
+                const bool here = n > 0 && begin <= first && first < end;
+                if (here) {
+                    const int64_t off = first - begin;
+                    start[0] = b;
+                    start[1] = static_cast<int>(off / n);
+                    start[2] = static_cast<int>(off % n);
+                }
+                if (__any_sync(0xffffffffu, here)) break;
+                before += __shfl_sync(0xffffffffu, sum, 31) * subs;
+            }
+        }
+        if (lane == 0) start[3] = static_cast<int>(mine);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    Walk w{};
+    w.left = start[3];
+    if (w.left > 0) {
+        w.b = start[0]; w.sub = start[1]; w.x = start[2];
+        w.read(p);
+    }
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // ------------------------------------------------------------ copies
+            const int boxes = KT / p.box_rows;
+            const int box = lane / kHalves, half = lane % kHalves;
+            const uint32_t box_bits = (p.box_rows == 128 ? 0xffffu : ((1u << (p.box_rows / 8)) - 1));
+            uint32_t n_kv = 0, n_seg = 0;
+            bool ok = true;
+            while (ok && w.left > 0) {
+                const int n = w.take();
+                const int kvh = w.sub / p.row_groups, rg = w.sub % p.row_groups;
+                const int n_ctx = (w.ctx + KT - 1) / KT;
+                const int head = w.b * kv.kv_heads + kvh;
+                const int* table = kv.table + static_cast<size_t>(w.b) * kv.max_blocks;
+                const auto row_of = [&](int x) -> int {   // pool row of this lane's box in context tile x, -1: no block, -2: nothing to load
+                    const int pos = x * KT + box * p.box_rows;
+                    if (x >= n_ctx || box >= boxes || pos >= w.ctx) return -2;
+                    const int block = kv.block_of(pos);
+                    const int page = table[block];
+                    return page < 0 || page >= kv.num_blocks ? -1
+                                                             : (page * kv.kv_heads + kvh) * kv.block_tokens + (pos - block * kv.block_tokens);
+                };
+                int row = row_of(w.x);
+                ok = ptx::mbar_wait(ptx::smem_u32(q_empty), (n_seg & 1) ^ 1, abort_flag, status, kCodeTree | 1);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (lane == 0) {
+                    const uint32_t bar = ptx::smem_u32(q_full);
+                    ptx::mbar_expect_tx(bar, Sh::kQTiles * Sh::kQBytes);
+                    const int q_row = head * p.rows_all + rg * ROWS;
+                    for (int i = 0; i < Sh::kQTiles; ++i)
+                        for (int h = 0; h < kHalves; ++h)
+                            ptx::tma_load_2d(ptx::smem_u32(q_smem + i * Sh::kQBytes + h * kHalfBytes), &map_q, bar, 64 * h, q_row + 128 * i);
+                }
+                ++n_seg;
+                for (int x = w.x; ok && x < w.x + n; ++x, ++n_kv) {
+                    const int s = n_kv % kStages;
+                    const uint32_t parity = ((n_kv / kStages) & 1) ^ 1;
+                    const int mine = row;
+                    row = x + 1 < w.x + n ? row_of(x + 1) : -2;    // in flight while this tile waits for its stage
+                    const bool draft = x >= n_ctx;
+                    const uint32_t missing = __reduce_or_sync(0xffffffffu, mine == -1 ? box_bits << (box * (p.box_rows / 8)) : 0u);
+                    const uint32_t loaded = __popc(__ballot_sync(0xffffffffu, mine > -2)) * (p.box_rows * 128);
+                    if (missing && lane == 0) atomicOr(status, kCodeDecodeBounds);
+                    const int src = mine == -1 ? p.pool_rows : mine;   // outside the tensor map: reads zeros
+#pragma unroll
+                    for (int kvi = 0; kvi < 2; ++kvi) {
+                        uint64_t* empty = kvi ? v_empty : k_empty;
+                        uint64_t* full = kvi ? v_full : k_full;
+                        uint8_t* stage = (kvi ? v_smem : k_smem) + s * kTileBytes;
+                        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty[s]), parity, abort_flag, status, kCodeTree | 1);
+                        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+                        const uint32_t bar = ptx::smem_u32(&full[s]);
+                        if (lane == 0) {
+                            if (!kvi) bad[n_kv % kBadRing] = missing;
+                            ptx::mbar_expect_tx(bar, draft ? kTileBytes : loaded);
+                        }
+                        __syncwarp();
+                        if (draft) {
+                            if (lane < kHalves)
+                                ptx::tma_load_3d(ptx::smem_u32(stage + lane * kHalfBytes), kvi ? &map_dv : &map_dk, bar, 64 * lane, (x - n_ctx) * KT, head);
+                        } else if (mine > -2) {
+                            ptx::tma_load_2d(ptx::smem_u32(stage + half * kHalfBytes + box * p.box_rows * 128), kvi ? &map_v : &map_k, bar, 64 * half, src);
+                        }
+                    }
+                }
+                w.advance(p, n);
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ MMA issue
+            if (lane == 0) {
+                constexpr uint32_t idesc_qk = ptx::umma_idesc_bf16(128, KT, 0, 0);
+                constexpr uint32_t idesc_pv = ptx::umma_idesc_bf16(128, D, 0, 1);
+                uint32_t n_kv = 0, n_seg = 0, n_slot[2] = {0, 0};   // tiles, pieces and slot uses so far
+                bool ok = true;
+                while (ok && w.left > 0) {
+                    const int n = w.take();
+                    const int items = kTwoTiles ? 2 * n : n;
+                    ok = ptx::mbar_wait(ptx::smem_u32(q_full), n_seg & 1, abort_flag, status, kCodeTree | 2);
+                    if (!ok) break;
+                    // S_t = Q . K_j^T for item i (tile j, slot t)
+                    const auto issue_qk = [&](int i) -> bool {
+                        const int t = i & 1, j = kTwoTiles ? i >> 1 : i;
+                        const uint32_t g = n_kv + j;
+                        if (!ptx::mbar_wait(ptx::smem_u32(&k_full[g % kStages]), (g / kStages) & 1, abort_flag, status, kCodeTree | 2)) return false;
+                        ptx::tc_fence_after();
+                        const uint32_t qa = ptx::smem_u32(q_smem + (kTwoTiles ? t : 0) * Sh::kQBytes);
+                        const uint32_t ka = ptx::smem_u32(k_smem + (g % kStages) * kTileBytes);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = (kk / 4) * kHalfBytes + (kk % 4) * 32;
+                            ptx::umma_bf16(tmem_base + t * KT, ptx::umma_desc_k_sw128(qa + off), ptx::umma_desc_k_sw128(ka + off), idesc_qk, kk != 0);
+                        }
+                        ptx::umma_commit(ptx::smem_u32(&s_full[t]));
+                        if (!kTwoTiles || t == 1) ptx::umma_commit(ptx::smem_u32(&k_empty[g % kStages]));
+                        if (i == items - 1) ptx::umma_commit(ptx::smem_u32(q_empty));
+                        return true;
+                    };
+                    for (int i = 0; ok && i < 2 && i < items; ++i) ok = issue_qk(i);
+                    for (int i = 0; ok && i < items; ++i) {
+                        const int t = i & 1, j = kTwoTiles ? i >> 1 : i;
+                        const uint32_t g = n_kv + j;
+                        ok = ptx::mbar_wait(ptx::smem_u32(&p_full[t]), n_slot[t] & 1, abort_flag, status, kCodeTree | 2) &&
+                             ptx::mbar_wait(ptx::smem_u32(&v_full[g % kStages]), (g / kStages) & 1, abort_flag, status, kCodeTree | 2);
+                        if (!ok) break;
+                        ++n_slot[t];
+                        ptx::tc_fence_after();
+                        const uint32_t va = ptx::smem_u32(v_smem + (g % kStages) * kTileBytes);
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; ++kk)   // O_t += P_t . V_j
+                            ptx::umma_bf16_ts(tmem_base + kOCol + t * D, tmem_base + t * KT + kk * 8,
+                                              ptx::umma_desc_mn_sw128(va + kk * 16 * 128, kHalfBytes, 1024), idesc_pv, (i >> 1 | kk) != 0);
+                        if (!kTwoTiles || t == 1) ptx::umma_commit(ptx::smem_u32(&v_empty[g % kStages]));
+                        if (i + 2 >= items) ptx::umma_commit(ptx::smem_u32(&o_full[t]));
+                        // the tensor pipe runs in order: P_t is consumed before S_t is overwritten
+                        if (i + 2 < items) ok = issue_qk(i + 2);
+                    }
+                    n_kv += n;
+                    ++n_seg;
+                    w.advance(p, n);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // ---------------------------------------------------------------- softmax groups
+        const int t = warp >> 2;
+        const int quarter = warp & 3;
+        const int r = quarter * 32 + lane;                       // tensor-memory lane
+        const int tile_row = (kTwoTiles ? t * 128 : 0) + r;      // row inside the row group
+        const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_addr = tmem_base + lane_base + t * KT;
+        const uint32_t o_addr = tmem_base + lane_base + kOCol + t * D;
+        uint8_t* parent = parent_smem + t * SFB_MAX_TREE_NODES;
+        uint32_t n_kv = 0, n_slot = 0, n_out = 0, n_seg = 0, n_par = 0;
+        bool ok = true;
+        while (ok && w.left > 0) {
+            const int n = w.take();
+            const int kvh = w.sub / p.row_groups, rg = w.sub % p.row_groups;
+            const int n_ctx = (w.ctx + KT - 1) / KT;
+            const int row = rg * ROWS + tile_row;                // query row of the pair
+            const int node = row % t_.nodes;
+            const bool live_row = row < p.rows_all && node < w.count;
+            const bool live_warp = __any_sync(0xffffffffu, live_row);
+            float m_used = -INFINITY, row_sum = 0.0F;
+            int used = 0;
+            for (int j = kTwoTiles ? 0 : t; ok && j < n; j += kTwoTiles ? 1 : 2, ++used) {
+                const int x = w.x + j;
+                const uint32_t g = n_kv + j;
+                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[t]), n_slot & 1, abort_flag, status, kCodeTree | 4);
+                if (!ok) break;
+                ++n_slot;
+                ptx::tc_fence_after();
+                const bool draft = x >= n_ctx;
+                const int key0 = draft ? (x - n_ctx) * KT : x * KT;
+                const int live = min(KT, (draft ? w.count : w.ctx) - key0);
+                uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                bool masked = live < KT;
+                if (draft) {
+                    masked = true;
+                    for (int i = r; i < w.count; i += 128) {
+                        int up = t_.parents[static_cast<size_t>(w.b) * t_.nodes + i];
+                        if (up < -1 || up >= i) {
+                            up = -1;
+                            atomicOr(status, kCodeDecodeBounds);
+                        }
+                        parent[i] = static_cast<uint8_t>(up);   // (-1 becomes 255; a parent is at most 254)
+                    }
+                    ptx::mbar_arrive(ptx::smem_u32(&par_full[t]));
+                    ok = ptx::mbar_wait(ptx::smem_u32(&par_full[t]), n_par & 1, abort_flag, status, kCodeTree | 4);
+                    if (!ok) break;
+                    ++n_par;
+                    see[0] = see[1] = see[2] = see[3] = 0u;
+                    for (int i = live_row ? node : -1; i >= 0;) {
+                        const int at = i - key0;
+                        if (at >= 0 && at < KT) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                if (at >> 5 == q) see[q] |= 1u << (at & 31);
+                        }
+                        const int up = parent[i];
+                        i = up == 255 ? -1 : up;
+                    }
+                } else {
+                    const uint32_t missing = bad[g % kBadRing];
+                    if (live < KT || missing) {
+                        masked = true;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int left = live - 32 * q;
+                            uint32_t bits = left >= 32 ? 0xffffffffu : (left > 0 ? (1u << left) - 1 : 0u);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                if (missing >> (4 * q + u) & 1u) bits &= ~(0xffu << (8 * u));
+                            see[q] = bits;
+                        }
+                    }
+                }
+                if (live < KT) {
+                    // rows of V past the live keys: whatever the block (or the stage) holds becomes zero
+                    ok = ptx::mbar_wait(ptx::smem_u32(&v_full[g % kStages]), (g / kStages) & 1, abort_flag, status, kCodeTree | 4);
+                    if (!ok) break;
+                    uint8_t* v_tile = v_smem + (g % kStages) * kTileBytes;
+                    for (int i = r; i < (KT - live) * 8 * kHalves; i += 128) {
+                        const int piece = i & 7, half = (i >> 3) % kHalves, dead = live + (i >> 3) / kHalves;
+                        *reinterpret_cast<uint4*>(v_tile + half * kHalfBytes + dead * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    ptx::fence_proxy_async();
+                }
+                if (live_warp) {
+                    uint32_t raw[KT / 32][32];
+                    ptx::tmem_ld_32x32(s_addr, raw[0]);
+                    ptx::tmem_ld_32x32(s_addr + 32, raw[1]);
+                    ptx::tmem_ld_32x32(s_addr + 64, raw[2]);
+                    ptx::tmem_ld_32x32(s_addr + 96, raw[3]);
+                    ptx::tmem_ld_wait();
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!(see[c] >> i & 1u)) raw[c][i] = 0xff800000u;  // -inf, and 2^-inf = 0 below
+                    }
+                    float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            const uint32_t* v = &raw[c][i];
+                            mx0 = max3(mx0, __uint_as_float(v[0]), __uint_as_float(v[1]));
+                            mx1 = max3(mx1, __uint_as_float(v[2]), __uint_as_float(v[3]));
+                            mx2 = max3(mx2, __uint_as_float(v[4]), __uint_as_float(v[5]));
+                            mx3 = max3(mx3, __uint_as_float(v[6]), __uint_as_float(v[7]));
+                        }
+                    const float tile_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * t_.scale_log2;
+                    // lazy running maximum: O_t is only touched when it outgrows the one in use by 2^8; every earlier
+                    // product of this slot has finished when S_t is complete
+                    const bool grow = tile_max > m_used + kRescaleThreshold;
+                    if (used > 0 && __any_sync(0xffffffffu, grow)) {
+                        const float alpha = grow ? exp2_fast(m_used - tile_max) : 1.0F;
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            ptx::tmem_ld_32x32(o_addr + c * 32, o);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            ptx::tmem_st_32x32(o_addr + c * 32, o);
+                        }
+                        ptx::tmem_st_wait();
+                        row_sum *= alpha;
+                    }
+                    if (grow) m_used = tile_max;
+                    const float neg_m = m_used == -INFINITY ? 0.0F : -m_used;
+                    float s0 = 0.0F, s1 = 0.0F, s2 = 0.0F, s3 = 0.0F;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float x0 = exp2_fast(fmaf(__uint_as_float(raw[c][i]), t_.scale_log2, neg_m));
+                            const float x1 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 1]), t_.scale_log2, neg_m));
+                            const float x2 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 2]), t_.scale_log2, neg_m));
+                            const float x3 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 3]), t_.scale_log2, neg_m));
+                            s0 += x0; s1 += x1; s2 += x2; s3 += x3;
+                            // the weights are rounded to bf16 for the product; the row sum keeps 32 bits
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(x0, x1), hi = __floats2bfloat162_rn(x2, x3);
+                            packed[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
+                            packed[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+                        }
+                        ptx::tmem_st_32x16(s_addr + c * 16, packed);
+                    }
+                    ptx::tmem_st_wait();
+                    row_sum += (s0 + s1) + (s2 + s3);
+                }
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(ptx::smem_u32(&p_full[t]));
+            }
+            if (ok && used > 0) {
+                ok = ptx::mbar_wait(ptx::smem_u32(&o_full[t]), n_out & 1, abort_flag, status, kCodeTree | 4);
+                ++n_out;
+                ptx::tc_fence_after();
+            }
+            if (!ok) break;
+            // ---- the piece's result
+            float f0 = 1.0F, f1 = 0.0F;     // factors of this group's and (ROWS == 128) the other group's accumulator
+            if constexpr (!kTwoTiles) {
+                if (t == 1) {
+                    ml_smem[r] = make_float2(m_used, row_sum);
+                    ptx::mbar_arrive(ptx::smem_u32(ml_full));
+                    ok = ptx::mbar_wait(ptx::smem_u32(o_free), n_seg & 1, abort_flag, status, kCodeTree | 4);
+                } else {
+                    ok = ptx::mbar_wait(ptx::smem_u32(ml_full), n_seg & 1, abort_flag, status, kCodeTree | 4);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const float2 other = ml_smem[r];
+                    const float top = fmaxf(m_used, other.x);
+                    f0 = m_used == -INFINITY ? 0.0F : exp2_fast(m_used - top);
+                    f1 = other.x == -INFINITY ? 0.0F : exp2_fast(other.x - top);
+                    row_sum = row_sum * f0 + other.y * f1;
+                    m_used = top;
+                }
+                if (!ok) break;
+            }
+            const bool whole = w.x == 0 && n == w.tiles;
+            const int64_t pair = static_cast<int64_t>(w.b) * kv.kv_heads * p.row_groups + w.sub;
+            if ((kTwoTiles || t == 0) && live_warp) {
+                const float inv = whole ? (row_sum > 0.0F ? 1.0F / row_sum : 0.0F) : 1.0F;
+                f0 *= inv;
+                f1 *= inv;
+                const bool second = !kTwoTiles && n > 1;
+                const int64_t piece = static_cast<int64_t>(blockIdx.x) + pair;
+                bf16* dst = static_cast<bf16*>(t_.out) +
+                            tree_out_row(t_, w.b, kvh * (t_.q_heads / kv.kv_heads) + row / t_.nodes, node) * D;
+                float* part = p.part_o + (piece * ROWS + tile_row) * D;
+                if (!whole && live_row) p.part_ml[piece * ROWS + tile_row] = make_float2(m_used, row_sum);
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32], o2[32];
+                    ptx::tmem_ld_32x32(o_addr + c * 32, o);
+                    if (second) ptx::tmem_ld_32x32(o_addr + D + c * 32, o2);
+                    ptx::tmem_ld_wait();
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        v[i] = __uint_as_float(o[i]) * f0;
+                        if (second && f1 != 0.0F) v[i] = fmaf(__uint_as_float(o2[i]), f1, v[i]);
+                    }
+                    if (!live_row) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 packed;
+                            __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
+                            reinterpret_cast<uint4*>(dst + c * 32)[i] = packed;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            reinterpret_cast<float4*>(part + c * 32)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    }
+                }
+            }
+            if (!kTwoTiles && t == 0) {
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(ptx::smem_u32(o_free));
+            }
+            if (threadIdx.x == 0 && w.x == 0) {   // (one thread per pair: the owner of its first tile)
+                // the range length is the same for all CTAs but the last, so the last CTA of the pair follows from it
+                const int64_t per = start[3];
+                const int64_t beyond = w.tiles - n;
+                p.pair_span[pair] = make_int2(blockIdx.x, static_cast<int>(blockIdx.x + (beyond + per - 1) / per));
+            }
+            n_kv += n;
+            ++n_seg;
+            w.advance(p, n);
+        }
+    }
+
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (*abort_flag)
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight land before the CTA leaves
+    if (warp == 9) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// Joins the pieces of pairs that were cut: one warp per query row.
+template <int D>
+__global__ void __launch_bounds__(256)
+tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
+    constexpr int V = D / 32;
+    const TreeParams& t = p.t;
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const int slices = rows_cta / 8;
+    const int64_t pair = blockIdx.x / slices;
+    const int tile_row = (blockIdx.x % slices) * 8 + (threadIdx.x >> 5);
+    const int subs = t.kv.kv_heads * p.row_groups;
+    const int b = static_cast<int>(pair / subs), sub = static_cast<int>(pair % subs);
+    const int kvh = sub / p.row_groups, rg = sub % p.row_groups;
+    const int row = rg * rows_cta + tile_row, node = row % t.nodes;
+    if (row >= p.rows_all || node >= tree_node_count(t, b)) return;
+    const int2 span = p.pair_span[pair];
+    if (span.x == span.y) return;   // written by the attention kernel itself
+    float top = -INFINITY;
+    for (int c = span.x; c <= span.y; ++c) top = fmaxf(top, p.part_ml[(c + pair) * rows_cta + tile_row].x);
+    float sum = 0.0F, acc[V] = {};
+    for (int c = span.x; c <= span.y; ++c) {
+        const float2 ml = p.part_ml[(c + pair) * rows_cta + tile_row];
+        if (ml.x == -INFINITY) continue;
+        const float f = exp2_fast(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        const float* part = p.part_o + ((c + pair) * rows_cta + tile_row) * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(part + i);
+            acc[i] = fmaf(v.x, f, acc[i]);
+            acc[i + 1] = fmaf(v.y, f, acc[i + 1]);
+        }
+    }
+    const float inv = sum > 0.0F ? 1.0F / sum : 0.0F;
+    bf16* dst = static_cast<bf16*>(t.out) + tree_out_row(t, b, kvh * (t.q_heads / t.kv.kv_heads) + row / t.nodes, node) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<__nv_bfloat162*>(dst + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+}
+
+struct TcLayout {
+    int rows_all, rows_cta, row_groups, grid;
+    int64_t pairs;
+    size_t ml, span, total;   // part_o first
+};
+
+TcLayout tc_layout(const sfb_tree_args& a) {
+    TcLayout l{};
+    l.rows_all = a.q_heads / a.kv_heads * a.nodes;
+    l.rows_cta = l.rows_all <= 128 ? 128 : 256;
+    l.row_groups = ceil_div(l.rows_all, l.rows_cta);
+    l.pairs = static_cast<int64_t>(a.batch) * a.kv_heads * l.row_groups;
+    const int covered = a.max_blocks * a.block_tokens;
+    const int limit = a.max_context < covered ? a.max_context : covered;
+    const int64_t most = l.pairs * (ceil_div(limit, KT) + ceil_div(a.nodes, KT));
+    int ctas = sm_count();
+    if (a.splits > 0 && l.pairs * a.splits < ctas) ctas = static_cast<int>(l.pairs * a.splits);
+    l.grid = static_cast<int>(most < ctas ? most : ctas);
+    const size_t pieces = static_cast<size_t>(l.grid + l.pairs);
+    l.ml = sizeof(float) * pieces * l.rows_cta * a.head_dim;
+    l.span = l.ml + sizeof(float2) * pieces * l.rows_cta;
+    l.total = l.span + sizeof(int2) * static_cast<size_t>(l.pairs);
+    return l;
+}
+
+template <int D, int ROWS>
+sfb_status launch_tc(const sfb_tree_args& a, const TcLayout& l, TreeTcParams& p, cudaStream_t stream) {
+    CUtensorMap mq, mk, mv, mdk, mdv;
+    const uint64_t heads = static_cast<uint64_t>(a.batch) * a.kv_heads;
+    if (!encode_tensor_map_bf16_2d(&mq, a.q, heads * l.rows_all, D, 128, 64) ||
+        !encode_tensor_map_bf16_2d(&mk, a.k_pool, p.pool_rows, D, p.box_rows, 64) ||
+        !encode_tensor_map_bf16_2d(&mv, a.v_pool, p.pool_rows, D, p.box_rows, 64) ||
+        !encode_tensor_map_bf16_3d(&mdk, a.draft_k, D, a.nodes, heads, D, static_cast<uint64_t>(a.nodes) * D, 64, KT, 1) ||
+        !encode_tensor_map_bf16_3d(&mdv, a.draft_v, D, a.nodes, heads, D, static_cast<uint64_t>(a.nodes) * D, 64, KT, 1))
+        return SFB_CUDA_ERROR;
+    constexpr int smem = Shape<D, ROWS>::kSmemBytes;
+    static_assert(smem <= 227 * 1024, "shared memory of one SM");
+    SFB_CUDA(cudaFuncSetAttribute(tree_tcgen05_kernel<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    SFB_CUDA(launch_dependent(tree_tcgen05_kernel<D, ROWS>, dim3(l.grid), dim3(kThreads), smem, stream, mq, mk, mv, mdk, mdv, p));
+    SFB_TRY(check_launch("attention_tree_tcgen05"));
+    SFB_CUDA(launch_dependent(tree_join_kernel<D>, dim3(static_cast<unsigned>(l.pairs * (ROWS / 8))), dim3(256), 0, stream, p, ROWS));
+    return check_launch("attention_tree_join");
+}
+
+}  // namespace
+
+bool tree_tcgen05_supported(const sfb_tree_args& a) {
+    const int64_t pool_rows = static_cast<int64_t>(a.num_blocks) * a.kv_heads * a.block_tokens;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.nodes;
+    return a.dtype == SFB_BF16 && (a.head_dim == 128 || a.head_dim == 64) && a.head_dim_value == a.head_dim &&
+           a.block_tokens % 8 == 0 && pool_rows < (int64_t{1} << 30) && rows < (int64_t{1} << 26) && aligned16(a.q) &&
+           aligned16(a.k_pool) && aligned16(a.v_pool) && aligned16(a.draft_k) && aligned16(a.draft_v) && aligned16(a.out);
+}
+
+// (by type, sizes and layout alone: the size is asked for before the addresses are known)
+size_t tree_tcgen05_workspace(const sfb_tree_args& a) { return tc_layout(a).total; }
+
+sfb_status tree_tcgen05(const sfb_tree_args& a, const TreeParams& t, cudaStream_t stream) {
+    const TcLayout l = tc_layout(a);
+    TreeTcParams p{};
+    p.t = t;
+    p.rows_all = l.rows_all; p.row_groups = l.row_groups; p.pairs = l.pairs;
+    p.box_rows = 8;
+    while (p.box_rows < 128 && a.block_tokens % (2 * p.box_rows) == 0) p.box_rows *= 2;
+    p.pool_rows = a.num_blocks * a.kv_heads * a.block_tokens;
+    char* ws = static_cast<char*>(a.workspace);
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + l.ml);
+    p.pair_span = reinterpret_cast<int2*>(ws + l.span);
+    if (a.head_dim == 128)
+        return l.rows_cta == 128 ? launch_tc<128, 128>(a, l, p, stream) : launch_tc<128, 256>(a, l, p, stream);
+    return l.rows_cta == 128 ? launch_tc<64, 128>(a, l, p, stream) : launch_tc<64, 256>(a, l, p, stream);
+}
+
+}  // namespace sfb

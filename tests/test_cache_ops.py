@@ -673,7 +673,7 @@ def test_workspace_sizes_need_no_device(sfb):
     s.kv_heads = 2
     assert lib.sfb_attention_sparse_workspace(C.byref(s)) == 0                          # refused arguments
     t = valid_args("tree")
-    t.splits = 1
+    t.splits, t.dtype = 1, L.F32
     assert lib.sfb_attention_tree_workspace(C.byref(t)) == 0                            # no partial results to keep
 
 
