@@ -357,6 +357,7 @@ int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wante
 }
 
 sfb_status step_attention(const StepParams& p, int dtype, cudaStream_t stream) {
+    if (step_mma_supported(p, dtype)) return step_mma(p, stream);
     return dtype == SFB_F32 ? step_typed<float>(p, stream) : step_typed<bf16>(p, stream);
 }
 

@@ -73,6 +73,8 @@ struct StepParams {
     float scale_log2;
 };
 
+bool step_mma_supported(const StepParams& p, int dtype);   // attention_step_mma.cu
+sfb_status step_mma(const StepParams& p, cudaStream_t stream);
 sfb_status step_attention(const StepParams& p, int dtype, cudaStream_t stream);
 int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wanted, int* chunk_blocks);
 
