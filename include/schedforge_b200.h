@@ -405,7 +405,8 @@ sfb_status sfb_k_paged_kv_bounds(const sfb_bounds_args* args, sfb_stream stream)
 
 /* Decode attention of one query token per sequence over the blocks that matter to it.  For each (sequence, K/V head)
  * every live block gets a score that no logit of the block exceeds (before scaling),
- *   score = max over the K/V head's query heads of sum_d max(q_d * low_d, q_d * high_d),  accumulated in 64 bits,
+ *   score = max over the K/V head's query heads of sum_d max(q_d * low_d, q_d * high_d),  accumulated in 64 bits
+ * (elements with q_d = 0 add nothing),
  * and min(budget_blocks, live blocks) blocks are kept: the first sink_blocks, the last recent_blocks, and of the others those with the
  * highest scores (ties: the lower index; a NaN score ranks last).  selected[b, kv_head, :] lists the kept logical
  * block indices in ascending order, -1 behind them.  out is the softmax attention over the live positions of the

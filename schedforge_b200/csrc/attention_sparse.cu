@@ -4,17 +4,30 @@
 // (sfb_k_paged_kv_bounds).  sum_d max(q_d low_d, q_d high_d) then bounds every logit of the block from above at a
 // sixteenth of the keys' bytes (16-token blocks), and the blocks with the largest bounds are attended to.
 // Three steps: scores (memory-bound on the bounds), selection (one CTA per (sequence, K/V head)), attention over the
-// list (step_attention).  Scores are summed in 64 bits: ranks follow from them, and with 64 bits a different order of
-// summation cannot swap two blocks that are not equal for all purposes.
+// list (step_attention).  Ranks follow from the scores, so they count in 64 bits, where a different order of summation
+// cannot swap two blocks that are not equal for all purposes.  64-bit arithmetic for all blocks would take longer than
+// their bytes (two products an element and head: 537 million at eight sequences of 128 thousand tokens), so the pass
+// over all blocks sums in 32 bits, and only blocks whose rank those sums leave open are scored again.
 #include "cache_ops.cuh"
+#include "ptx_sm100.cuh"
 #include "select.cuh"
 
 namespace sfb {
 namespace {
 
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+}
+__device__ __forceinline__ void load4(const bf16* p, float (&v)[4]) {
+    const uint2 f = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(f.x << 16); v[1] = __uint_as_float(f.x & 0xffff0000u);
+    v[2] = __uint_as_float(f.y << 16); v[3] = __uint_as_float(f.y & 0xffff0000u);
+}
+
 template <class T>
 __global__ void __launch_bounds__(128)
-bounds_kernel(const __grid_constant__ PagedView kv, const int* __restrict__ start_len, T* __restrict__ bounds) {
+bounds_kernel(const __grid_constant__ PagedView kv, const int* __restrict__ start_len, T* __restrict__ bounds, int vec) {
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependents_may_launch();
     grid_dependency_wait();
@@ -27,6 +40,24 @@ bounds_kernel(const __grid_constant__ PagedView kv, const int* __restrict__ star
         const int live = min(kv.block_tokens, end - block * kv.block_tokens);
         const T* keys = static_cast<const T*>(kv.k_pool) + row * kv.dim;
         T* dst = bounds + row / kv.block_tokens * 2 * kv.dim;
+        if (vec) {   // four elements a lane, every token's load in flight
+            for (int d = lane * 4; d < kv.dim; d += 128) {
+                float lo[4] = {INFINITY, INFINITY, INFINITY, INFINITY}, hi[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 16
+                for (int t = 0; t < live; ++t) {
+                    float v[4];
+                    load4(keys + static_cast<int64_t>(t) * kv.dim + d, v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { lo[e] = fminf(lo[e], v[e]); hi[e] = fmaxf(hi[e], v[e]); }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dst[d + e] = from_float<T>(lo[e]);
+                    dst[kv.dim + d + e] = from_float<T>(hi[e]);
+                }
+            }
+            continue;
+        }
         for (int d = lane; d < kv.dim; d += 32) {
             float lo = INFINITY, hi = -INFINITY;
 #pragma unroll 8
@@ -44,14 +75,16 @@ bounds_kernel(const __grid_constant__ PagedView kv, const int* __restrict__ star
 struct ScoreParams {
     PagedView kv;
     const void *q, *bounds;
-    double* scores;       // [batch * kv_heads][score_stride]
-    int q_heads, score_stride;
+    float* scores;        // [batch * kv_heads][score_stride], summed in 32 bits
+    float* sizes;         // [batch * kv_heads][gridDim.x]: the largest |bound| among the blocks of a CTA
+    int q_heads, score_stride, batch_blocks, cta_blocks;
 };
 
-// One warp per block; lane owns every 32nd element.
+// Any layout: one warp per block, lane owns every 32nd element.
 template <class T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 score_kernel(const __grid_constant__ ScoreParams p) {
+    __shared__ float size_of[4];
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependents_may_launch();
@@ -60,42 +93,319 @@ score_kernel(const __grid_constant__ ScoreParams p) {
     const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
     const int group = p.q_heads / kv.kv_heads;
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group) * kv.dim;
-    for (int block = blockIdx.x * 8 + warp; block < blocks; block += gridDim.x * 8) {
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    float size = 0.0F;
+    for (int block = blockIdx.x * 16 + warp; block < min(blocks, (static_cast<int>(blockIdx.x) + 1) * 16); block += 4) {
         const int page = kv.table[static_cast<size_t>(b) * kv.max_blocks + block];
-        double best = __longlong_as_double(0x7ff8000000000000ll);  // NaN: ranks last
+        float best = __uint_as_float(0x7fc00000u);  // NaN: ranks last
         if (page >= 0 && page < kv.num_blocks) {
             const T* lo = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * kv.dim;
             const T* hi = lo + kv.dim;
             for (int g = 0; g < group; ++g) {
-                double s = 0.0;
+                float s = 0.0F;
                 for (int d = lane; d < kv.dim; d += 32) {
-                    const float qv = to_float(q[g * kv.dim + d]);
-                    s += static_cast<double>(qv) * static_cast<double>(to_float(qv > 0.0F ? hi[d] : lo[d]));
+                    const float qv = to_float(q[g * kv.dim + d]), l = to_float(lo[d]), h = to_float(hi[d]);
+                    s = fmaf(qv, qv > 0.0F ? h : l, s);
+                    size = fmaxf(size, fmaxf(fabsf(l), fabsf(h)));
                 }
                 s = warp_sum(s);
-                best = fmax(best, s);  // (fmax ignores NaN)
+                best = fmaxf(best, s);  // (fmaxf ignores NaN)
             }
         } else if (lane == 0) {
             atomicOr(kv.status, kCodeDecodeBounds);
         }
-        if (lane == 0) p.scores[(static_cast<size_t>(b) * kv.kv_heads + kvh) * p.score_stride + block] = best;
+        if (lane == 0) p.scores[row * p.score_stride + block] = best;
+    }
+    size = warp_max(size);
+    if (lane == 0) size_of[warp] = size;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
+}
+
+// Sums of N values over LPR lanes: every step halves the values a lane still carries as long as there are several, so
+// that N values cost N - 1 exchanges instead of N log2(LPR).  Lane `sub` ends with the values of index
+// sub * N / LPR ... (all lanes of a run of LPR / N with the same one where N < LPR).
+template <int N, int LPR>
+__device__ __forceinline__ void spread_sums(float (&v)[N], int sub) {
+    int n = N;
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+        if (n > 1) {
+            n >>= 1;
+            const bool upper = (sub & o) != 0;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
+                if (i < n) {
+                    const float keep = upper ? v[i + n] : v[i], send = upper ? v[i] : v[i + n];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                }
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+        }
     }
 }
 
-constexpr int kSelectThreads = 512;
+// dim % 8 == 0 and 16-byte aligned rows.  Each of a CTA's four warps works on its own through the blocks of the CTA's
+// range: batches of about 8 KB of bounds come into its part of shared memory by bulk copies (one per block: low and
+// high are contiguous), three batches in flight, so 96 KB per CTA and two CTAs per SM whatever the warps do.
+// LPR lanes share a block, eight elements each, 32 / LPR blocks at once and four times over.  With q+ = max(q, 0) and
+// q- = min(q, 0) the bound is q+ . high + q- . low: two fused multiply-adds an element and no selection.
+constexpr int kScoreRows = 4, kScoreStages = 3, kScoreWarps = 4, kScoreBatchBytes = 8192;
+constexpr uint32_t kCodeScore = 0x20;
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <class T, int LPR, int GC>
+__global__ void __launch_bounds__(kScoreWarps * 32)
+score_vec_kernel(const __grid_constant__ ScoreParams p) {
+    constexpr int RPW = 32 / LPR, N = kScoreRows * GC, kPass = RPW * kScoreRows;   // blocks a warp scores at once
+    constexpr int kLeft = N > LPR ? N / LPR : 1;        // values a lane ends with
+    extern __shared__ __align__(16) uint8_t score_smem[];   // [warps][stages][batch][2 * dim]
+    __shared__ uint64_t bars[kScoreWarps][kScoreStages];
+    __shared__ uint32_t abort_word;
+    __shared__ float size_of[kScoreWarps];
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPR, rg = lane / LPR;
+    const int group = p.q_heads / kv.kv_heads, batch = p.batch_blocks;
+    const uint32_t block_bytes = static_cast<uint32_t>(2 * kv.dim * sizeof(T));
+    if (lane == 0) {
+        for (int s = 0; s < kScoreStages; ++s) ptx::mbar_init(ptx::smem_u32(&bars[warp][s]), 1);
+        if (warp == 0) abort_word = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async();
+    }
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    __syncthreads();
+    const int ctx = kv.length(b);
+    const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    const int last = min(blocks, (static_cast<int>(blockIdx.x) + 1) * p.cta_blocks);
+    const int begin = blockIdx.x * p.cta_blocks + warp * batch;      // batches go round the warps
+    const int step = kScoreWarps * batch;
+    const int* table = kv.table + static_cast<size_t>(b) * kv.max_blocks;
+    uint8_t* mine = score_smem + static_cast<size_t>(warp) * kScoreStages * batch * block_bytes;
+    const bool inside = sub * 8 < kv.dim;
+
+    // lane i brings block i of a batch (batch <= 32); -1: no such block in the pool
+    const auto page_of = [&](int base) -> int {
+        const int block = base + lane;
+        if (lane >= batch || block >= last) return -2;
+        const int page = table[block];
+        if (page >= 0 && page < kv.num_blocks) return page;
+        atomicOr(kv.status, kCodeDecodeBounds);
+        return -1;
+    };
+    const auto issue = [&](int stage, int page) {
+        const uint32_t bar = ptx::smem_u32(&bars[warp][stage]);
+        const int n = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) ptx::mbar_expect_tx(bar, n * block_bytes);
+        __syncwarp();
+        if (page >= 0)
+            bulk_load(ptx::smem_u32(mine + (static_cast<size_t>(stage) * batch + lane) * block_bytes),
+                      static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * kv.dim, block_bytes, bar);
+    };
+    unsigned there[kScoreStages];       // lanes whose block exists, per stage
+#pragma unroll
+    for (int s = 0; s < kScoreStages; ++s) {
+        const int page = begin + s * step < last ? page_of(begin + s * step) : -2;
+        there[s] = __ballot_sync(0xffffffffu, page >= 0);
+        if (begin + s * step < last) issue(s, page);
+    }
+    float pos[GC][8], neg[GC][8], size = 0.0F;
+    const auto load_heads = [&](int g0) {
+#pragma unroll
+        for (int g = 0; g < GC; ++g) {
+            Raw8<T> raw;   // (heads past the group repeat its last: the largest score does not change)
+            if (inside) raw.load(static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + min(g0 + g, group - 1)) * kv.dim + sub * 8);
+            else raw.zero();
+            raw.get(pos[g]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                neg[g][e] = fminf(pos[g][e], 0.0F);
+                pos[g][e] = fmaxf(pos[g][e], 0.0F);
+            }
+        }
+    };
+    load_heads(0);
+    int stage = 0, phase = 0;
+    for (int base = begin; base < last; base += step) {
+        const int ahead = base + kScoreStages * step;
+        const int next_page = ahead < last ? page_of(ahead) : -2;     // in flight while this batch is scored
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bars[warp][stage]), phase, &abort_word, kv.status, kCodeScore))) break;
+        unsigned present = 0;
+#pragma unroll
+        for (int s = 0; s < kScoreStages; ++s)
+            if (s == stage) present = there[s];
+        const uint8_t* rows = mine + static_cast<size_t>(stage) * batch * block_bytes;
+        for (int pass = 0; pass < batch && base + pass < last; pass += kPass) {
+            float best[kLeft];
+#pragma unroll 1
+            for (int g0 = 0; g0 < group; g0 += GC) {
+                if (group > GC) load_heads(g0);
+                float s[N];
+#pragma unroll
+                for (int u = 0; u < kScoreRows; ++u) {
+                    const int i = pass + u * RPW + rg;
+                    Raw8<T> lo, hi;
+                    if (inside && (present >> i & 1u)) {
+                        const T* src = reinterpret_cast<const T*>(rows + static_cast<size_t>(i) * block_bytes) + sub * 8;
+                        lo.load(src);
+                        hi.load(src + kv.dim);
+                    } else {
+                        lo.zero();
+                        hi.zero();
+                    }
+                    float l[8], h[8];
+                    lo.get(l);
+                    hi.get(h);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) size = fmaxf(size, fmaxf(fabsf(l[e]), fabsf(h[e])));
+#pragma unroll
+                    for (int g = 0; g < GC; ++g) {
+                        float a = 0.0F;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) a = fmaf(neg[g][e], l[e], fmaf(pos[g][e], h[e], a));
+                        s[u * GC + g] = a;
+                    }
+                }
+                spread_sums<N, LPR>(s, sub);
+                // index = block * GC + head: the largest over the heads, first among a lane's own values
+                float top[kLeft];
+                constexpr int kOwn = kLeft < GC ? kLeft : GC;     // heads a lane holds of one block
+#pragma unroll
+                for (int i = 0; i < kLeft; ++i) {
+                    top[i] = s[i];
+#pragma unroll
+                    for (int k = 1; k < kOwn; ++k) top[i] = fmaxf(top[i], s[i / kOwn * kOwn + (i + k) % kOwn]);
+                }
+                constexpr int kFirst = N < LPR ? LPR / N : 1;     // lane distance of two heads
+#pragma unroll
+                for (int o = kFirst; o < kFirst * (GC / kOwn); o <<= 1)
+#pragma unroll
+                    for (int i = 0; i < kLeft; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+                for (int i = 0; i < kLeft; ++i) best[i] = g0 == 0 ? top[i] : fmaxf(best[i], top[i]);
+            }
+            // the first lane (and value) of every block writes its score
+#pragma unroll
+            for (int i = 0; i < kLeft; ++i) {
+                const int index = N >= LPR ? sub * kLeft + i : sub / (LPR / N);
+                const bool first = index % GC == 0 && (N >= LPR || sub % (LPR / N) == 0);
+                const int at = pass + index / GC * RPW + rg;
+                if (first && at < batch && base + at < last)
+                    p.scores[row * p.score_stride + base + at] = present >> at & 1u ? best[i] : __uint_as_float(0x7fc00000u);
+            }
+        }
+        __syncwarp();
+        if (ahead < last) {
+            const unsigned now = __ballot_sync(0xffffffffu, next_page >= 0);
+#pragma unroll
+            for (int s = 0; s < kScoreStages; ++s)
+                if (s == stage) there[s] = now;
+            issue(stage, next_page);
+        }
+        if (++stage == kScoreStages) { stage = 0; phase ^= 1; }
+    }
+    size = warp_max(size);
+    if (lane == 0) size_of[warp] = size;
+    __syncthreads();
+    if (abort_word)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);  // let copies in flight land before the CTA exits
+    if (threadIdx.x == 0)
+        p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
+}
+
+// How the scoring kernel takes the blocks: lanes per block (0: the kernel for any layout), blocks per batch and per CTA.
+struct ScoreShape {
+    int lanes, batch, cta_blocks;
+};
+ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
+    if (a.head_dim % 8 != 0 || !aligned16(a.bounds) || !aligned16(a.q)) return {0, 0, 16};
+    ScoreShape s{};
+    s.lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
+    const int pass = 32 / s.lanes * kScoreRows;
+    s.batch = kScoreBatchBytes / (2 * a.head_dim * static_cast<int>(dtype_size(a.dtype)));
+    if (s.batch > 32) s.batch = 32;
+    s.batch = s.batch / pass * pass;
+    // ranges of at least one batch a warp, longer while there are enough of them for four rounds of two CTAs per SM
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads;
+    const int64_t ctas = 8LL * sm_count() / rows > 0 ? 8LL * sm_count() / rows : 1;
+    const int round = kScoreWarps * s.batch;
+    s.cta_blocks = ceil_div(ceil_div(blocks, static_cast<int>(ctas < blocks ? ctas : blocks)), round) * round;
+    return s;
+}
+
+template <class T>
+sfb_status launch_scores(const ScoreParams& p, const ScoreShape& shape, int batch, cudaStream_t stream) {
+    const PagedView& kv = p.kv;
+    const int group = p.q_heads / kv.kv_heads;
+    const dim3 grid(ceil_div(p.score_stride, shape.cta_blocks), kv.kv_heads, batch);
+    const size_t smem = shape.lanes ? sizeof(T) * 2 * kv.dim * static_cast<size_t>(shape.batch) * kScoreStages * kScoreWarps : 0;
+    const auto go = [&](auto kernel) -> sfb_status {
+        if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        SFB_CUDA(launch_dependent(kernel, grid, dim3(128), smem, stream, p));
+        return check_launch("sparse_scores");
+    };
+    const auto by_group = [&](auto k1, auto k2, auto k4) -> sfb_status { return group == 1 ? go(k1) : group == 2 ? go(k2) : go(k4); };
+    if (shape.lanes == 8) return by_group(score_vec_kernel<T, 8, 1>, score_vec_kernel<T, 8, 2>, score_vec_kernel<T, 8, 4>);
+    if (shape.lanes == 16) return by_group(score_vec_kernel<T, 16, 1>, score_vec_kernel<T, 16, 2>, score_vec_kernel<T, 16, 4>);
+    if (shape.lanes == 32) return by_group(score_vec_kernel<T, 32, 1>, score_vec_kernel<T, 32, 2>, score_vec_kernel<T, 32, 4>);
+    return go(score_kernel<T>);
+}
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectCached = 40960;   // scores kept in shared memory (160 KB); longer rows are read from memory each time
 
 struct SelectParams {
     PagedView kv;
-    const double* scores;
+    const void *q, *bounds;
+    const float *scores, *sizes;
+    double* exact;        // [batch * kv_heads][score_stride]
     int* selected;
-    int score_stride, budget, sink, recent;
+    int q_heads, score_stride, size_count, blocks_per_size, budget, sink, recent, cached;
 };
 
+// Score of one block in 64 bits, by one warp.
+template <class T>
+__device__ double exact_score(const SelectParams& p, int b, int kvh, int block) {
+    const PagedView& kv = p.kv;
+    const int lane = threadIdx.x & 31, group = p.q_heads / kv.kv_heads;
+    const int page = kv.table[static_cast<size_t>(b) * kv.max_blocks + block];
+    double best = __longlong_as_double(0x7ff8000000000000ll);  // NaN: ranks last
+    if (page < 0 || page >= kv.num_blocks) return best;
+    const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group) * kv.dim;
+    const T* lo = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * kv.dim;
+    const T* hi = lo + kv.dim;
+    for (int g = 0; g < group; ++g) {
+        double s = 0.0;
+        for (int d = lane; d < kv.dim; d += 32) {
+            const float qv = to_float(q[g * kv.dim + d]);
+            if (qv != 0.0F) s += static_cast<double>(qv) * static_cast<double>(to_float(qv > 0.0F ? hi[d] : lo[d]));
+        }
+        best = fmax(best, warp_sum(s));  // (fmax ignores NaN)
+    }
+    return best;
+}
+
+// The scores of the pass before are sums in 32 bits: at most 8 + 5 roundings, so each is within
+//   err = 2^-20 * (largest |q|_1 of the heads) * (largest |bound|)
+// of the exact one (13 * 2^-24 with room for what the test itself rounds).  Any value t with k scores at or above
+// it and fewer than k (or at most k) above it then decides every block but those within 2 err of t: those are
+// scored again in 64 bits and ranked by that.  Typically none to a handful; equal blocks, or bounds so large that err is
+// not finite, send more through the second pass, never a wrong one through the first.
+template <class T>
 __global__ void __launch_bounds__(kSelectThreads)
 select_kernel(const __grid_constant__ SelectParams p) {
     __shared__ SelectShared sh;
+    __shared__ float most[2][kSelectThreads / 32];
+    __shared__ int counts[2];
     const PagedView& kv = p.kv;
-    const int b = blockIdx.y, kvh = blockIdx.x;
+    const int b = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependents_may_launch();
     grid_dependency_wait();
     const int ctx = kv.length(b);
@@ -107,30 +417,103 @@ select_kernel(const __grid_constant__ SelectParams p) {
         for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < n ? i : -1;
         return;
     }
-    const double* scores = p.scores + row * p.score_stride;
-    const int recent_from = n - p.recent, sink = p.sink;
-    const auto key = [&](int i) -> uint64_t { return i < sink || i >= recent_from ? ~0ull : order_key(scores[i]); };
-    const Threshold t = select_threshold<kSelectThreads>(sh, n, k, key);
-    int written = 0, ties = 0;
-    for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-        const int i = i0 + threadIdx.x;
-        const uint64_t v = i < n ? key(i) : 0;
-        const bool tie = i < n && t.cut != 0 && v == t.low;
-        const bool above = i < n && (t.cut != 0 ? v > t.low : v >= t.low);
-        int above_rank, tie_rank, above_total, tie_total;
-        flag_ranks<kSelectThreads>(sh.scan, above, tie, above_rank, tie_rank, above_total, tie_total);
-        const int tie_room = t.cut - ties;                   // ties still to be kept, lowest indices first
-        const int at = written + above_rank + min(tie_rank, max(tie_room, 0));
-        if (above || (tie && tie_rank < tie_room)) out[at] = i;
-        written += above_total + min(tie_total, max(tie_room, 0));
-        ties += tie_total;
+    extern __shared__ float cached[];
+    const float* scores = p.scores + row * p.score_stride;
+    if (p.cached) {
+        for (int i = threadIdx.x; i < n; i += kSelectThreads) cached[i] = scores[i];
+        scores = cached;   // (ordered by the barrier below)
     }
+    double* exact = p.exact + row * p.score_stride;
+    const int recent_from = n - p.recent, sink = p.sink;
+    const auto forced = [&](int i) { return i < sink || i >= recent_from; };
+    // the error of the 32-bit scores
+    const int group = p.q_heads / kv.kv_heads;
+    float norm = 0.0F, size = 0.0F;
+    for (int g = warp; g < group; g += kSelectThreads / 32) {
+        const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + g) * kv.dim;
+        float s = 0.0F;
+        for (int d = lane; d < kv.dim; d += 32) s += fabsf(to_float(q[d]));
+        s = warp_sum(s);
+        norm = s > norm || s != s ? s : norm;
+    }
+    for (int i = threadIdx.x; i < (n + p.blocks_per_size - 1) / p.blocks_per_size; i += kSelectThreads)
+        size = fmaxf(size, p.sizes[row * p.size_count + i]);
+    size = warp_max(size);
+    if (lane == 0) { most[0][warp] = norm; most[1][warp] = size; }
+    if (threadIdx.x < 2) counts[threadIdx.x] = 0;
+    __syncthreads();
+    norm = size = 0.0F;
+    for (int w = 0; w < kSelectThreads / 32; ++w) {
+        norm = most[0][w] > norm || most[0][w] != most[0][w] ? most[0][w] : norm;
+        size = fmaxf(size, most[1][w]);
+    }
+    const float err2 = 2.0F * 9.5367431640625e-7F * norm * size;  // 2 err
+    // class of a block: 2 kept, 0 left out, 1 to be ranked in 64 bits
+    const int n_forced = min(sink, n) + min(p.recent, n) - max(0, min(sink, n) - max(recent_from, 0));
+    float above = INFINITY, below = INFINITY;
+    if (k > n_forced) {
+        const Threshold first = select_threshold<kSelectThreads>(
+            sh, n, k - n_forced, [&](int i) -> uint64_t { return forced(i) ? 0 : order_key(scores[i]); });
+        const uint32_t image = static_cast<uint32_t>(first.low);
+        const float t = __uint_as_float(image >> 31 ? image & 0x7fffffffu : ~image);
+        above = t + err2;
+        below = t - err2;
+    }
+    const bool open = k > n_forced;
+    const auto classify = [&](int i) -> int {
+        if (forced(i)) return 2;
+        if (!open) return 0;
+        const float v = scores[i];
+        return v > above ? 2 : (v < below ? 0 : 1);   // (NaN anywhere: 1)
+    };
+    int near = 0, kept = 0;
+    for (int i = threadIdx.x; i < n; i += kSelectThreads) {
+        const int c = classify(i);
+        near += c == 1;
+        kept += c == 2;
+    }
+    near = __reduce_add_sync(0xffffffffu, near);
+    kept = __reduce_add_sync(0xffffffffu, kept);
+    if (lane == 0) {
+        atomicAdd(&counts[0], near);
+        atomicAdd(&counts[1], kept);
+    }
+    __syncthreads();
+    const int room = k - counts[1];       // near blocks still to be kept
+    Threshold last{0, 0};
+    if (room > 0 && room < counts[0]) {
+        for (int i0 = warp * 32; i0 < n; i0 += kSelectThreads) {
+            unsigned todo = __ballot_sync(0xffffffffu, i0 + lane < n && classify(i0 + lane) == 1);
+            while (todo) {
+                const int i = i0 + __ffs(todo) - 1;
+                todo &= todo - 1;
+                const double v = exact_score<T>(p, b, kvh, i);
+                if (lane == 0) exact[i] = v;
+            }
+        }
+        __syncthreads();
+        last = select_threshold<kSelectThreads>(sh, n, room, [&](int i) -> uint64_t { return classify(i) == 1 ? order_key(exact[i]) : 0; });
+    }
+    const bool ranked = room > 0 && room < counts[0];
+    walk_ranks<kSelectThreads>(sh.walk, n,
+        [&](int i) {
+            const int c = classify(i);
+            if (c == 2 || (c == 1 && room > 0 && !ranked)) return 1;
+            if (c == 0 || room <= 0) return 0;
+            const uint64_t v = order_key(exact[i]);
+            if (last.cut == 0) return v >= last.low ? 1 : 0;
+            return v > last.low ? 1 : (v == last.low ? 2 : 0);
+        },
+        [&](int i, bool take, bool tie, int rank, int ties) {   // ties: the first last.cut of them, lowest indices first
+            const int at = rank + min(ties, last.cut);
+            if ((take || (tie && ties < last.cut)) && at < k) out[at] = i;
+        });
     for (int i = k + threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = -1;
 }
 
 struct SparseLayout {
-    int score_stride, splits, chunk_blocks;
-    size_t scores, partials, total;
+    int score_stride, splits, chunk_blocks, size_count;
+    size_t scores, sizes, partials, total;   // exact scores come first
 };
 
 SparseLayout sparse_layout(const sfb_sparse_args& a) {
@@ -141,9 +524,12 @@ SparseLayout sparse_layout(const sfb_sparse_args& a) {
     l.score_stride = blocks;
     const int64_t kept = a.budget_blocks < blocks ? a.budget_blocks : blocks;
     l.splits = step_splits(a.batch, a.kv_heads, static_cast<int>(kept * a.block_tokens), a.block_tokens, a.splits, &l.chunk_blocks);
-    l.scores = round_up16(sizeof(double) * static_cast<size_t>(a.batch) * a.kv_heads * blocks);
-    l.partials = sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.splits * (a.head_dim_value + 2);
-    l.total = l.scores + l.partials;
+    const size_t rows = static_cast<size_t>(a.batch) * a.kv_heads;
+    l.size_count = ceil_div(blocks, 16);     // no scoring kernel takes fewer blocks a CTA
+    l.scores = round_up16(sizeof(double) * rows * blocks);
+    l.sizes = l.scores + round_up16(sizeof(float) * rows * blocks);
+    l.partials = l.sizes + round_up16(sizeof(float) * rows * l.size_count);
+    l.total = l.partials + sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.splits * (a.head_dim_value + 2);
     return l;
 }
 
@@ -173,13 +559,14 @@ sfb_status sfb_k_paged_kv_bounds(const sfb_bounds_args* a, sfb_stream stream) {
     SFB_REQUIRE(a->max_tokens > 0, "block bounds: max_tokens must be positive");
     const PagedView kv = make_view(a->k_pool, a->k_pool, a->block_table, a->end_len, a->kv_heads, a->head_dim, a->head_dim,
                                    a->block_tokens, a->max_blocks, a->num_blocks, a->max_blocks * a->block_tokens);
+    const int vec = a->head_dim % 4 == 0 && aligned16(a->k_pool);
     const int64_t touched = a->max_tokens / a->block_tokens + 2;
     const int64_t spread = touched < a->max_blocks ? touched : a->max_blocks;
     const dim3 grid(static_cast<unsigned>(ceil_div64(spread, 4)), a->kv_heads, a->batch);
     if (a->dtype == SFB_F32)
-        SFB_CUDA(launch_dependent(bounds_kernel<float>, grid, dim3(128), 0, as_stream(stream), kv, a->start_len, static_cast<float*>(a->bounds)));
+        SFB_CUDA(launch_dependent(bounds_kernel<float>, grid, dim3(128), 0, as_stream(stream), kv, a->start_len, static_cast<float*>(a->bounds), vec));
     else
-        SFB_CUDA(launch_dependent(bounds_kernel<bf16>, grid, dim3(128), 0, as_stream(stream), kv, a->start_len, static_cast<bf16*>(a->bounds)));
+        SFB_CUDA(launch_dependent(bounds_kernel<bf16>, grid, dim3(128), 0, as_stream(stream), kv, a->start_len, static_cast<bf16*>(a->bounds), vec));
     return check_launch("paged_kv_bounds");
 }
 
@@ -197,21 +584,28 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
                                    a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
     cudaStream_t s = as_stream(stream);
     char* ws = static_cast<char*>(a->workspace);
+    double* exact = reinterpret_cast<double*>(ws);
+    float *scores = reinterpret_cast<float*>(ws + l.scores), *sizes = reinterpret_cast<float*>(ws + l.sizes);
+    const ScoreShape shape = score_shape(*a, l.score_stride);
     {
-        const ScoreParams p{kv, a->q, a->bounds, reinterpret_cast<double*>(ws), a->q_heads, l.score_stride};
-        const dim3 grid(ceil_div(l.score_stride, 8), a->kv_heads, a->batch);
-        if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(score_kernel<float>, grid, dim3(256), 0, s, p));
-        else SFB_CUDA(launch_dependent(score_kernel<bf16>, grid, dim3(256), 0, s, p));
-        SFB_TRY(check_launch("sparse_scores"));
+        const ScoreParams p{kv, a->q, a->bounds, scores, sizes, a->q_heads, l.score_stride, shape.batch, shape.cta_blocks};
+        SFB_TRY(a->dtype == SFB_F32 ? launch_scores<float>(p, shape, a->batch, s) : launch_scores<bf16>(p, shape, a->batch, s));
     }
     {
-        const SelectParams p{kv, reinterpret_cast<const double*>(ws), a->selected, l.score_stride, a->budget_blocks, a->sink_blocks,
-                             a->recent_blocks};
-        SFB_CUDA(launch_dependent(select_kernel, dim3(a->kv_heads, a->batch), dim3(kSelectThreads), 0, s, p));
+        const SelectParams p{kv, a->q, a->bounds, scores, sizes, exact, a->selected, a->q_heads, l.score_stride,
+                             ceil_div(l.score_stride, shape.cta_blocks), shape.cta_blocks, a->budget_blocks, a->sink_blocks, a->recent_blocks, l.score_stride <= kSelectCached};
+        const dim3 grid(a->kv_heads, a->batch);
+        const size_t smem = p.cached ? sizeof(float) * l.score_stride : 0;
+        const auto go = [&](auto kernel) -> sfb_status {
+            if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            SFB_CUDA(launch_dependent(kernel, grid, dim3(kSelectThreads), smem, s, p));
+            return SFB_OK;
+        };
+        SFB_TRY(a->dtype == SFB_F32 ? go(select_kernel<float>) : go(select_kernel<bf16>));
         SFB_TRY(check_launch("sparse_select"));
     }
     StepParams p{};
-    p.kv = kv; p.q = a->q; p.out = a->out; p.partials = reinterpret_cast<float*>(ws + l.scores);
+    p.kv = kv; p.q = a->q; p.out = a->out; p.partials = reinterpret_cast<float*>(ws + l.partials);
     p.selected = a->selected; p.budget = a->budget_blocks;
     p.batch = a->batch; p.q_heads = a->q_heads; p.splits = l.splits; p.chunk_blocks = l.chunk_blocks;
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;

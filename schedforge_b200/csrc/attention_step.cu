@@ -13,33 +13,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kRows = 4;  // rows in flight per lane group
 
-template <class T> struct Raw8;
-template <> struct Raw8<float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const float* p) {
-        a = *reinterpret_cast<const float4*>(p);
-        b = *reinterpret_cast<const float4*>(p + 4);
-    }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.0F, 0.0F, 0.0F, 0.0F); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-};
-template <> struct Raw8<bf16> {
-    uint4 a;
-    __device__ __forceinline__ void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-};
-
 // Eight elements of a row: lane `sub` of LPR owns [8 * sub, 8 * sub + 8) (VEC: dim % 8 == 0 and 16-byte aligned rows),
 // or every LPR-th element.
 template <class T, int LPR, bool VEC>
@@ -335,19 +308,16 @@ PagedView make_view(const void* k_pool, const void* v_pool, const int* table, co
     return kv;
 }
 
-// Splits of `tokens` positions: whole blocks, at most 128 splits (the merge keeps one weight per split in shared
-// memory), as long as the CTAs still fill the GPU (two to four per SM).  Long splits stream better (the ramp of a CTA
-// is paid once), short ones fill the GPU when there are few sequences; 64 positions is the least worth a CTA.
+// Splits of `tokens` positions, in whole blocks.  Two CTAs per SM keep the memory system full, so a split is as long
+// as that allows (its ramp is paid once and there is less to merge), but at most 2048 positions, which evens out ragged
+// contexts, and at least 64.  At most 128 splits: the merge keeps one weight per split in shared memory.
 int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wanted, int* chunk_blocks) {
     const int blocks = tokens > 0 ? ceil_div(tokens, block_tokens) : 1;
     int splits = wanted;
     if (splits <= 0) {
-        int chunk = 2048;
-        splits = ceil_div(tokens, chunk);
-        while (static_cast<int64_t>(batch) * kv_heads * splits < 4LL * sm_count() && chunk > 64) {
-            chunk /= 2;
-            splits = ceil_div(tokens, chunk);
-        }
+        const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, slots = 2LL * sm_count();
+        splits = static_cast<int>(slots / pairs < tokens / 64 ? slots / pairs : tokens / 64);
+        if (splits < ceil_div(tokens, 2048)) splits = ceil_div(tokens, 2048);
     }
     if (splits > 128) splits = 128;
     if (splits > blocks) splits = blocks;

@@ -117,6 +117,7 @@ struct EvictParams {
     const int* positions;
     int* positions_out;
     int* new_len;
+    uint8_t* kept;         // [batch * kv_heads][max_context]
     int* moves;            // per (sequence, K/V head): count, then max_moves destinations, then max_moves sources
     int max_moves, stride, budget, sink, recent;
 };
@@ -139,6 +140,7 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     int* positions_out = p.positions_out + row * p.stride;
     int* to = p.moves + row * (1 + 2 * static_cast<size_t>(p.max_moves)) + 1;
     int* since = to + p.max_moves;
+    uint8_t* kept_bits = p.kept + row * kv.limit;
     if (k == n) {
         if (threadIdx.x == 0) to[-1] = 0;
         for (int i = threadIdx.x; i < n; i += kEvictThreads) {
@@ -155,32 +157,45 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     newest = __reduce_max_sync(0xffffffffu, newest_of[lane]);
     const int64_t recent_from = static_cast<int64_t>(newest) - p.recent;
     const int sink = p.sink;
-    const auto key = [&](int i) -> uint64_t {
-        const int at = positions[i];
-        return at < sink || at > recent_from ? ~0ull : order_key(weights[i]);
-    };
-    const Threshold t = select_threshold<kEvictThreads>(sh, n, k, key);
-    int ties = 0, holes = 0, tails = 0;
-    for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
-        const int i = i0 + threadIdx.x;
-        const uint64_t v = i < n ? key(i) : 0;
-        const bool tie = i < n && t.cut != 0 && v == t.low;
-        int tie_rank, unused, tie_total, unused_total;
-        flag_ranks<kEvictThreads>(sh.scan, tie, false, tie_rank, unused, tie_total, unused_total);
-        const bool kept = i < n && (tie ? tie_rank < t.cut - ties : (t.cut != 0 ? v > t.low : v >= t.low));
-        ties += tie_total;
-        const bool hole = i < k && !kept, tail = i >= k && kept;
-        int hole_rank, tail_rank, hole_total, tail_total;
-        flag_ranks<kEvictThreads>(sh.scan, hole, tail, hole_rank, tail_rank, hole_total, tail_total);
-        if (hole) to[holes + hole_rank] = i;
-        if (tail) since[tails + tail_rank] = i;
-        holes += hole_total;
-        tails += tail_total;
-        if (i < k && kept) {
-            weights_out[i] = weights[i];
-            positions_out[i] = positions[i];
-        }
-    }
+    // rows kept by their position are counted first; the rest of the budget goes to the largest weights of the others
+    const auto safe = [&](int i) { return positions[i] < sink || positions[i] > recent_from; };
+    int n_safe = 0;
+    for (int i = threadIdx.x; i < n; i += kEvictThreads) n_safe += safe(i);
+    n_safe = __reduce_add_sync(0xffffffffu, n_safe);
+    __syncthreads();
+    if (lane == 0) newest_of[warp] = n_safe;
+    __syncthreads();
+    n_safe = __reduce_add_sync(0xffffffffu, newest_of[lane]);
+    const int room = k - n_safe;      // (positions that repeat can make more rows safe than the budget holds)
+    const auto key = [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); };
+    Threshold t{~0ull, 0};
+    if (room > 0) t = select_threshold<kEvictThreads>(sh, n, room, key);
+    // two walks in slot order: which rows are kept (ties go to the lower slot), then the ranks of freed slots and moved rows
+    walk_ranks<kEvictThreads>(sh.walk, n,
+        [&](int i) {
+            const bool s = safe(i);
+            return (s ? 2 : 0) | (!s && room > 0 && t.cut != 0 && order_key(weights[i]) == t.low ? 1 : 0);
+        },
+        [&](int i, bool tie, bool s, int ties, int safes) {
+            bool kept = s ? safes < k : (tie ? ties < t.cut : false);
+            if (!s && !tie && room > 0) {
+                const uint64_t v = order_key(weights[i]);
+                kept = t.cut != 0 ? v > t.low : v >= t.low;
+            }
+            kept_bits[i] = kept;
+        });
+    __syncthreads();
+    const uint64_t totals = walk_ranks<kEvictThreads>(sh.walk, n,
+        [&](int i) { return i < k ? (kept_bits[i] ? 0 : 1) : (kept_bits[i] ? 2 : 0); },
+        [&](int i, bool hole, bool tail, int holes, int tails) {
+            if (hole) { if (holes < p.max_moves) to[holes] = i; }
+            else if (tail) { if (tails < p.max_moves) since[tails] = i; }
+            else if (i < k) {
+                weights_out[i] = weights[i];
+                positions_out[i] = positions[i];
+            }
+        });
+    const int holes = min(min(static_cast<int>(totals & 0xffffffffu), static_cast<int>(totals >> 32)), p.max_moves);   // (both counts are equal)
     __syncthreads();  // the lists, and every read of weights and positions that an aliased output may overwrite
     for (int j = threadIdx.x; j < holes; j += kEvictThreads) {
         weights_out[to[j]] = weights[since[j]];
@@ -221,6 +236,10 @@ int evict_max_moves(const sfb_evict_args& a) {
     const int limit = a.max_context < covered ? a.max_context : covered;
     const int beyond = limit - a.budget;
     return beyond <= 0 ? 0 : (beyond < a.budget ? beyond : a.budget);
+}
+
+size_t evict_moves_bytes(const sfb_evict_args& a) {
+    return round_up16(sizeof(int) * static_cast<size_t>(a.batch) * a.kv_heads * (1 + 2 * static_cast<size_t>(evict_max_moves(a))));
 }
 
 sfb_status check_evict(const sfb_evict_args* a) {
@@ -324,7 +343,7 @@ sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream 
 
 size_t sfb_paged_kv_evict_workspace(const sfb_evict_args* a) {
     if (check_evict(a) != SFB_OK) return 0;
-    return sizeof(int) * static_cast<size_t>(a->batch) * a->kv_heads * (1 + 2 * static_cast<size_t>(evict_max_moves(*a)));
+    return evict_moves_bytes(*a) + static_cast<size_t>(a->batch) * a->kv_heads * (a->max_context < a->max_blocks * a->block_tokens ? a->max_context : a->max_blocks * a->block_tokens);
 }
 
 sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
@@ -338,6 +357,7 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
                      a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
     p.weights = a->weights; p.weights_out = a->weights_out; p.positions = a->positions; p.positions_out = a->positions_out;
     p.new_len = a->new_len; p.moves = static_cast<int*>(a->workspace); p.max_moves = evict_max_moves(*a);
+    p.kept = static_cast<uint8_t*>(a->workspace) + evict_moves_bytes(*a);
     p.stride = a->weight_stride; p.budget = a->budget; p.sink = a->sink_tokens; p.recent = a->recent_tokens;
     SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), 0, s, p));
     SFB_TRY(check_launch("evict_select"));

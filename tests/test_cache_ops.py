@@ -660,15 +660,15 @@ def test_workspace_sizes_need_no_device(sfb):
     lib = sfb.load()
     a = valid_args("evict")
     a.max_context = 20
-    assert lib.sfb_paged_kv_evict_workspace(C.byref(a)) == 4 * 2 * 1 * (1 + 2 * 4)     # 20 - 16 rows may move
+    assert lib.sfb_paged_kv_evict_workspace(C.byref(a)) == 80 + 2 * 20     # 20 - 16 rows may move: 9 words a head; one byte a position
     a.budget = 1000
-    assert lib.sfb_paged_kv_evict_workspace(C.byref(a)) == 4 * 2
+    assert lib.sfb_paged_kv_evict_workspace(C.byref(a)) == 16 + 2 * 20
     w = valid_args("weights")
     w.splits = 1
     assert lib.sfb_attention_weights_workspace(C.byref(w)) == 2 * 2 * 66 * 4 + 2 * 2 * 20 * 4
     s = valid_args("sparse")
     s.splits = 1
-    assert lib.sfb_attention_sparse_workspace(C.byref(s)) == 2 * 2 * 8 + 2 * 2 * 66 * 4
+    assert lib.sfb_attention_sparse_workspace(C.byref(s)) == 2 * 2 * 8 + 16 + 16 + 2 * 2 * 66 * 4   # exact, 32-bit, sizes, partials
     s.q_heads = 3
     s.kv_heads = 2
     assert lib.sfb_attention_sparse_workspace(C.byref(s)) == 0                          # refused arguments
