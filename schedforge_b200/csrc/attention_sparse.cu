@@ -9,6 +9,7 @@
 // their bytes (two products an element and head: 537 million at eight sequences of 128 thousand tokens), so the pass
 // over all blocks sums in 32 bits, and only blocks whose rank those sums leave open are scored again.
 #include "cache_ops.cuh"
+#include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
 #include "select.cuh"
 
@@ -320,18 +321,168 @@ score_vec_kernel(const __grid_constant__ ScoreParams p) {
         p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
 }
 
-// How the scoring kernel takes the blocks: lanes per block (0: the kernel for any layout), blocks per batch and per CTA.
+// bf16, dim % 16 == 0: the same ring, with the products on the tensor path.  16 blocks are the rows of A (low and high
+// side by side are 2 dim columns), q- and q+ of up to eight heads the columns of B: 2 dim / 16 instructions replace
+// 4 dim multiply-adds a block and head, which bounded the form above (sparse decode of 8 x 131072 tokens: 90 us of
+// scores).  Rows are 16 bytes further apart than their length, so that ldmatrix meets no bank twice.
+template <int KS>   // steps of 16 columns in one half: dim / 16
+__global__ void __launch_bounds__(kScoreWarps * 32)
+score_mma_kernel(const __grid_constant__ ScoreParams p) {
+    constexpr int kBatch = 16, D = KS * 16, kRowBytes = 4 * D + 16;
+    extern __shared__ __align__(16) uint8_t score_smem[];   // [warps][stages][16][kRowBytes]
+    __shared__ uint64_t bars[kScoreWarps][kScoreStages];
+    __shared__ uint32_t abort_word;
+    __shared__ float size_of[kScoreWarps];
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
+    const int group = p.q_heads / kv.kv_heads;
+    if (lane == 0) {
+        for (int s = 0; s < kScoreStages; ++s) ptx::mbar_init(ptx::smem_u32(&bars[warp][s]), 1);
+        if (warp == 0) abort_word = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async();
+    }
+    grid_dependents_may_launch();
+    grid_dependency_wait();
+    __syncthreads();
+    const int ctx = kv.length(b);
+    const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    const int last = min(blocks, (static_cast<int>(blockIdx.x) + 1) * p.cta_blocks);
+    const int begin = blockIdx.x * p.cta_blocks + warp * kBatch;
+    constexpr int kStep = kScoreWarps * kBatch;
+    const int* table = kv.table + static_cast<size_t>(b) * kv.max_blocks;
+    uint8_t* mine = score_smem + warp * kScoreStages * kBatch * kRowBytes;
+    const auto page_of = [&](int base) -> int {   // lane i < 16 brings block i of a batch
+        const int block = base + lane;
+        if (lane >= kBatch || block >= last) return -2;
+        const int page = table[block];
+        if (page >= 0 && page < kv.num_blocks) return page;
+        atomicOr(kv.status, kCodeDecodeBounds);
+        return -1;
+    };
+    const auto issue = [&](int stage, int page) -> unsigned {
+        const unsigned present = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t bar = ptx::smem_u32(&bars[warp][stage]);
+        if (lane == 0) ptx::mbar_expect_tx(bar, __popc(present) * 4 * D);
+        __syncwarp();
+        if (page >= 0)
+            bulk_load(ptx::smem_u32(mine + (stage * kBatch + lane) * kRowBytes),
+                      static_cast<const bf16*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * D, 4 * D, bar);
+        return present;
+    };
+    unsigned there[kScoreStages];
+#pragma unroll
+    for (int s = 0; s < kScoreStages; ++s) there[s] = begin + s * kStep < last ? issue(s, page_of(begin + s * kStep)) : 0u;
+    // B fragments: columns are heads, rows k: q- for the low half, q+ for the high half
+    uint32_t qb[2 * KS][2];
+    const auto load_heads = [&](int g0) {
+        const int g = g0 + (lane >> 2);
+        const bf16* q = static_cast<const bf16*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + min(g, group - 1)) * D;
+        const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0F, 0.0F);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(q + 16 * k + 8 * h + 2 * quad);
+                const __nv_bfloat162 neg = __hmin2_nan(v, zero), pos = __hmax2_nan(v, zero);   // (a NaN in q reaches every score)
+                qb[k][h] = *reinterpret_cast<const uint32_t*>(&neg);
+                qb[KS + k][h] = *reinterpret_cast<const uint32_t*>(&pos);
+            }
+    };
+    load_heads(0);
+    __nv_bfloat162 most = __floats2bfloat162_rn(0.0F, 0.0F), least = most;
+    int stage = 0, phase = 0;
+    for (int base = begin; base < last; base += kStep) {
+        const int ahead = base + kScoreStages * kStep;
+        const int next_page = ahead < last ? page_of(ahead) : -2;     // in flight while this batch is scored
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bars[warp][stage]), phase, &abort_word, kv.status, kCodeScore))) break;
+        unsigned present = 0;
+#pragma unroll
+        for (int s = 0; s < kScoreStages; ++s)
+            if (s == stage) present = there[s];
+        const uint32_t rows = ptx::smem_u32(mine + stage * kBatch * kRowBytes) + (lane & 15) * kRowBytes + (lane >> 4) * 16;
+        float best[2] = {-INFINITY, -INFINITY};   // rows lane / 4 and lane / 4 + 8
+#pragma unroll 1
+        for (int g0 = 0; g0 < group; g0 += 8) {
+            if (group > 8) load_heads(g0);
+            float c[2][4] = {};   // two chains: even and odd steps
+#pragma unroll
+            for (int k = 0; k < 2 * KS; ++k) {
+                uint32_t a[4];
+                ldmatrix_x4(rows + k * 32, a);
+                mma_bf16(c[k & 1], a, qb[k][0], qb[k][1]);
+                if (g0 == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool ok = present >> ((lane >> 2) + 8 * (i & 1)) & 1u;   // (a row that was not loaded holds anything)
+                        const uint32_t word = ok ? a[i] : 0u;
+                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&word);
+                        if (k < KS) least = __hmin2(least, v);
+                        else most = __hmax2(most, v);
+                    }
+                }
+            }
+            // columns 2 quad and 2 quad + 1 of the heads
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float x = g0 + 2 * quad < group ? c[0][2 * r] + c[1][2 * r] : -INFINITY;
+                const float y = g0 + 2 * quad + 1 < group ? c[0][2 * r + 1] + c[1][2 * r + 1] : -INFINITY;
+                best[r] = fmaxf(best[r], fmaxf(x, y));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
+            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
+            const int at = (lane >> 2) + 8 * r;
+            if (quad == 0 && base + at < last)
+                p.scores[row * p.score_stride + base + at] = present >> at & 1u ? best[r] : __uint_as_float(0x7fc00000u);
+        }
+        __syncwarp();
+        if (ahead < last) {
+            const unsigned now = issue(stage, next_page);
+#pragma unroll
+            for (int s = 0; s < kScoreStages; ++s)
+                if (s == stage) there[s] = now;
+        }
+        if (++stage == kScoreStages) { stage = 0; phase ^= 1; }
+    }
+    const float size = warp_max(fmaxf(fmaxf(__low2float(most), __high2float(most)), -fminf(__low2float(least), __high2float(least))));
+    // (low <= high, so the largest |bound| is the largest high or the smallest low)
+    if (lane == 0) size_of[warp] = size;
+    __syncthreads();
+    if (abort_word)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);  // let copies in flight land before the CTA exits
+    if (threadIdx.x == 0)
+        p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
+}
+
+// How the scores are taken: by which kernel, blocks per batch and per CTA, and the error of a score relative to
+// sum |q_d| * largest |bound|.
+enum ScoreKind { kScoreAny, kScoreVec, kScoreMma };
 struct ScoreShape {
+    ScoreKind kind;
     int lanes, batch, cta_blocks;
+    float error;
 };
 ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
-    if (a.head_dim % 8 != 0 || !aligned16(a.bounds) || !aligned16(a.q)) return {0, 0, 16};
-    ScoreShape s{};
-    s.lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
-    const int pass = 32 / s.lanes * kScoreRows;
-    s.batch = kScoreBatchBytes / (2 * a.head_dim * static_cast<int>(dtype_size(a.dtype)));
-    if (s.batch > 32) s.batch = 32;
-    s.batch = s.batch / pass * pass;
+    ScoreShape s{kScoreAny, 0, 0, 16, 9.5367431640625e-7F};   // 2^-20: at most 8 + 5 roundings of 2^-24
+    if (!aligned16(a.bounds) || !aligned16(a.q)) return s;
+    if (a.dtype == SFB_BF16 && a.head_dim % 16 == 0) {
+        s.kind = kScoreMma;
+        s.batch = 16;
+        s.error = 6.103515625e-5F;   // 2^-14: 2 dim <= 512 products, each addition good to 2^-23 at least
+    } else if (a.dtype == SFB_F32 && a.head_dim % 8 == 0) {
+        s.kind = kScoreVec;
+        s.lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
+        const int pass = 32 / s.lanes * kScoreRows;
+        s.batch = kScoreBatchBytes / (2 * a.head_dim * 4);
+        if (s.batch > 32) s.batch = 32;
+        s.batch = s.batch / pass * pass;
+    } else {
+        return s;
+    }
     // ranges of at least one batch a warp, longer while there are enough of them for four rounds of two CTAs per SM
     const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads;
     const int64_t ctas = 8LL * sm_count() / rows > 0 ? 8LL * sm_count() / rows : 1;
@@ -340,26 +491,39 @@ ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
     return s;
 }
 
-template <class T>
-sfb_status launch_scores(const ScoreParams& p, const ScoreShape& shape, int batch, cudaStream_t stream) {
+template <class Kernel>
+sfb_status launch_score(Kernel kernel, size_t smem, dim3 grid, const ScoreParams& p, cudaStream_t stream) {
+    if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    SFB_CUDA(launch_dependent(kernel, grid, dim3(128), smem, stream, p));
+    return check_launch("sparse_scores");
+}
+
+sfb_status launch_scores(const ScoreParams& p, const ScoreShape& shape, int batch, int dtype, cudaStream_t stream) {
     const PagedView& kv = p.kv;
     const int group = p.q_heads / kv.kv_heads;
     const dim3 grid(ceil_div(p.score_stride, shape.cta_blocks), kv.kv_heads, batch);
-    const size_t smem = shape.lanes ? sizeof(T) * 2 * kv.dim * static_cast<size_t>(shape.batch) * kScoreStages * kScoreWarps : 0;
-    const auto go = [&](auto kernel) -> sfb_status {
-        if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-        SFB_CUDA(launch_dependent(kernel, grid, dim3(128), smem, stream, p));
-        return check_launch("sparse_scores");
+    if (shape.kind == kScoreAny)
+        return dtype == SFB_F32 ? launch_score(score_kernel<float>, 0, grid, p, stream) : launch_score(score_kernel<bf16>, 0, grid, p, stream);
+    if (shape.kind == kScoreMma) {
+        const size_t smem = static_cast<size_t>(kScoreWarps) * kScoreStages * 16 * (4 * kv.dim + 16);
+        switch (kv.dim / 16) {
+#define SFB_SCORE_CASE(KS) case KS: return launch_score(score_mma_kernel<KS>, smem, grid, p, stream);
+            SFB_SCORE_CASE(1) SFB_SCORE_CASE(2) SFB_SCORE_CASE(3) SFB_SCORE_CASE(4) SFB_SCORE_CASE(5) SFB_SCORE_CASE(6) SFB_SCORE_CASE(7)
+            SFB_SCORE_CASE(8) SFB_SCORE_CASE(9) SFB_SCORE_CASE(10) SFB_SCORE_CASE(11) SFB_SCORE_CASE(12) SFB_SCORE_CASE(13)
+            SFB_SCORE_CASE(14) SFB_SCORE_CASE(15) SFB_SCORE_CASE(16)
+#undef SFB_SCORE_CASE
+        }
+    }
+    const size_t smem = sizeof(float) * 2 * kv.dim * static_cast<size_t>(shape.batch) * kScoreStages * kScoreWarps;
+    const auto by_group = [&](auto k1, auto k2, auto k4) -> sfb_status {
+        return group == 1 ? launch_score(k1, smem, grid, p, stream) : group == 2 ? launch_score(k2, smem, grid, p, stream) : launch_score(k4, smem, grid, p, stream);
     };
-    const auto by_group = [&](auto k1, auto k2, auto k4) -> sfb_status { return group == 1 ? go(k1) : group == 2 ? go(k2) : go(k4); };
-    if (shape.lanes == 8) return by_group(score_vec_kernel<T, 8, 1>, score_vec_kernel<T, 8, 2>, score_vec_kernel<T, 8, 4>);
-    if (shape.lanes == 16) return by_group(score_vec_kernel<T, 16, 1>, score_vec_kernel<T, 16, 2>, score_vec_kernel<T, 16, 4>);
-    if (shape.lanes == 32) return by_group(score_vec_kernel<T, 32, 1>, score_vec_kernel<T, 32, 2>, score_vec_kernel<T, 32, 4>);
-    return go(score_kernel<T>);
+    if (shape.lanes == 8) return by_group(score_vec_kernel<float, 8, 1>, score_vec_kernel<float, 8, 2>, score_vec_kernel<float, 8, 4>);
+    if (shape.lanes == 16) return by_group(score_vec_kernel<float, 16, 1>, score_vec_kernel<float, 16, 2>, score_vec_kernel<float, 16, 4>);
+    return by_group(score_vec_kernel<float, 32, 1>, score_vec_kernel<float, 32, 2>, score_vec_kernel<float, 32, 4>);
 }
 
 constexpr int kSelectThreads = 1024;
-constexpr int kSelectCached = 40960;   // scores kept in shared memory (160 KB); longer rows are read from memory each time
 
 struct SelectParams {
     PagedView kv;
@@ -368,7 +532,14 @@ struct SelectParams {
     double* exact;        // [batch * kv_heads][score_stride]
     int* selected;
     int q_heads, score_stride, size_count, blocks_per_size, budget, sink, recent, cached;
+    float error;
 };
+
+// Inverse of order_key(float).
+__device__ __forceinline__ float score_of_key(uint64_t key) {
+    const uint32_t image = static_cast<uint32_t>(key);
+    return __uint_as_float(image >> 31 ? image & 0x7fffffffu : ~image);
+}
 
 // Score of one block in 64 bits, by one warp.
 template <class T>
@@ -392,9 +563,9 @@ __device__ double exact_score(const SelectParams& p, int b, int kvh, int block) 
     return best;
 }
 
-// The scores of the pass before are sums in 32 bits: at most 8 + 5 roundings, so each is within
-//   err = 2^-20 * (largest |q|_1 of the heads) * (largest |bound|)
-// of the exact one (13 * 2^-24 with room for what the test itself rounds).  Any value t with k scores at or above
+// The scores of the pass before are sums in 32 bits, each within
+//   err = error * (largest |q|_1 of the heads) * (largest |bound|)
+// of the exact one (score_shape).  Any value t with k scores at or above
 // it and fewer than k (or at most k) above it then decides every block but those within 2 err of t: those are
 // scored again in 64 bits and ranked by that.  Typically none to a handful; equal blocks, or bounds so large that err is
 // not finite, send more through the second pass, never a wrong one through the first.
@@ -447,15 +618,36 @@ select_kernel(const __grid_constant__ SelectParams p) {
         norm = most[0][w] > norm || most[0][w] != most[0][w] ? most[0][w] : norm;
         size = fmaxf(size, most[1][w]);
     }
-    const float err2 = 2.0F * 9.5367431640625e-7F * norm * size;  // 2 err
-    // class of a block: 2 kept, 0 left out, 1 to be ranked in 64 bits
     const int n_forced = min(sink, n) + min(p.recent, n) - max(0, min(sink, n) - max(recent_from, 0));
+    const float err2 = 2.0F * p.error * norm * size;  // 2 err
+    if (p.cached && k > n_forced) {
+        const bool settled = select_mask<kSelectThreads>(
+            sh, n, k - n_forced, [&](int i) -> uint64_t { return forced(i) ? 0 : order_key(scores[i]); },
+            [&](uint64_t& low, uint64_t& high) {   // whatever the tolerance lets change places with the k-th (NaN, infinity: all)
+                const float from = score_of_key(low) - err2, to = score_of_key(high) + err2;
+                low = from > -INFINITY ? order_key(from) : 1;
+                high = to < INFINITY ? order_key(to) : ~0ull;
+            },
+            [&](int j) -> uint64_t { return order_key(exact_score<T>(p, b, kvh, sh.near[j])); });
+        if (settled) {
+            walk_bits<kSelectThreads>(sh.walk, (n + 31) / 32,
+                [&](int w, unsigned& take, unsigned& none) {
+                    take = sh.words[w];
+                    none = 0;
+                    for (int i = w * 32; i < min(sink, w * 32 + 32); ++i) take |= 1u << (i & 31);
+                    for (int i = max(max(recent_from, 0), w * 32); i < min(n, w * 32 + 32); ++i) take |= 1u << (i & 31);
+                },
+                [&](int i, int rank) { if (rank < k) out[rank] = i; }, [](int, int) {});
+            for (int i = k + threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = -1;
+            return;
+        }
+    }
+    // class of a block: 2 kept, 0 left out, 1 to be ranked in 64 bits
     float above = INFINITY, below = INFINITY;
     if (k > n_forced) {
         const Threshold first = select_threshold<kSelectThreads>(
             sh, n, k - n_forced, [&](int i) -> uint64_t { return forced(i) ? 0 : order_key(scores[i]); });
-        const uint32_t image = static_cast<uint32_t>(first.low);
-        const float t = __uint_as_float(image >> 31 ? image & 0x7fffffffu : ~image);
+        const float t = score_of_key(first.low);
         above = t + err2;
         below = t - err2;
     }
@@ -589,11 +781,11 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
     const ScoreShape shape = score_shape(*a, l.score_stride);
     {
         const ScoreParams p{kv, a->q, a->bounds, scores, sizes, a->q_heads, l.score_stride, shape.batch, shape.cta_blocks};
-        SFB_TRY(a->dtype == SFB_F32 ? launch_scores<float>(p, shape, a->batch, s) : launch_scores<bf16>(p, shape, a->batch, s));
+        SFB_TRY(launch_scores(p, shape, a->batch, a->dtype, s));
     }
     {
         const SelectParams p{kv, a->q, a->bounds, scores, sizes, exact, a->selected, a->q_heads, l.score_stride,
-                             ceil_div(l.score_stride, shape.cta_blocks), shape.cta_blocks, a->budget_blocks, a->sink_blocks, a->recent_blocks, l.score_stride <= kSelectCached};
+                             ceil_div(l.score_stride, shape.cta_blocks), shape.cta_blocks, a->budget_blocks, a->sink_blocks, a->recent_blocks, l.score_stride <= kMaskItems, shape.error};
         const dim3 grid(a->kv_heads, a->batch);
         const size_t smem = p.cached ? sizeof(float) * l.score_stride : 0;
         const auto go = [&](auto kernel) -> sfb_status {

@@ -10,6 +10,7 @@
 // Tokens of a unit past the context may hold anything: their scores are masked, and their V rows are zeroed in shared
 // memory first (0 * NaN).  Waits are bounded.
 #include "cache_ops.cuh"
+#include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
 
 namespace sfb {
@@ -30,24 +31,6 @@ struct Shape {
     static constexpr int kStages = D == 128 ? 3 : 6;
 };
 
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 // 16-byte chunk `chunk` (of D / 8) of token row `row` inside a swizzled unit.
 __device__ __forceinline__ uint32_t unit_chunk(uint32_t unit, int row, int chunk) {
     return unit + (chunk >> 3) * (U * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);

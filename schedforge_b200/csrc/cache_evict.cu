@@ -119,10 +119,42 @@ struct EvictParams {
     int* new_len;
     uint8_t* kept;         // [batch * kv_heads][max_context]
     int* moves;            // per (sequence, K/V head): count, then max_moves destinations, then max_moves sources
-    int max_moves, stride, budget, sink, recent;
+    int max_moves, stride, budget, sink, recent, masked;   // masked: rows of at most kMaskItems slots
 };
 
 constexpr int kEvictThreads = 1024;
+
+// Lists the kept rows of a row too long, or with too many equal weights, for the bit mask: two walks in slot order,
+// which rows are kept (ties go to the lower slot), then the ranks of freed slots and moved rows.
+template <class Safe>
+__device__ int evict_lists(const EvictParams& p, SelectShared& sh, const float* weights, const int* positions, float* weights_out,
+                           int* positions_out, uint8_t* kept_bits, int* to, int* since, int n, int k, int room, const Threshold& t, Safe safe) {
+    walk_ranks<kEvictThreads>(sh.walk, n,
+        [&](int i) {
+            const bool s = safe(i);
+            return (s ? 2 : 0) | (!s && room > 0 && t.cut != 0 && order_key(weights[i]) == t.low ? 1 : 0);
+        },
+        [&](int i, bool tie, bool s, int ties, int safes) {
+            bool kept = s ? safes < k : (tie ? ties < t.cut : false);
+            if (!s && !tie && room > 0) {
+                const uint64_t v = order_key(weights[i]);
+                kept = t.cut != 0 ? v > t.low : v >= t.low;
+            }
+            kept_bits[i] = kept;
+        });
+    __syncthreads();
+    const uint64_t totals = walk_ranks<kEvictThreads>(sh.walk, n,
+        [&](int i) { return i < k ? (kept_bits[i] ? 0 : 1) : (kept_bits[i] ? 2 : 0); },
+        [&](int i, bool hole, bool tail, int holes, int tails) {
+            if (hole) { if (holes < p.max_moves) to[holes] = i; }
+            else if (tail) { if (tails < p.max_moves) since[tails] = i; }
+            else if (i < k) {
+                weights_out[i] = weights[i];
+                positions_out[i] = positions[i];
+            }
+        });
+    return min(min(static_cast<int>(totals & 0xffffffffu), static_cast<int>(totals >> 32)), p.max_moves);
+}
 
 __global__ void __launch_bounds__(kEvictThreads)
 evict_select_kernel(const __grid_constant__ EvictParams p) {
@@ -159,43 +191,56 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     const int sink = p.sink;
     // rows kept by their position are counted first; the rest of the budget goes to the largest weights of the others
     const auto safe = [&](int i) { return positions[i] < sink || positions[i] > recent_from; };
+    extern __shared__ uint32_t keys[];   // masked: the weights' keys, 0 for safe rows
     int n_safe = 0;
-    for (int i = threadIdx.x; i < n; i += kEvictThreads) n_safe += safe(i);
+    for (int i = threadIdx.x; i < n; i += kEvictThreads) {
+        const bool is_safe = safe(i);
+        n_safe += is_safe;
+        if (p.masked) keys[i] = is_safe ? 0u : static_cast<uint32_t>(order_key(weights[i]));
+    }
     n_safe = __reduce_add_sync(0xffffffffu, n_safe);
     __syncthreads();
     if (lane == 0) newest_of[warp] = n_safe;
     __syncthreads();
     n_safe = __reduce_add_sync(0xffffffffu, newest_of[lane]);
     const int room = k - n_safe;      // (positions that repeat can make more rows safe than the budget holds)
-    const auto key = [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); };
-    Threshold t{~0ull, 0};
-    if (room > 0) t = select_threshold<kEvictThreads>(sh, n, room, key);
-    // two walks in slot order: which rows are kept (ties go to the lower slot), then the ranks of freed slots and moved rows
-    walk_ranks<kEvictThreads>(sh.walk, n,
-        [&](int i) {
-            const bool s = safe(i);
-            return (s ? 2 : 0) | (!s && room > 0 && t.cut != 0 && order_key(weights[i]) == t.low ? 1 : 0);
-        },
-        [&](int i, bool tie, bool s, int ties, int safes) {
-            bool kept = s ? safes < k : (tie ? ties < t.cut : false);
-            if (!s && !tie && room > 0) {
-                const uint64_t v = order_key(weights[i]);
-                kept = t.cut != 0 ? v > t.low : v >= t.low;
-            }
-            kept_bits[i] = kept;
-        });
-    __syncthreads();
-    const uint64_t totals = walk_ranks<kEvictThreads>(sh.walk, n,
-        [&](int i) { return i < k ? (kept_bits[i] ? 0 : 1) : (kept_bits[i] ? 2 : 0); },
-        [&](int i, bool hole, bool tail, int holes, int tails) {
-            if (hole) { if (holes < p.max_moves) to[holes] = i; }
-            else if (tail) { if (tails < p.max_moves) since[tails] = i; }
-            else if (i < k) {
+    int holes = 0;
+    bool settled = false;
+    if (p.masked && n_safe <= k) {
+        if (room > 0) {
+            settled = select_mask<kEvictThreads>(sh, n, room, [&](int i) -> uint64_t { return keys[i]; }, [](uint64_t&, uint64_t&) {},
+                                                 [&](int j) -> uint64_t { return keys[sh.near[j]]; });
+        } else {
+            for (int w = threadIdx.x; w < (n + 31) / 32; w += kEvictThreads) sh.words[w] = 0;
+            settled = true;
+            __syncthreads();
+        }
+    }
+    if (settled) {
+        for (int i0 = warp * 32; i0 < n; i0 += kEvictThreads) {
+            const unsigned word = __ballot_sync(0xffffffffu, i0 + lane < n && keys[i0 + lane] == 0u);
+            if (lane == 0) sh.words[i0 >> 5] |= word;
+        }
+        __syncthreads();
+        const uint64_t totals = walk_bits<kEvictThreads>(sh.walk, (n + 31) / 32,
+            [&](int w, unsigned& hole, unsigned& tail) {
+                const int at = w * 32;
+                const unsigned front = at + 32 <= k ? ~0u : (at >= k ? 0u : (1u << (k - at)) - 1);
+                hole = ~sh.words[w] & front;
+                tail = sh.words[w] & ~front;
+            },
+            [&](int i, int rank) { if (rank < p.max_moves) to[rank] = i; }, [&](int i, int rank) { if (rank < p.max_moves) since[rank] = i; });
+        holes = min(min(static_cast<int>(totals & 0xffffffffu), static_cast<int>(totals >> 32)), p.max_moves);   // (both counts are equal)
+        for (int i = threadIdx.x; i < k; i += kEvictThreads)
+            if (sh.words[i >> 5] >> (i & 31) & 1u) {
                 weights_out[i] = weights[i];
                 positions_out[i] = positions[i];
             }
-        });
-    const int holes = min(min(static_cast<int>(totals & 0xffffffffu), static_cast<int>(totals >> 32)), p.max_moves);   // (both counts are equal)
+    } else {
+        Threshold t{~0ull, 0};
+        if (room > 0) t = select_threshold<kEvictThreads>(sh, n, room, [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); });
+        holes = evict_lists(p, sh, weights, positions, weights_out, positions_out, kept_bits, to, since, n, k, room, t, safe);
+    }
     __syncthreads();  // the lists, and every read of weights and positions that an aliased output may overwrite
     for (int j = threadIdx.x; j < holes; j += kEvictThreads) {
         weights_out[to[j]] = weights[since[j]];
@@ -359,7 +404,10 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
     p.new_len = a->new_len; p.moves = static_cast<int*>(a->workspace); p.max_moves = evict_max_moves(*a);
     p.kept = static_cast<uint8_t*>(a->workspace) + evict_moves_bytes(*a);
     p.stride = a->weight_stride; p.budget = a->budget; p.sink = a->sink_tokens; p.recent = a->recent_tokens;
-    SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), 0, s, p));
+    p.masked = p.kv.limit <= kMaskItems;
+    const size_t key_bytes = p.masked ? sizeof(uint32_t) * static_cast<size_t>(p.kv.limit) : 0;
+    SFB_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(uint32_t) * kMaskItems)));
+    SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
     SFB_TRY(check_launch("evict_select"));
     const dim3 grid(p.max_moves > 0 ? (p.max_moves > 64 * 8 ? 64 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
     const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool);

@@ -1,9 +1,10 @@
 // Selection of the k largest of n keys by one CTA, ties to the lower index.
 //
-// Keys are unsigned 64-bit words whose order is the order wanted; a key of 0 does not take part.  The k-th largest key is found by narrowing a
-// range: the keys inside it are counted in 2048 equal bins, the bin that holds the k-th becomes the next range.  A
-// range of 64 bits needs at most six passes; scores that differ in their leading bits need one or two, because a range
-// whose keys are all wanted, or that has shrunk to one value, ends the search.
+// Keys are unsigned 64-bit words whose order is the order wanted; a key of 0 does not take part.  Rows of up to
+// kMaskItems keys: the keys are counted in 2048 equal bins of their range, what lies above the bin of the k-th is kept,
+// and the few keys inside it are ranked against one another (select_mask; bits in shared memory).  Where too
+// many keys share that bin, and for longer rows, the range is narrowed bin by bin until it holds one value
+// (select_threshold: at most six passes for 64 bits).
 #pragma once
 
 #include "common.cuh"
@@ -25,6 +26,10 @@ __device__ __forceinline__ uint64_t order_key(float v) {
     return (u >> 31) ? static_cast<uint32_t>(~u) : (u | 0x80000000u);
 }
 
+constexpr int kMaskItems = 40960;   // one bit each in shared memory
+constexpr int kMaskWords = kMaskItems / 32;
+constexpr int kNearItems = 512;     // keys ranked against one another
+
 struct SelectShared {
     unsigned hist[kSelectBins];
     uint64_t lo[32], hi[32];
@@ -32,6 +37,10 @@ struct SelectShared {
     unsigned long long walk[32];
     uint64_t low, high;
     int rest, done;
+    unsigned words[kMaskWords];
+    int near[kNearItems];
+    uint64_t near_key[kNearItems];
+    int near_count, kept_count;
 };
 
 // What is kept: keys above `low`, and, where cut != 0, the first `cut` keys equal to it (in index order); where cut
@@ -42,8 +51,10 @@ struct Threshold {
 };
 
 // All threads of the CTA call it; 1 <= k <= number of keys that are not 0.  key(i) is evaluated several times.
+// enough: a bin of at most that many keys ends the search as well; the k-th key is then among the keys of
+// [sh.low, sh.high] and the result says how many of those are wanted.
 template <int THREADS, class Key>
-__device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key) {
+__device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key, unsigned enough = 0) {
     constexpr int kWarps = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t lo = ~0ull, hi = 0;
@@ -105,8 +116,8 @@ __device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key) {
             sh.rest = rest - static_cast<int>(above);
             sh.low = first;
             sh.high = high - first < span ? high : first + span;
-            sh.done = shift == 0 || sh.hist[bin] == static_cast<unsigned>(sh.rest);
-            if (sh.hist[bin] == static_cast<unsigned>(sh.rest)) sh.rest = 0;  // the whole bin is wanted
+            sh.done = shift == 0 || sh.hist[bin] == static_cast<unsigned>(sh.rest) || sh.hist[bin] <= enough;
+            if (enough == 0 && sh.hist[bin] == static_cast<unsigned>(sh.rest)) sh.rest = 0;  // the whole bin is wanted
         }
         __syncthreads();
         if (sh.done) break;
@@ -114,6 +125,103 @@ __device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key) {
     const Threshold found{sh.low, sh.rest};
     __syncthreads();
     return found;
+}
+
+// Bits of the k largest keys in sh.words (n <= kMaskItems; keys of 0 get none).  widen(low, high) may extend the range of
+// keys that are ranked, and rank(j) gives the final key of near item j (index sh.near[j]; called by whole warps, all of
+// whose lanes return it): how keys known to a tolerance only are ranked exactly where it matters.  Returns false, with
+// nothing settled, where more than kNearItems keys are in that range.  All threads call it; sh is ready for use afterwards.
+template <int THREADS, class Key, class Widen, class Rank>
+__device__ bool select_mask(SelectShared& sh, int n, int k, Key key, Widen widen, Rank rank) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    select_threshold<THREADS>(sh, n, k, key, kNearItems / 8);
+    uint64_t low = sh.low, high = sh.high;
+    widen(low, high);
+    if (threadIdx.x == 0) sh.near_count = sh.kept_count = 0;
+    __syncthreads();
+    int kept = 0;
+    for (int i0 = warp * 32; i0 < n; i0 += THREADS) {
+        const int i = i0 + lane;
+        const uint64_t v = i < n ? key(i) : 0;
+        const unsigned word = __ballot_sync(0xffffffffu, v > high);
+        kept += __popc(word);
+        if (lane == 0) sh.words[i0 >> 5] = word;
+        if (v != 0 && v >= low && v <= high) {
+            const int at = atomicAdd(&sh.near_count, 1);
+            if (at < kNearItems) sh.near[at] = i;
+        }
+    }
+    if (lane == 0 && kept) atomicAdd(&sh.kept_count, kept);
+    __syncthreads();
+    const int near = sh.near_count, room = k - sh.kept_count;
+    if (near > kNearItems) return false;
+    if (room >= near) {
+        for (int j = threadIdx.x; j < near; j += THREADS) atomicOr(&sh.words[sh.near[j] >> 5], 1u << (sh.near[j] & 31));
+    } else {
+        for (int j = warp; j < near; j += THREADS / 32) {
+            const uint64_t v = rank(j);
+            if (lane == 0) sh.near_key[j] = v;
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < near; j += THREADS) {
+            const uint64_t v = sh.near_key[j];
+            const int i = sh.near[j];
+            int before = 0;
+            for (int o = 0; o < near; ++o) {
+                const uint64_t w = sh.near_key[o];
+                before += w > v || (w == v && sh.near[o] < i);
+            }
+            if (before < room) atomicOr(&sh.words[i >> 5], 1u << (i & 31));
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
+// Walks the set bits of two masks of `words` words in ascending order: visit_a(index, rank), visit_b(index, rank).
+// Returns the totals (a in the low, b in the high half).
+template <int THREADS, class Words, class VisitA, class VisitB>
+__device__ __forceinline__ uint64_t walk_bits(unsigned long long* scan, int words, Words get, VisitA visit_a, VisitB visit_b) {
+    constexpr int kWarps = THREADS / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stretch = ((words + kWarps - 1) / kWarps + 31) & ~31;
+    const int begin = min(words, warp * stretch), end = min(words, begin + stretch);
+    uint64_t sum = 0;
+    for (int w = begin + lane; w < end; w += 32) {
+        unsigned a, b;
+        get(w, a, b);
+        sum += static_cast<uint64_t>(__popc(b)) << 32 | static_cast<unsigned>(__popc(a));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) scan[warp] = sum;
+    __syncthreads();
+    uint64_t before = 0, total = 0;
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) {
+        const uint64_t v = scan[w];
+        if (w < warp) before += v;
+        total += v;
+    }
+    __syncthreads();
+    for (int w0 = begin; w0 < end; w0 += 32) {
+        const int w = w0 + lane;
+        unsigned a = 0, b = 0;
+        if (w < end) get(w, a, b);
+        const uint64_t own = static_cast<uint64_t>(__popc(b)) << 32 | static_cast<unsigned>(__popc(a));
+        uint64_t incl = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const uint64_t at = before + incl - own;
+        int ra = static_cast<int>(at & 0xffffffffu), rb = static_cast<int>(at >> 32);
+        for (; a; a &= a - 1) visit_a(w * 32 + __ffs(a) - 1, ra++);
+        for (; b; b &= b - 1) visit_b(w * 32 + __ffs(b) - 1, rb++);
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return total;
 }
 
 // Walks [0, n) in index order with the flags a(i) and b(i), each warp a contiguous stretch: visit(i, a, b, ra, rb) is

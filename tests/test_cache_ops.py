@@ -338,7 +338,13 @@ SPARSE_CASES = [
     ("bf16", 8, 2, 64, 64, 32, [4000, 2111], 40, 1, 4, 3),
     ("bf16", 16, 2, 128, 128, 48, [4000, 2111], 17, 0, 1, 0),
     ("bf16", 6, 2, 80, 96, 16, [500], 9, 1, 1, 0),
+    ("bf16", 22, 2, 72, 72, 16, [900, 33], 9, 1, 1, 0),         # eleven heads, head_dim no multiple of 16
+    ("bf16", 22, 2, 256, 64, 16, [1900], 19, 1, 1, 0),
+    ("f32", 20, 2, 128, 128, 16, [3000, 100], 30, 0, 2, 0),
+    ("f32", 2, 1, 256, 256, 16, [3000], 30, 0, 2, 0),
+    ("f32", 8, 2, 96, 96, 8, [3000], 30, 0, 2, 0),
     ("bf16", 16, 1, 64, 64, 16, [40000], 300, 1, 4, 0),
+    ("bf16", 2, 1, 16, 16, 1, [43000], 300, 1, 4, 0),             # blocks of one token, more of them than the bit mask holds
 ]
 
 
@@ -533,6 +539,7 @@ def plain_evict(weights, positions, n, budget, sink, recent):
     ("bf16", 2, 64, 64, 32, [5000, 4097], 4096, 0, 4096),       # everything kept is recent
     ("bf16", 1, 80, 7, 16, [100], 1000, 1, 1),                   # nothing leaves
     ("f32", 3, 8, 8, 16, [3000], 1, 1, 0),                       # all but one leave
+    ("f32", 1, 8, 8, 64, [50000, 41000], 20000, 3, 100),         # rows too long for the bit mask
 ])
 def test_evict(dev, port, alias, dtype, hkv, d, dv, block, lens, budget, sink, recent):
     rng = np.random.default_rng(budget)
