@@ -210,7 +210,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == 8) {
             // ------------------------------------------------------------ copies
             const int boxes = KT / p.box_rows;
@@ -279,61 +279,68 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
         } else if (warp == 9) {
             // ------------------------------------------------------------ MMA issue
-            if (lane == 0) {
-                constexpr uint32_t idesc_qk = ptx::umma_idesc_bf16(128, KT, 0, 0);
-                constexpr uint32_t idesc_pv = ptx::umma_idesc_bf16(128, D, 0, 1);
-                uint32_t n_kv = 0, n_seg = 0, n_slot[2] = {0, 0};   // tiles, pieces and slot uses so far
-                bool ok = true;
-                while (ok && w.left > 0) {
-                    const int n = w.take();
-                    const int items = kTwoTiles ? 2 * n : n;
-                    ok = ptx::mbar_wait(ptx::smem_u32(q_full), n_seg & 1, abort_flag, status, kCodeTree | 2);
-                    if (!ok) break;
-                    // S_t = Q . K_j^T for item i (tile j, slot t)
-                    const auto issue_qk = [&](int i) -> bool {
-                        const int t = i & 1, j = kTwoTiles ? i >> 1 : i;
-                        const uint32_t g = n_kv + j;
-                        if (!ptx::mbar_wait(ptx::smem_u32(&k_full[g % kStages]), (g / kStages) & 1, abort_flag, status, kCodeTree | 2)) return false;
-                        ptx::tc_fence_after();
-                        const uint32_t qa = ptx::smem_u32(q_smem + (kTwoTiles ? t : 0) * Sh::kQBytes);
-                        const uint32_t ka = ptx::smem_u32(k_smem + (g % kStages) * kTileBytes);
+            // (the whole warp walks along, so that the operands are uniform; one lane of it issues)
+            constexpr uint32_t idesc_qk = ptx::umma_idesc_bf16(128, KT, 0, 0);
+            constexpr uint32_t idesc_pv = ptx::umma_idesc_bf16(128, D, 0, 1);
+            const uint64_t q_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(q_smem)), k_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(k_smem)),
+                           v_desc = ptx::umma_desc_mn_sw128(ptx::smem_u32(v_smem), kHalfBytes, 1024);
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            uint32_t n_kv = 0, n_seg = 0, slot_parity[2] = {0, 0};   // tiles and pieces so far, parity of each slot's uses
+            const auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort_flag, status, kCodeTree | 2));
+            };
+            bool ok = true;
+            while (ok && w.left > 0) {
+                const int n = __shfl_sync(0xffffffffu, w.take(), 0);
+                const int items = kTwoTiles ? 2 * n : n;
+                ok = wait(q_full, n_seg & 1);
+                if (!ok) break;
+                // S_t = Q . K_j^T for item i (tile j, slot t)
+                const auto issue_qk = [&](int i, int t) -> bool {
+                    const uint32_t g = n_kv + (kTwoTiles ? i >> 1 : i), stage = g % kStages;
+                    if (!wait(&k_full[stage], (g / kStages) & 1)) return false;
+                    ptx::tc_fence_after();
+                    // (a step along K only adds to the address field of the descriptors)
+                    const uint64_t qa = q_desc + (kTwoTiles ? t : 0) * (Sh::kQBytes >> 4), ka = k_desc + stage * (kTileBytes >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = (kk / 4) * kHalfBytes + (kk % 4) * 32;
-                            ptx::umma_bf16(tmem_base + t * KT, ptx::umma_desc_k_sw128(qa + off), ptx::umma_desc_k_sw128(ka + off), idesc_qk, kk != 0);
-                        }
-                        ptx::umma_commit(ptx::smem_u32(&s_full[t]));
-                        if (!kTwoTiles || t == 1) ptx::umma_commit(ptx::smem_u32(&k_empty[g % kStages]));
-                        if (i == items - 1) ptx::umma_commit(ptx::smem_u32(q_empty));
-                        return true;
-                    };
-                    for (int i = 0; ok && i < 2 && i < items; ++i) ok = issue_qk(i);
-                    for (int i = 0; ok && i < items; ++i) {
-                        const int t = i & 1, j = kTwoTiles ? i >> 1 : i;
-                        const uint32_t g = n_kv + j;
-                        ok = ptx::mbar_wait(ptx::smem_u32(&p_full[t]), n_slot[t] & 1, abort_flag, status, kCodeTree | 2) &&
-                             ptx::mbar_wait(ptx::smem_u32(&v_full[g % kStages]), (g / kStages) & 1, abort_flag, status, kCodeTree | 2);
-                        if (!ok) break;
-                        ++n_slot[t];
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const int off = (kk / 4) * (kHalfBytes >> 4) + (kk % 4) * (32 >> 4);
+                        ptx::umma_bf16_warp(tmem + t * KT, qa + off, ka + off, idesc_qk, kk != 0);
+                    }
+                    ptx::umma_commit_warp(ptx::smem_u32(&s_full[t]));
+                    if (!kTwoTiles || t == 1) ptx::umma_commit_warp(ptx::smem_u32(&k_empty[stage]));
+                    if (i == items - 1) ptx::umma_commit_warp(ptx::smem_u32(q_empty));
+                    return true;
+                };
+                ok = issue_qk(0, 0);
+                if (ok && items > 1) ok = issue_qk(1, 1);
+                for (int i0 = 0; ok && i0 < items; i0 += 2) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int i = i0 + t;
+                        if (!ok || i >= items) continue;
+                        const uint32_t g = n_kv + (kTwoTiles ? i >> 1 : i), stage = g % kStages;
+                        ok = wait(&v_full[stage], (g / kStages) & 1) && wait(&p_full[t], slot_parity[t]);
+                        if (!ok) continue;
+                        slot_parity[t] ^= 1;
                         ptx::tc_fence_after();
-                        const uint32_t va = ptx::smem_u32(v_smem + (g % kStages) * kTileBytes);
+                        const uint64_t va = v_desc + stage * (kTileBytes >> 4);
 #pragma unroll
                         for (int kk = 0; kk < KT / 16; ++kk)   // O_t += P_t . V_j
-                            ptx::umma_bf16_ts(tmem_base + kOCol + t * D, tmem_base + t * KT + kk * 8,
-                                              ptx::umma_desc_mn_sw128(va + kk * 16 * 128, kHalfBytes, 1024), idesc_pv, (i >> 1 | kk) != 0);
-                        if (!kTwoTiles || t == 1) ptx::umma_commit(ptx::smem_u32(&v_empty[g % kStages]));
-                        if (i + 2 >= items) ptx::umma_commit(ptx::smem_u32(&o_full[t]));
+                            ptx::umma_bf16_ts_warp(tmem + kOCol + t * D, tmem + t * KT + kk * 8, va + kk * (16 * 128 >> 4), idesc_pv, (i0 | kk) != 0);
                         // the tensor pipe runs in order: P_t is consumed before S_t is overwritten
-                        if (i + 2 < items) ok = issue_qk(i + 2);
+                        if (i + 2 < items) ok = issue_qk(i + 2, t);
+                        if (!kTwoTiles || t == 1) ptx::umma_commit_warp(ptx::smem_u32(&v_empty[stage]));
+                        if (i + 2 >= items) ptx::umma_commit_warp(ptx::smem_u32(&o_full[t]));
                     }
-                    n_kv += n;
-                    ++n_seg;
-                    w.advance(p, n);
                 }
+                n_kv += n;
+                ++n_seg;
+                w.advance(p, n);
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // ---------------------------------------------------------------- softmax groups
         const int t = warp >> 2;
         const int quarter = warp & 3;
