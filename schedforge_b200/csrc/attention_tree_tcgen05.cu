@@ -12,7 +12,7 @@
 // directly; the pieces of a pair that was cut are kept as (maximum, sum, numerator) and joined by a second kernel.
 //
 // 384 threads, roles as in the prefill kernel: two softmax groups of 128 threads (thread = row = tensor-memory lane),
-// one copy warp, one MMA-issuing thread; S and P share tensor memory columns, P is the A operand of P.V.
+// two copy warps (Q and K, V), one MMA warp; S and P share tensor memory columns, P is the A operand of P.V.
 //   ROWS = 256: the two groups own two 128-row tiles and meet every key tile;
 //   ROWS = 128: both own the same rows and take alternate key tiles, each with its own running maximum and
 //               accumulator; the first group joins them at the end of a piece, out of tensor memory.
@@ -211,12 +211,21 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == 8) {
-            // ------------------------------------------------------------ copies
+        if (warp == 8 || warp == 11) {
+            // ------------------------------------------------------------ copies: warp 8 Q and K, warp 11 V
+            const bool keys = warp == 8;
+            uint64_t* empty = keys ? k_empty : v_empty;
+            uint64_t* full = keys ? k_full : v_full;
+            uint8_t* ring = keys ? k_smem : v_smem;
+            const CUtensorMap* map_pool = keys ? &map_k : &map_v;
+            const CUtensorMap* map_draft = keys ? &map_dk : &map_dv;
             const int boxes = KT / p.box_rows;
             const int box = lane / kHalves, half = lane % kHalves;
             const uint32_t box_bits = (p.box_rows == 128 ? 0xffffu : ((1u << (p.box_rows / 8)) - 1));
             uint32_t n_kv = 0, n_seg = 0;
+            const auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort_flag, status, kCodeTree | 1));
+            };
             bool ok = true;
             while (ok && w.left > 0) {
                 const int n = w.take();
@@ -233,46 +242,39 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                                              : (page * kv.kv_heads + kvh) * kv.block_tokens + (pos - block * kv.block_tokens);
                 };
                 int row = row_of(w.x);
-                ok = ptx::mbar_wait(ptx::smem_u32(q_empty), (n_seg & 1) ^ 1, abort_flag, status, kCodeTree | 1);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                if (lane == 0) {
-                    const uint32_t bar = ptx::smem_u32(q_full);
-                    ptx::mbar_expect_tx(bar, Sh::kQTiles * Sh::kQBytes);
-                    const int q_row = head * p.rows_all + rg * ROWS;
-                    for (int i = 0; i < Sh::kQTiles; ++i)
-                        for (int h = 0; h < kHalves; ++h)
-                            ptx::tma_load_2d(ptx::smem_u32(q_smem + i * Sh::kQBytes + h * kHalfBytes), &map_q, bar, 64 * h, q_row + 128 * i);
+                if (keys) {
+                    ok = wait(q_empty, (n_seg & 1) ^ 1);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        const uint32_t bar = ptx::smem_u32(q_full);
+                        ptx::mbar_expect_tx(bar, Sh::kQTiles * Sh::kQBytes);
+                        const int q_row = head * p.rows_all + rg * ROWS;
+                        for (int i = 0; i < Sh::kQTiles; ++i)
+                            for (int h = 0; h < kHalves; ++h)
+                                ptx::tma_load_2d(ptx::smem_u32(q_smem + i * Sh::kQBytes + h * kHalfBytes), &map_q, bar, 64 * h, q_row + 128 * i);
+                    }
+                    ++n_seg;
                 }
-                ++n_seg;
-                for (int x = w.x; ok && x < w.x + n; ++x, ++n_kv) {
+                for (int x = w.x; x < w.x + n; ++x, ++n_kv) {
                     const int s = n_kv % kStages;
-                    const uint32_t parity = ((n_kv / kStages) & 1) ^ 1;
                     const int mine = row;
                     row = x + 1 < w.x + n ? row_of(x + 1) : -2;    // in flight while this tile waits for its stage
                     const bool draft = x >= n_ctx;
                     const uint32_t missing = __reduce_or_sync(0xffffffffu, mine == -1 ? box_bits << (box * (p.box_rows / 8)) : 0u);
                     const uint32_t loaded = __popc(__ballot_sync(0xffffffffu, mine > -2)) * (p.box_rows * 128);
                     if (missing && lane == 0) atomicOr(status, kCodeDecodeBounds);
-                    const int src = mine == -1 ? p.pool_rows : mine;   // outside the tensor map: reads zeros
-#pragma unroll
-                    for (int kvi = 0; kvi < 2; ++kvi) {
-                        uint64_t* empty = kvi ? v_empty : k_empty;
-                        uint64_t* full = kvi ? v_full : k_full;
-                        uint8_t* stage = (kvi ? v_smem : k_smem) + s * kTileBytes;
-                        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty[s]), parity, abort_flag, status, kCodeTree | 1);
-                        if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
-                        const uint32_t bar = ptx::smem_u32(&full[s]);
-                        if (lane == 0) {
-                            if (!kvi) bad[n_kv % kBadRing] = missing;
-                            ptx::mbar_expect_tx(bar, draft ? kTileBytes : loaded);
-                        }
-                        __syncwarp();
-                        if (draft) {
-                            if (lane < kHalves)
-                                ptx::tma_load_3d(ptx::smem_u32(stage + lane * kHalfBytes), kvi ? &map_dv : &map_dk, bar, 64 * lane, (x - n_ctx) * KT, head);
-                        } else if (mine > -2) {
-                            ptx::tma_load_2d(ptx::smem_u32(stage + half * kHalfBytes + box * p.box_rows * 128), kvi ? &map_v : &map_k, bar, 64 * half, src);
-                        }
+                    ok = wait(&empty[s], ((n_kv / kStages) & 1) ^ 1);
+                    if (!ok) break;
+                    const uint32_t bar = ptx::smem_u32(&full[s]), stage = ptx::smem_u32(ring + s * kTileBytes);
+                    if (lane == 0) {
+                        if (keys) bad[n_kv % kBadRing] = missing;
+                        ptx::mbar_expect_tx(bar, draft ? kTileBytes : loaded);
+                    }
+                    __syncwarp();
+                    if (draft) {
+                        if (lane < kHalves) ptx::tma_load_3d(stage + lane * kHalfBytes, map_draft, bar, 64 * lane, (x - n_ctx) * KT, head);
+                    } else if (mine > -2) {   // (a row outside the tensor map reads zeros)
+                        ptx::tma_load_2d(stage + half * kHalfBytes + box * p.box_rows * 128, map_pool, bar, 64 * half, mine == -1 ? p.pool_rows : mine);
                     }
                 }
                 w.advance(p, n);
