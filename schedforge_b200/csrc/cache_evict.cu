@@ -21,65 +21,121 @@ struct AddParams {
     int* positions;
     const int* query_position;
     int64_t logit_stride;
-    int q_heads, splits, stride;
+    int q_heads, splits, stride, wide;   // wide: rows of weights start on 16 bytes
 };
 
 constexpr int kAddThreads = 256;
-constexpr int kAddChunk = 1024;  // positions per CTA
+constexpr int kAddHeads = 16;      // heads whose statistics are kept at once
 
-// CTA (chunk, K/V head, sequence): maxima and sums of the heads from the split records, then its share of the heads'
-// outputs, then its positions.
+// Grid (group + position chunks, K/V head, sequence).  The first `group` CTAs join the splits of one query head each into its
+// output; the others add the weights of `chunk` positions.  Maxima and sums come from the split records.
 template <class T>
 __global__ void __launch_bounds__(kAddThreads)
-add_weights_kernel(const __grid_constant__ AddParams p) {
-    extern __shared__ float stats[];  // [group] maximum, [group] 1 / sum
+add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
+    __shared__ float factor[128];                  // of every split (output CTAs)
+    __shared__ float half_sum[256];
+    __shared__ float2 stats[kAddHeads];            // maximum, 1 / sum
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.q_heads / kv.kv_heads, record = kv.dim_v + 2;
     grid_dependents_may_launch();
     grid_dependency_wait();
-    const int ctx = kv.length(b);
-    const int first = blockIdx.x * kAddChunk;
     const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
-    if (first >= ctx && blockIdx.x >= group) return;
-    for (int g = warp; g < group; g += kAddThreads / 32) {
+    // maximum and sum of one head, by one warp; factors of the splits for the output
+    const auto statistics = [&](int g, bool keep) -> float2 {
         const float* rec = p.partials + (row0 + g) * p.splits * record;
-        float top = -INFINITY, sum = 0.0F;
-        for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, rec[static_cast<size_t>(s) * record]);
+        float m[4], top = -INFINITY, sum = 0.0F;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = lane + 32 * i;
+            m[i] = s < p.splits ? rec[static_cast<size_t>(s) * record] : -INFINITY;
+            top = fmaxf(top, m[i]);
+        }
         top = warp_max(top);
-        for (int s = lane; s < p.splits; s += 32) {
-            const float m = rec[static_cast<size_t>(s) * record];
-            if (m != -INFINITY) sum += rec[static_cast<size_t>(s) * record + 1] * exp2f(m - top);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = lane + 32 * i;
+            m[i] = m[i] == -INFINITY ? 0.0F : exp2f(m[i] - top);
+            if (s < p.splits) sum += rec[static_cast<size_t>(s) * record + 1] * m[i];
         }
         sum = warp_sum(sum);
-        if (lane == 0) {
-            stats[g] = top == -INFINITY ? 0.0F : top;
-            stats[group + g] = sum > 0.0F ? 1.0F / sum : 0.0F;
+        const float inv = sum > 0.0F ? 1.0F / sum : 0.0F;
+        if (keep) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (lane + 32 * i < p.splits) factor[lane + 32 * i] = m[i] * inv;
         }
-    }
-    __syncthreads();
-    for (int g = blockIdx.x; g < group; g += gridDim.x) {
-        const float* rec = p.partials + (row0 + g) * p.splits * record;
+        return make_float2(top == -INFINITY ? 0.0F : top, inv);
+    };
+    if (blockIdx.x < group) {
+        const int g = blockIdx.x;
+        if (warp == 0) statistics(g, true);
+        __syncthreads();
+        const float* rec = p.partials + (row0 + g) * p.splits * record + 2;
         T* dst = static_cast<T*>(p.out) + (row0 + g) * kv.dim_v;
-        for (int d = threadIdx.x; d < kv.dim_v; d += kAddThreads) {
+        // two halves of the CTA take alternate splits
+        const int half = threadIdx.x >> 7;
+        for (int d0 = 0; d0 < kv.dim_v; d0 += 128) {
+            const int d = d0 + (threadIdx.x & 127);
             float a = 0.0F;
+            if (d < kv.dim_v)
+#pragma unroll 8
+                for (int s = half; s < p.splits; s += 2) {
+                    const float f = factor[s];
+                    if (f != 0.0F) a = fmaf(rec[static_cast<size_t>(s) * record + d], f, a);
+                }
+            half_sum[threadIdx.x] = a;
+            __syncthreads();
+            if (half == 0 && d < kv.dim_v) dst[d] = from_float<T>(a + half_sum[threadIdx.x + 128]);
+            __syncthreads();
+        }
+        return;
+    }
+    const int ctx = kv.length(b);
+    const int first = (blockIdx.x - group) * chunk, end = min(ctx, first + chunk);
+    if (first >= ctx) return;
+    const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
+    for (int g0 = 0; g0 < group; g0 += kAddHeads) {
+        const int heads = min(kAddHeads, group - g0);
+        __syncthreads();
+        for (int g = warp; g < heads; g += kAddThreads / 32) {
+            const float2 s = statistics(g0 + g, false);
+            if (lane == 0) stats[g] = s;
+        }
+        __syncthreads();
+        // (later rounds of a group of more than kAddHeads heads add to what the first left)
+        const float* before = g0 == 0 ? p.weights : p.weights_out;
+        const float* logits = p.logits + (row0 + g0) * p.logit_stride;
+        const auto add_one = [&](int t) {
+            float w = 0.0F;
+            for (int g = 0; g < heads; ++g) w = fmaf(exp2_fast(logits[g * p.logit_stride + t] - stats[g].x), stats[g].y, w);
+            p.weights_out[wrow + t] = (before ? before[wrow + t] : 0.0F) + w;
+        };
+        if (chunk == kAddThreads) {
+            if (first + threadIdx.x < end) add_one(first + threadIdx.x);
+        } else {   // four consecutive positions a thread
+            for (int t = first + 4 * threadIdx.x; t < end; t += 4 * kAddThreads) {
+                if (t + 4 > end || !p.wide) {
+                    for (int i = 0; i < 4; ++i)
+                        if (t + i < end) add_one(t + i);
+                    continue;
+                }
+                float4 w = make_float4(0.0F, 0.0F, 0.0F, 0.0F), sum = w;
+                if (before) w = *reinterpret_cast<const float4*>(before + wrow + t);
 #pragma unroll 4
-            for (int s = 0; s < p.splits; ++s) {
-                const float m = rec[static_cast<size_t>(s) * record];
-                if (m != -INFINITY) a = fmaf(rec[static_cast<size_t>(s) * record + 2 + d], exp2f(m - stats[g]), a);
+                for (int g = 0; g < heads; ++g) {
+                    const float4 x = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t);
+                    const float2 st = stats[g];
+                    sum.x = fmaf(exp2_fast(x.x - st.x), st.y, sum.x);
+                    sum.y = fmaf(exp2_fast(x.y - st.x), st.y, sum.y);
+                    sum.z = fmaf(exp2_fast(x.z - st.x), st.y, sum.z);
+                    sum.w = fmaf(exp2_fast(x.w - st.x), st.y, sum.w);
+                }
+                *reinterpret_cast<float4*>(p.weights_out + wrow + t) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
             }
-            dst[d] = from_float<T>(a * stats[group + g]);
         }
     }
-    const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
-    const int end = min(ctx, first + kAddChunk);
-    for (int t = first + threadIdx.x; t < end; t += kAddThreads) {
-        float w = 0.0F;
-        for (int g = 0; g < group; ++g)
-            w = fmaf(exp2f(p.logits[(row0 + g) * p.logit_stride + t] - stats[g]), stats[group + g], w);
-        p.weights_out[wrow + t] = (p.weights ? p.weights[wrow + t] : 0.0F) + w;
-        if (p.positions && t == ctx - 1) p.positions[wrow + t] = p.query_position[b];
-    }
+    if (p.positions && first <= ctx - 1 && ctx - 1 < end && threadIdx.x == 0) p.positions[wrow + ctx - 1] = p.query_position[b];
 }
 
 struct WeightsLayout {
@@ -376,13 +432,16 @@ sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream 
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
     SFB_TRY(step_attention(p, a->dtype, s));
     const AddParams add{p.kv, p.partials, p.logits, a->weights, a->weights_out, a->out, a->positions, a->query_position,
-                        l.logit_stride, a->q_heads, l.splits, a->weight_stride};
+                        l.logit_stride, a->q_heads, l.splits, a->weight_stride,
+                        a->weight_stride % 4 == 0 && aligned16(a->weights) && aligned16(a->weights_out)};
     const int group = a->q_heads / a->kv_heads;
-    const dim3 grid(ceil_div(p.kv.limit, kAddChunk), a->kv_heads, a->batch);
-    const size_t smem = sizeof(float) * 2 * group;
-    if (smem > 48 * 1024) return fail(SFB_UNSUPPORTED, "decode weights: more than 6144 query heads per K/V head");
-    if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(add_weights_kernel<float>, grid, dim3(kAddThreads), smem, s, add));
-    else SFB_CUDA(launch_dependent(add_weights_kernel<bf16>, grid, dim3(kAddThreads), smem, s, add));
+    // few CTAs: one position a thread; many: long chunks, so that the statistics are read less often
+    const int64_t pairs = static_cast<int64_t>(a->kv_heads) * a->batch;
+    int chunk = kAddThreads;
+    while (chunk < 16 * kAddThreads && pairs * ceil_div(p.kv.limit, chunk) > 4LL * sm_count()) chunk *= 4;
+    const dim3 grid(group + ceil_div(p.kv.limit, chunk), a->kv_heads, a->batch);
+    if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(add_weights_kernel<float>, grid, dim3(kAddThreads), 0, s, add, chunk));
+    else SFB_CUDA(launch_dependent(add_weights_kernel<bf16>, grid, dim3(kAddThreads), 0, s, add, chunk));
     return check_launch("decode_weights_add");
 }
 
