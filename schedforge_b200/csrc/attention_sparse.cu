@@ -8,6 +8,8 @@
 // cannot swap two blocks that are not equal for all purposes.  64-bit arithmetic for all blocks would take longer than
 // their bytes (two products an element and head: 537 million at eight sequences of 128 thousand tokens), so the pass
 // over all blocks sums in 32 bits, and only blocks whose rank those sums leave open are scored again.
+#include <algorithm>
+
 #include "cache_ops.cuh"
 #include "mma_sync.cuh"
 #include "ptx_sm100.cuh"
@@ -704,24 +706,26 @@ select_kernel(const __grid_constant__ SelectParams p) {
 }
 
 struct SparseLayout {
-    int score_stride, splits, chunk_blocks, size_count;
+    int score_stride, size_count;
+    StepPlan step;
     size_t scores, sizes, partials, total;   // exact scores come first
 };
 
-SparseLayout sparse_layout(const sfb_sparse_args& a) {
+SparseLayout sparse_layout(const sfb_sparse_args& a, bool wide) {
     SparseLayout l{};
     const int covered = a.max_blocks * a.block_tokens;
     const int limit = a.max_context < covered ? a.max_context : covered;
     const int blocks = limit > 0 ? ceil_div(limit, a.block_tokens) : 1;
     l.score_stride = blocks;
     const int64_t kept = a.budget_blocks < blocks ? a.budget_blocks : blocks;
-    l.splits = step_splits(a.batch, a.kv_heads, static_cast<int>(kept * a.block_tokens), a.block_tokens, a.splits, &l.chunk_blocks);
+    l.step = step_plan(a.dtype, a.head_dim, a.head_dim_value, a.batch, a.q_heads, a.kv_heads, static_cast<int>(kept * a.block_tokens),
+                       a.block_tokens, a.num_blocks, a.splits, wide);
     const size_t rows = static_cast<size_t>(a.batch) * a.kv_heads;
     l.size_count = ceil_div(blocks, 16);     // no scoring kernel takes fewer blocks a CTA
     l.scores = round_up16(sizeof(double) * rows * blocks);
     l.sizes = l.scores + round_up16(sizeof(float) * rows * blocks);
     l.partials = l.sizes + round_up16(sizeof(float) * rows * l.size_count);
-    l.total = l.partials + sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.splits * (a.head_dim_value + 2);
+    l.total = l.partials + l.step.bytes;
     return l;
 }
 
@@ -764,14 +768,14 @@ sfb_status sfb_k_paged_kv_bounds(const sfb_bounds_args* a, sfb_stream stream) {
 
 size_t sfb_attention_sparse_workspace(const sfb_sparse_args* a) {
     if (check_sparse(a) != SFB_OK) return 0;
-    return sparse_layout(*a).total;
+    return std::max(sparse_layout(*a, true).total, sparse_layout(*a, false).total);   // (the addresses may not be set yet)
 }
 
 sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream stream) {
     SFB_TRY(check_sparse(a));
     SFB_REQUIRE(a->q && a->bounds && a->context_len && a->out && a->selected && a->workspace, "sparse decode: null tensor");
     SFB_REQUIRE(aligned16(a->workspace), "sparse decode: the workspace has to be 16-byte aligned");
-    const SparseLayout l = sparse_layout(*a);
+    const SparseLayout l = sparse_layout(*a, aligned16(a->k_pool) && aligned16(a->v_pool) && aligned16(a->q));
     const PagedView kv = make_view(a->k_pool, a->v_pool, a->block_table, a->context_len, a->kv_heads, a->head_dim, a->head_dim_value,
                                    a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
     cudaStream_t s = as_stream(stream);
@@ -797,13 +801,14 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
         SFB_TRY(check_launch("sparse_select"));
     }
     StepParams p{};
-    p.kv = kv; p.q = a->q; p.out = a->out; p.partials = reinterpret_cast<float*>(ws + l.partials);
+    p.kv = kv; p.q = a->q; p.out = a->out;
+    p.part = step_partials(l.step, a->batch, a->q_heads, a->head_dim_value, ws + l.partials);
     p.selected = a->selected; p.budget = a->budget_blocks;
-    p.batch = a->batch; p.q_heads = a->q_heads; p.splits = l.splits; p.chunk_blocks = l.chunk_blocks;
+    p.batch = a->batch; p.q_heads = a->q_heads; p.chunk_blocks = l.step.chunk_blocks;
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
-    SFB_TRY(step_attention(p, a->dtype, s));
-    if (l.splits == 1) return SFB_OK;
-    return merge_partials({p.partials, a->out, nullptr, a->batch, a->q_heads, 1, a->head_dim_value, l.splits, 1}, a->dtype, s);
+    SFB_TRY(step_attention(p, l.step, a->dtype, s));
+    if (step_joined(l.step)) return SFB_OK;
+    return merge_partials({p.part, kv, a->out, nullptr, a->batch, a->q_heads, 1, a->head_dim_value, 1}, a->dtype, s);
 }
 
 }  // extern "C"

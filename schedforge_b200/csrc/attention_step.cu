@@ -198,10 +198,10 @@ step_kernel(const __grid_constant__ StepParams p) {
             }
         }
         const size_t row = static_cast<size_t>(b) * p.q_heads + head0 + g;
-        if (p.splits == 1 && !p.logits) {
-            if (c >= 2) static_cast<T*>(p.out)[row * kv.dim_v + c - 2] = from_float<T>(sum > 0.0F ? value / sum : value);
+        if (p.part.splits == 1 && !p.logits) {
+            if (c >= 2) static_cast<T*>(p.out)[row * kv.dim_v + c - 2] = from_float<T>(sum == 0.0F ? 0.0F : value / sum);
         } else {
-            p.partials[(row * p.splits + split) * record + c] = c == 0 ? top : c == 1 ? sum : value;
+            p.part.ml[(row * p.part.splits + split) * record + c] = c == 0 ? top : c == 1 ? sum : value;
         }
     }
 }
@@ -211,7 +211,7 @@ sfb_status launch_step(const StepParams& p, cudaStream_t stream) {
     const int group = p.q_heads / p.kv.kv_heads;
     const auto go = [&](auto kernel, int g) -> sfb_status {
         const size_t smem = sizeof(float) * kWarps * g * (p.kv.dim_v + 2);
-        const dim3 grid(p.splits, p.kv.kv_heads * ceil_div(group, g), p.batch);
+        const dim3 grid(p.part.splits, p.kv.kv_heads * ceil_div(group, g), p.batch);
         SFB_CUDA(launch_dependent(kernel, grid, dim3(kWarps * 32), smem, stream, p));
         return check_launch("attention_step");
     };
@@ -232,50 +232,38 @@ sfb_status step_typed(const StepParams& p, cudaStream_t stream) {
     return launch_step<T, 32, true>(p, stream);
 }
 
-// One CTA per output row; thread = output element (strided).
+// One CTA per output row; thread = output element (strided), the two halves of the CTA take alternate pieces.
 template <class T>
-__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ MergeParams p) {
-    __shared__ float weight[128];
+__global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ MergeParams p) {
+    __shared__ float factor[kMaxPieces];
+    __shared__ float other[128];
     const int row = blockIdx.x;
     const int node = row % p.nodes, head = (row / p.nodes) % p.q_heads, b = row / p.nodes / p.q_heads;
     grid_dependents_may_launch();
     grid_dependency_wait();
     if (p.node_count && node >= p.node_count[b]) return;
-    const int record = p.dim_v + 2;
-    const float* rec = p.partials + static_cast<size_t>(row) * p.splits * record;
-    if (threadIdx.x < 32) {
-        float m[4], top = -INFINITY, sum = 0.0F;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = threadIdx.x + 32 * i;
-            m[i] = s < p.splits ? rec[static_cast<size_t>(s) * record] : -INFINITY;
-            top = fmaxf(top, m[i]);
-        }
-        top = warp_max(top);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = threadIdx.x + 32 * i;
-            m[i] = m[i] == -INFINITY ? 0.0F : exp2f(m[i] - top);
-            if (s < p.splits) sum += rec[static_cast<size_t>(s) * record + 1] * m[i];
-        }
-        sum = warp_sum(sum);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = threadIdx.x + 32 * i;
-            if (s < p.splits) weight[s] = sum > 0.0F ? m[i] / sum : 0.0F;
-        }
-    }
+    RowPieces r;
+    if (p.part.span) r = row_pieces(p.part, p.kv.kv_heads, p.q_heads, b, head, p.kv.length(b));
+    else r = {static_cast<size_t>(row) * p.part.splits, 1, p.part.splits};
+    if (p.part.span && r.count == 1) return;   // written by the attention kernel itself
+    if (threadIdx.x < 32) row_statistics(p.part, r, factor);
     __syncthreads();
     T* dst = static_cast<T*>(p.out) + (p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
                                                      : static_cast<size_t>(row)) * p.dim_v;
-    for (int d = threadIdx.x; d < p.dim_v; d += 128) {
+    const int half = threadIdx.x >> 7;
+    for (int d0 = 0; d0 < p.dim_v; d0 += 128) {
+        const int d = d0 + (threadIdx.x & 127);
         float a = 0.0F;
+        if (d < p.dim_v)
 #pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-            const float w = weight[s];
-            if (w != 0.0F) a = fmaf(w, rec[static_cast<size_t>(s) * record + 2 + d], a);
-        }
-        dst[d] = from_float<T>(a);
+            for (int i = half; i < r.count; i += 2) {
+                const float f = factor[i];
+                if (f != 0.0F) a = fmaf(f, p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + d], a);
+            }
+        if (half) other[threadIdx.x & 127] = a;
+        __syncthreads();
+        if (!half && d < p.dim_v) dst[d] = from_float<T>(a + other[threadIdx.x]);
+        __syncthreads();
     }
 }
 
@@ -308,34 +296,59 @@ PagedView make_view(const void* k_pool, const void* v_pool, const int* table, co
     return kv;
 }
 
-// Splits of `tokens` positions, in whole blocks.  Two CTAs per SM keep the memory system full, so a split is as long
-// as that allows (its ramp is paid once and there is less to merge), but at most 2048 positions, which evens out ragged
-// contexts, and at least 64.  At most 128 splits: the merge keeps one weight per split in shared memory.
-int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wanted, int* chunk_blocks) {
+// The tensor-core kernel takes bf16, head_dim = head_dim_value = 128 or 64 and blocks of a multiple of 16 tokens; its
+// CTAs, two per SM, take equal ranges of all work.  The other one cuts every row into splits of whole blocks: as long as
+// two CTAs per SM allow (the ramp of a split is paid once), but at most 2048 positions, which evens out ragged
+// contexts, and at least 64.
+StepPlan step_plan(int dtype, int dim, int dim_v, int batch, int q_heads, int kv_heads, int tokens, int block_tokens, int num_blocks,
+                   int wanted, bool wide) {
+    StepPlan plan{};
     const int blocks = tokens > 0 ? ceil_div(tokens, block_tokens) : 1;
+    const int64_t slots = 2LL * sm_count(), heads = static_cast<int64_t>(batch) * kv_heads;
+    plan.mma = wide && dtype == SFB_BF16 && (dim == 128 || dim == 64) && dim_v == dim && block_tokens % 16 == 0 &&
+               static_cast<int64_t>(num_blocks) * kv_heads * block_tokens < (int64_t{1} << 30);
+    if (plan.mma) {
+        plan.pairs = heads * ceil_div(q_heads / kv_heads, kPieceHeads);
+        const int64_t units = plan.pairs * blocks * (block_tokens / 16);
+        int64_t ctas = wanted > 0 && plan.pairs * wanted < slots ? plan.pairs * wanted : slots;
+        if (ctas > kMaxPieces) ctas = kMaxPieces;
+        plan.ctas = static_cast<int>(units < ctas ? units : ctas);
+        plan.bytes = round_up16(sizeof(float) * (2 + dim_v) * kPieceHeads * static_cast<size_t>(plan.ctas + plan.pairs)) +
+                     sizeof(int2) * static_cast<size_t>(plan.pairs);
+        return plan;
+    }
     int splits = wanted;
     if (splits <= 0) {
-        const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, slots = 2LL * sm_count();
-        splits = static_cast<int>(slots / pairs < tokens / 64 ? slots / pairs : tokens / 64);
+        splits = static_cast<int>(slots / heads < tokens / 64 ? slots / heads : tokens / 64);
         if (splits < ceil_div(tokens, 2048)) splits = ceil_div(tokens, 2048);
     }
     if (splits > 128) splits = 128;
     if (splits > blocks) splits = blocks;
     if (splits < 1) splits = 1;
-    *chunk_blocks = ceil_div(blocks, splits);
-    return ceil_div(blocks, *chunk_blocks);
+    plan.chunk_blocks = ceil_div(blocks, splits);
+    plan.splits = ceil_div(blocks, plan.chunk_blocks);
+    plan.bytes = sizeof(float) * static_cast<size_t>(batch) * q_heads * plan.splits * (dim_v + 2);
+    return plan;
 }
 
-sfb_status step_attention(const StepParams& p, int dtype, cudaStream_t stream) {
-    if (step_mma_supported(p, dtype)) return step_mma(p, stream);
+Partials step_partials(const StepPlan& plan, int batch, int q_heads, int dim_v, void* workspace) {
+    float* ws = static_cast<float*>(workspace);
+    if (!plan.mma) return {ws, ws + 2, nullptr, plan.splits, dim_v + 2, dim_v + 2};
+    const size_t pieces = static_cast<size_t>(plan.ctas + plan.pairs) * kPieceHeads;
+    char* span = reinterpret_cast<char*>(ws) + round_up16(sizeof(float) * (2 + dim_v) * pieces);
+    return {ws + pieces * dim_v, ws, reinterpret_cast<int2*>(span), 0, 2, dim_v};
+}
+
+sfb_status step_attention(const StepParams& p, const StepPlan& plan, int dtype, cudaStream_t stream) {
+    if (plan.mma) return step_mma(p, plan, stream);
     return dtype == SFB_F32 ? step_typed<float>(p, stream) : step_typed<bf16>(p, stream);
 }
 
 sfb_status merge_partials(const MergeParams& p, int dtype, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.nodes;
     const dim3 grid(static_cast<unsigned>(rows));
-    if (dtype == SFB_F32) SFB_CUDA(launch_dependent(merge_kernel<float>, grid, dim3(128), 0, stream, p));
-    else SFB_CUDA(launch_dependent(merge_kernel<bf16>, grid, dim3(128), 0, stream, p));
+    if (dtype == SFB_F32) SFB_CUDA(launch_dependent(merge_kernel<float>, grid, dim3(256), 0, stream, p));
+    else SFB_CUDA(launch_dependent(merge_kernel<bf16>, grid, dim3(256), 0, stream, p));
     return check_launch("attention_merge");
 }
 

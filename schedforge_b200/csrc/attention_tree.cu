@@ -279,8 +279,7 @@ extern "C" {
 size_t sfb_attention_tree_workspace(const sfb_tree_args* a) {
     if (check_tree(a) != SFB_OK) return 0;
     const size_t simt = tree_layout(*a).total;
-    if (!tree_tcgen05_supported(*a)) return simt;
-    const size_t tensor = tree_tcgen05_workspace(*a);   // (pointers that are not 16-byte aligned take the other kernel)
+    const size_t tensor = tree_tcgen05_shape(*a) ? tree_tcgen05_workspace(*a) : 0;   // (the addresses may not be set yet)
     return tensor > simt ? tensor : simt;
 }
 
@@ -303,8 +302,8 @@ sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* a, sfb_stream stream)
     if (tensor) return tree_tcgen05(*a, p, s);
     SFB_TRY(a->dtype == SFB_F32 ? tree_simt<float>(p, s) : tree_simt<bf16>(p, s));
     if (l.splits == 1) return SFB_OK;
-    return merge_partials({p.partials, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, l.splits, a->token_major},
-                          a->dtype, s);
+    const Partials part{p.partials, p.partials + 2, nullptr, l.splits, a->head_dim_value + 2, a->head_dim_value + 2};
+    return merge_partials({part, p.kv, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, a->token_major}, a->dtype, s);
 }
 
 }  // extern "C"

@@ -16,7 +16,8 @@ struct TreeParams {
 };
 
 // bf16, head_dim = head_dim_value = 128 or 64 (attention_tree_tcgen05.cu).
-bool tree_tcgen05_supported(const sfb_tree_args& a);
+bool tree_tcgen05_shape(const sfb_tree_args& a);        // types and sizes
+bool tree_tcgen05_supported(const sfb_tree_args& a);    // and addresses
 size_t tree_tcgen05_workspace(const sfb_tree_args& a);
 sfb_status tree_tcgen05(const sfb_tree_args& a, const TreeParams& t, cudaStream_t stream);
 

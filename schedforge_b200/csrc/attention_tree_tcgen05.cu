@@ -120,8 +120,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     uint32_t* words = reinterpret_cast<uint32_t*>(v_empty + kStages);
     uint32_t* tmem_slot = words;
     volatile uint32_t* abort_flag = words + 1;
-    int* start = reinterpret_cast<int*>(words + 2);   // b, sub, x, tiles in the range
-    volatile uint32_t* bad = words + 6;               // [kBadRing], runs of eight keys without a block
+    int* start = reinterpret_cast<int*>(words + 2);   // even_range: b, sub, x, tiles in the range, tiles of a full range
+    volatile uint32_t* bad = words + 8;               // [kBadRing], runs of eight keys without a block
     const TreeParams& t_ = p.t;
     const PagedView& kv = t_.kv;
     uint32_t* status = kv.status;
@@ -160,43 +160,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     grid_dependents_may_launch();
     grid_dependency_wait();
     if (warp == 10) {
-        // this CTA's range of the tile list
-        const int64_t subs = static_cast<int64_t>(kv.kv_heads) * p.row_groups;
-        int64_t total = 0;
-        for (int b0 = 0; b0 < t_.batch; b0 += 32) {
-            const int b = b0 + lane;
-            int n = b < t_.batch ? tiles_of(kv.length(b), tree_node_count(t_, b)) : 0;
-            total += __reduce_add_sync(0xffffffffu, n);
-        }
-        total *= subs;
-        int64_t per = (total + gridDim.x - 1) / gridDim.x;
-        if (per < 1) per = 1;
-        const int64_t first = blockIdx.x * per;
-        const int64_t mine = first < total ? (total - first < per ? total - first : per) : 0;
-        int64_t before = 0;
-        if (mine > 0) {
-            for (int b0 = 0; b0 < t_.batch; b0 += 32) {
-                const int b = b0 + lane;
-                const int n = b < t_.batch ? tiles_of(kv.length(b), tree_node_count(t_, b)) : 0;
-                int sum = n;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += v;
-                }
-                const int64_t end = before + sum * subs, begin = end - n * subs;
-                const bool here = n > 0 && begin <= first && first < end;
-                if (here) {
-                    const int64_t off = first - begin;
-                    start[0] = b;
-                    start[1] = static_cast<int>(off / n);
-                    start[2] = static_cast<int>(off % n);
-                }
-                if (__any_sync(0xffffffffu, here)) break;
-                before += __shfl_sync(0xffffffffu, sum, 31) * subs;
-            }
-        }
-        if (lane == 0) start[3] = static_cast<int>(mine);
+        even_range(t_.batch, static_cast<int64_t>(kv.kv_heads) * p.row_groups, 1,
+                   [&](int b) { return tiles_of(kv.length(b), tree_node_count(t_, b)); }, start);
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -568,8 +533,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ptx::mbar_arrive(ptx::smem_u32(o_free));
             }
             if (threadIdx.x == 0 && w.x == 0) {   // (one thread per pair: the owner of its first tile)
-                // the range length is the same for all CTAs but the last, so the last CTA of the pair follows from it
-                const int64_t per = start[3];
+                // (all ranges but the last have one length: the last CTA of the pair follows from it)
+                const int64_t per = start[4];
                 const int64_t beyond = w.tiles - n;
                 p.pair_span[pair] = make_int2(blockIdx.x, static_cast<int>(blockIdx.x + (beyond + per - 1) / per));
             }
@@ -677,15 +642,18 @@ sfb_status launch_tc(const sfb_tree_args& a, const TcLayout& l, TreeTcParams& p,
 
 }  // namespace
 
-bool tree_tcgen05_supported(const sfb_tree_args& a) {
+bool tree_tcgen05_shape(const sfb_tree_args& a) {
     const int64_t pool_rows = static_cast<int64_t>(a.num_blocks) * a.kv_heads * a.block_tokens;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.nodes;
     return a.dtype == SFB_BF16 && (a.head_dim == 128 || a.head_dim == 64) && a.head_dim_value == a.head_dim &&
-           a.block_tokens % 8 == 0 && pool_rows < (int64_t{1} << 30) && rows < (int64_t{1} << 26) && aligned16(a.q) &&
-           aligned16(a.k_pool) && aligned16(a.v_pool) && aligned16(a.draft_k) && aligned16(a.draft_v) && aligned16(a.out);
+           a.block_tokens % 8 == 0 && pool_rows < (int64_t{1} << 30) && rows < (int64_t{1} << 26);
 }
 
-// (by type, sizes and layout alone: the size is asked for before the addresses are known)
+bool tree_tcgen05_supported(const sfb_tree_args& a) {
+    return tree_tcgen05_shape(a) && aligned16(a.q) && aligned16(a.k_pool) && aligned16(a.v_pool) && aligned16(a.draft_k) &&
+           aligned16(a.draft_v) && aligned16(a.out);
+}
+
 size_t tree_tcgen05_workspace(const sfb_tree_args& a) { return tc_layout(a).total; }
 
 sfb_status tree_tcgen05(const sfb_tree_args& a, const TreeParams& t, cudaStream_t stream) {

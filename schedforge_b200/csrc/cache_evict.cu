@@ -5,6 +5,8 @@
 // Eviction: one CTA per (sequence, K/V head) finds the threshold of the kept weights and lists the kept rows that
 // lie behind the new length and the freed slots before it.  There are equally many, and no slot is in both lists, so the
 // rows can move in any order and with any parallelism.
+#include <algorithm>
+
 #include "cache_ops.cuh"
 #include "select.cuh"
 
@@ -15,74 +17,50 @@ namespace {
 
 struct AddParams {
     PagedView kv;
-    const float *partials, *logits, *weights;
+    Partials part;
+    const float *logits, *weights;
     float* weights_out;
     void* out;
     int* positions;
     const int* query_position;
     int64_t logit_stride;
-    int q_heads, splits, stride, wide;   // wide: rows of weights start on 16 bytes
+    int q_heads, stride, wide;   // wide: rows of weights start on 16 bytes
 };
 
 constexpr int kAddThreads = 256;
 constexpr int kAddHeads = 16;      // heads whose statistics are kept at once
 
 // Grid (group + position chunks, K/V head, sequence).  The first `group` CTAs join the splits of one query head each into its
-// output; the others add the weights of `chunk` positions.  Maxima and sums come from the split records.
+// output; the others add the weights of `chunk` positions.  Maxima and sums come from the pieces.
 template <class T>
 __global__ void __launch_bounds__(kAddThreads)
 add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
-    __shared__ float factor[128];                  // of every split (output CTAs)
+    __shared__ float factor[kMaxPieces];           // of every piece (output CTAs)
     __shared__ float half_sum[256];
     __shared__ float2 stats[kAddHeads];            // maximum, 1 / sum
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int group = p.q_heads / kv.kv_heads, record = kv.dim_v + 2;
+    const int group = p.q_heads / kv.kv_heads;
     grid_dependents_may_launch();
     grid_dependency_wait();
     const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
-    // maximum and sum of one head, by one warp; factors of the splits for the output
-    const auto statistics = [&](int g, bool keep) -> float2 {
-        const float* rec = p.partials + (row0 + g) * p.splits * record;
-        float m[4], top = -INFINITY, sum = 0.0F;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = lane + 32 * i;
-            m[i] = s < p.splits ? rec[static_cast<size_t>(s) * record] : -INFINITY;
-            top = fmaxf(top, m[i]);
-        }
-        top = warp_max(top);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = lane + 32 * i;
-            m[i] = m[i] == -INFINITY ? 0.0F : exp2f(m[i] - top);
-            if (s < p.splits) sum += rec[static_cast<size_t>(s) * record + 1] * m[i];
-        }
-        sum = warp_sum(sum);
-        const float inv = sum > 0.0F ? 1.0F / sum : 0.0F;
-        if (keep) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < p.splits) factor[lane + 32 * i] = m[i] * inv;
-        }
-        return make_float2(top == -INFINITY ? 0.0F : top, inv);
-    };
+    const int ctx = kv.length(b);
     if (blockIdx.x < group) {
         const int g = blockIdx.x;
-        if (warp == 0) statistics(g, true);
+        const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g, ctx);
+        if (warp == 0) row_statistics(p.part, r, factor);
         __syncthreads();
-        const float* rec = p.partials + (row0 + g) * p.splits * record + 2;
         T* dst = static_cast<T*>(p.out) + (row0 + g) * kv.dim_v;
-        // two halves of the CTA take alternate splits
+        // two halves of the CTA take alternate pieces
         const int half = threadIdx.x >> 7;
         for (int d0 = 0; d0 < kv.dim_v; d0 += 128) {
             const int d = d0 + (threadIdx.x & 127);
             float a = 0.0F;
             if (d < kv.dim_v)
 #pragma unroll 8
-                for (int s = half; s < p.splits; s += 2) {
-                    const float f = factor[s];
-                    if (f != 0.0F) a = fmaf(rec[static_cast<size_t>(s) * record + d], f, a);
+                for (int i = half; i < r.count; i += 2) {
+                    const float f = factor[i];
+                    if (f != 0.0F) a = fmaf(p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + d], f, a);
                 }
             half_sum[threadIdx.x] = a;
             __syncthreads();
@@ -91,7 +69,6 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
         }
         return;
     }
-    const int ctx = kv.length(b);
     const int first = (blockIdx.x - group) * chunk, end = min(ctx, first + chunk);
     if (first >= ctx) return;
     const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
@@ -99,7 +76,7 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
         const int heads = min(kAddHeads, group - g0);
         __syncthreads();
         for (int g = warp; g < heads; g += kAddThreads / 32) {
-            const float2 s = statistics(g0 + g, false);
+            const float2 s = row_statistics(p.part, row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx), nullptr);
             if (lane == 0) stats[g] = s;
         }
         __syncthreads();
@@ -139,18 +116,19 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
 }
 
 struct WeightsLayout {
-    int splits, chunk_blocks;
+    StepPlan step;
     int64_t logit_stride;
     size_t partials, total;
 };
 
-WeightsLayout weights_layout(const sfb_weights_args& a) {
+WeightsLayout weights_layout(const sfb_weights_args& a, bool wide) {
     WeightsLayout l{};
     const int covered = a.max_blocks * a.block_tokens;
     const int limit = a.max_context < covered ? a.max_context : covered;
-    l.splits = step_splits(a.batch, a.kv_heads, limit, a.block_tokens, a.splits, &l.chunk_blocks);
+    l.step = step_plan(a.dtype, a.head_dim, a.head_dim_value, a.batch, a.q_heads, a.kv_heads, limit, a.block_tokens, a.num_blocks,
+                       a.splits, wide);
     l.logit_stride = (limit + 3) & ~3;
-    l.partials = round_up16(sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.splits * (a.head_dim_value + 2));
+    l.partials = round_up16(l.step.bytes);
     l.total = l.partials + sizeof(float) * static_cast<size_t>(a.batch) * a.q_heads * l.logit_stride;
     return l;
 }
@@ -411,7 +389,7 @@ extern "C" {
 
 size_t sfb_attention_weights_workspace(const sfb_weights_args* a) {
     if (check_weights(a) != SFB_OK) return 0;
-    return weights_layout(*a).total;
+    return std::max(weights_layout(*a, true).total, weights_layout(*a, false).total);   // (the addresses may not be set yet)
 }
 
 sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream stream) {
@@ -419,20 +397,20 @@ sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream 
     SFB_REQUIRE(a->q && a->context_len && a->out && a->weights_out && a->workspace, "decode weights: null tensor");
     SFB_REQUIRE(!a->positions || a->query_position, "decode weights: positions without query_position");
     SFB_REQUIRE(aligned16(a->workspace), "decode weights: the workspace has to be 16-byte aligned");
-    const WeightsLayout l = weights_layout(*a);
+    const WeightsLayout l = weights_layout(*a, aligned16(a->k_pool) && aligned16(a->v_pool) && aligned16(a->q));
     cudaStream_t s = as_stream(stream);
     StepParams p{};
     p.kv = make_view(a->k_pool, a->v_pool, a->block_table, a->context_len, a->kv_heads, a->head_dim, a->head_dim_value,
                      a->block_tokens, a->max_blocks, a->num_blocks, a->max_context);
     p.q = a->q; p.out = a->out;
-    p.partials = static_cast<float*>(a->workspace);
+    p.part = step_partials(l.step, a->batch, a->q_heads, a->head_dim_value, a->workspace);
     p.logits = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + l.partials);
     p.logit_stride = l.logit_stride;
-    p.batch = a->batch; p.q_heads = a->q_heads; p.splits = l.splits; p.chunk_blocks = l.chunk_blocks;
+    p.batch = a->batch; p.q_heads = a->q_heads; p.chunk_blocks = l.step.chunk_blocks;
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
-    SFB_TRY(step_attention(p, a->dtype, s));
-    const AddParams add{p.kv, p.partials, p.logits, a->weights, a->weights_out, a->out, a->positions, a->query_position,
-                        l.logit_stride, a->q_heads, l.splits, a->weight_stride,
+    SFB_TRY(step_attention(p, l.step, a->dtype, s));
+    const AddParams add{p.kv, p.part, p.logits, a->weights, a->weights_out, a->out, a->positions, a->query_position,
+                        l.logit_stride, a->q_heads, a->weight_stride,
                         a->weight_stride % 4 == 0 && aligned16(a->weights) && aligned16(a->weights_out)};
     const int group = a->q_heads / a->kv_heads;
     // few CTAs: one position a thread; many: long chunks, so that the statistics are read less often

@@ -55,36 +55,59 @@ PagedView make_view(const void* k_pool, const void* v_pool, const int* table, co
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline size_t round_up16(size_t n) { return (n + 15) & ~size_t(15); }
 
+// ---- partial results -------------------------------------------------------------------------------------------------
+// A query row's attention may be cut along the keys; each piece leaves its maximum (base-2 units), its sum and its
+// numerator.  Two arrangements: a fixed number of splits per row, or, where every CTA takes an equal range of all rows'
+// work, the pieces of CTAs first..last of the row's (sequence, K/V head) pair, piece = CTA + pair.
+struct Partials {
+    float* ml;         // maximum and sum of index i at ml[i * ml_step]
+    float* o;          // numerator of index i at o[i * o_step]
+    int2* span;        // first and last CTA of every pair; nullptr: fixed splits
+    int splits, ml_step, o_step;
+};
+constexpr int kPieceHeads = 8;    // query heads per pair in the arrangement by CTAs
+constexpr int kMaxPieces = 512;   // pieces of one row (the joining kernels keep a factor for each)
+
 // ---- one query token per sequence --------------------------------------------------------------------------------
 // Attention of the query heads of one K/V head over the blocks of a list (selected != nullptr) or over the whole
-// context.  Split s of a (sequence, K/V head) covers list entries [s * chunk_blocks, (s + 1) * chunk_blocks) and leaves
-// (maximum, sum, numerator) in partials; maxima and logits are in base-2 units.  logits != nullptr: the scaled logit of
-// every position is kept there.
+// context.  logits != nullptr: the scaled logit of every position is kept there (base-2 units), and every row leaves a
+// partial result.
 struct StepParams {
     PagedView kv;
     const void* q;
     void* out;
-    float* partials;
+    Partials part;
     float* logits;          // [batch, q_heads, logit_stride]
     const int* selected;    // [batch, kv_heads, budget]
     int64_t logit_stride;
     int budget;
-    int batch, q_heads, splits, chunk_blocks;
+    int batch, q_heads, chunk_blocks;
     float scale_log2;
 };
 
-bool step_mma_supported(const StepParams& p, int dtype);   // attention_step_mma.cu
-sfb_status step_mma(const StepParams& p, cudaStream_t stream);
-sfb_status step_attention(const StepParams& p, int dtype, cudaStream_t stream);
-int step_splits(int batch, int kv_heads, int tokens, int block_tokens, int wanted, int* chunk_blocks);
+// How a step is cut; decided by type, sizes and the wanted splits alone, so that the workspace can be sized without
+// the tensors.
+struct StepPlan {
+    bool mma;            // attention_step_mma.cu: even ranges; else attention_step.cu: fixed splits
+    int ctas, splits, chunk_blocks;
+    int64_t pairs;
+    size_t bytes;        // of the partial results
+};
+StepPlan step_plan(int dtype, int dim, int dim_v, int batch, int q_heads, int kv_heads, int tokens, int block_tokens, int num_blocks,
+                   int wanted, bool wide);
+Partials step_partials(const StepPlan& plan, int batch, int q_heads, int dim_v, void* workspace);
+sfb_status step_attention(const StepParams& p, const StepPlan& plan, int dtype, cudaStream_t stream);
+sfb_status step_mma(const StepParams& p, const StepPlan& plan, cudaStream_t stream);
+inline bool step_joined(const StepPlan& plan) { return !plan.mma && plan.splits == 1; }   // nothing is left to join
 
-// ---- merge of split partials ---------------------------------------------------------------------------------------
+// ---- joining --------------------------------------------------------------------------------------------------------
 // Rows are (b, q_head, node); nodes == 1 and node_count == nullptr for single-token decode.
 struct MergeParams {
-    const float* partials;  // [rows][splits][dim_v + 2]
+    Partials part;
+    PagedView kv;            // lengths and heads (arrangement by CTAs)
     void* out;
     const int* node_count;
-    int batch, q_heads, nodes, dim_v, splits, token_major;
+    int batch, q_heads, nodes, dim_v, token_major;
 };
 sfb_status merge_partials(const MergeParams& p, int dtype, cudaStream_t stream);
 
@@ -116,6 +139,84 @@ template <> struct Raw8<bf16> {
         }
     }
 };
+
+// Where the pieces of query row (b, head) lie: indices first + i * step, i < count.  ctx: the sequence's length.
+struct RowPieces {
+    size_t first;
+    int step, count;
+};
+__device__ __forceinline__ RowPieces row_pieces(const Partials& part, int kv_heads, int q_heads, int b, int head, int ctx) {
+    if (!part.span) return {(static_cast<size_t>(b) * q_heads + head) * part.splits, 1, part.splits};
+    if (ctx == 0) return {0, 0, 0};
+    const int group = q_heads / kv_heads, chunks = (group + kPieceHeads - 1) / kPieceHeads;
+    const int in_group = head % group;
+    const size_t pair = (static_cast<size_t>(b) * kv_heads + head / group) * chunks + in_group / kPieceHeads;
+    const int2 span = part.span[pair];
+    return {(span.x + pair) * kPieceHeads + in_group % kPieceHeads, kPieceHeads, min(span.y - span.x + 1, kMaxPieces)};
+}
+
+// Maximum and 1 / sum of a row (0 for an empty one) out of its pieces, by one warp; factors != nullptr: the factor of
+// every piece.
+__device__ __forceinline__ float2 row_statistics(const Partials& part, const RowPieces& r, float* factors) {
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY, sum = 0.0F;
+    for (int i = lane; i < r.count; i += 32) top = fmaxf(top, part.ml[(r.first + static_cast<size_t>(i) * r.step) * part.ml_step]);
+    top = warp_max(top);
+    if (top == -INFINITY) top = 0.0F;
+    for (int i = lane; i < r.count; i += 32) {
+        const float* ml = part.ml + (r.first + static_cast<size_t>(i) * r.step) * part.ml_step;
+        const float f = ml[0] == -INFINITY ? 0.0F : exp2f(ml[0] - top);
+        sum += ml[1] * f;
+        if (factors) factors[i] = f;
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.0F ? 0.0F : 1.0F / sum;
+    if (factors)
+        for (int i = lane; i < r.count; i += 32) factors[i] *= inv;   // (its own entries)
+    return make_float2(top, inv);
+}
+
+// The range of CTA blockIdx.x when the work units of `batch` sequences (count(b) units for each of their `subs` pairs)
+// are laid end to end and cut into gridDim.x equal ranges (a multiple of `granule` units each).  One whole warp calls it.  out: sequence, pair inside
+// it, unit inside the pair, units of this CTA (0: none), units of a full range.
+template <class Count>
+__device__ __forceinline__ void even_range(int batch, int64_t subs, int granule, Count count, int* out) {
+    const int lane = threadIdx.x & 31;
+    const int first_count = lane < batch ? count(lane) : 0;   // (the only ones up to 32 sequences)
+    int64_t total = __reduce_add_sync(0xffffffffu, first_count);
+    for (int b0 = 32; b0 < batch; b0 += 32) total += __reduce_add_sync(0xffffffffu, b0 + lane < batch ? count(b0 + lane) : 0);
+    total *= subs;
+    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    per = (per + granule - 1) / granule * granule;
+    if (per < granule) per = granule;
+    const int64_t first = blockIdx.x * per;
+    const int64_t mine = first < total ? (total - first < per ? total - first : per) : 0;
+    if (mine > 0) {
+        int64_t before = 0;
+        for (int b0 = 0; b0 < batch; b0 += 32) {
+            const int n = b0 == 0 ? first_count : (b0 + lane < batch ? count(b0 + lane) : 0);
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const int64_t end = before + sum * subs, begin = end - n * subs;
+            const bool here = n > 0 && begin <= first && first < end;
+            if (here) {
+                out[0] = b0 + lane;
+                out[1] = static_cast<int>((first - begin) / n);
+                out[2] = static_cast<int>((first - begin) % n);
+            }
+            if (__any_sync(0xffffffffu, here)) break;
+            before += __shfl_sync(0xffffffffu, sum, 31) * subs;
+        }
+    }
+    if (lane == 0) {
+        out[3] = static_cast<int>(mine);
+        out[4] = static_cast<int>(per);
+    }
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

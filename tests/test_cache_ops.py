@@ -671,10 +671,10 @@ def test_workspace_sizes_need_no_device(sfb):
     a.budget = 1000
     assert lib.sfb_paged_kv_evict_workspace(C.byref(a)) == 16 + 2 * 20
     w = valid_args("weights")
-    w.splits = 1
+    w.splits, w.dtype = 1, L.F32
     assert lib.sfb_attention_weights_workspace(C.byref(w)) == 2 * 2 * 66 * 4 + 2 * 2 * 20 * 4
     s = valid_args("sparse")
-    s.splits = 1
+    s.splits, s.dtype = 1, L.F32
     assert lib.sfb_attention_sparse_workspace(C.byref(s)) == 2 * 2 * 8 + 16 + 16 + 2 * 2 * 66 * 4   # exact, 32-bit, sizes, partials
     s.q_heads = 3
     s.kv_heads = 2
