@@ -80,7 +80,7 @@ struct ScoreParams {
     const void *q, *bounds;
     float* scores;        // [batch * kv_heads][score_stride], summed in 32 bits
     float* sizes;         // [batch * kv_heads][gridDim.x]: the largest |bound| among the blocks of a CTA
-    int q_heads, score_stride, batch_blocks, cta_blocks;
+    int q_heads, score_stride, batch_blocks, cta_blocks, heads;   // heads: K/V heads a CTA takes
 };
 
 // Any layout: one warp per block, lane owns every 32nd element.
@@ -323,24 +323,40 @@ score_vec_kernel(const __grid_constant__ ScoreParams p) {
         p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
 }
 
-// bf16, dim % 16 == 0: the same ring, with the products on the tensor path.  16 blocks are the rows of A (low and high
-// side by side are 2 dim columns), q- and q+ of up to eight heads the columns of B: 2 dim / 16 instructions replace
-// 4 dim multiply-adds a block and head, which bounded the form above (sparse decode of 8 x 131072 tokens: 90 us of
-// scores).  Rows are 16 bytes further apart than their length, so that ldmatrix meets no bank twice.
+// bf16, dim % 16 == 0: the products on the tensor path.  16 blocks are the rows of A (low and high side by side are
+// 2 dim columns), q- and q+ of up to eight heads the columns of B: 2 dim / 16 instructions replace 4 dim multiply-adds a
+// block and head.  A CTA takes `heads` K/V heads of a sequence at once (all of them up to eight): their bounds lie side by
+// side, so a block is one copy of heads * 4 dim bytes (4 KB at eight heads of 128; copies of one head's 512 bytes ran at
+// 3.8 TB/s).  A copy warp keeps three stages of 16 * (warps / heads) blocks in flight; each of the other warps takes one head
+// of 16 blocks of every stage.  Rows are 16 bytes further apart than their length, so that ldmatrix meets no bank twice.
 template <int KS>   // steps of 16 columns in one half: dim / 16
-__global__ void __launch_bounds__(kScoreWarps * 32)
+struct ScoreMma {
+    static constexpr int D = KS * 16;
+    static constexpr int kWarps = KS <= 8 ? 8 : 4;       // that compute
+    static constexpr int kMaxBlocks = kWarps * 16;       // per stage
+};
+
+template <int KS>
+__global__ void __launch_bounds__((ScoreMma<KS>::kWarps + 1) * 32)
 score_mma_kernel(const __grid_constant__ ScoreParams p) {
-    constexpr int kBatch = 16, D = KS * 16, kRowBytes = 4 * D + 16;
-    extern __shared__ __align__(16) uint8_t score_smem[];   // [warps][stages][16][kRowBytes]
-    __shared__ uint64_t bars[kScoreWarps][kScoreStages];
+    using Sh = ScoreMma<KS>;
+    constexpr int D = Sh::D, kWarps = Sh::kWarps, kWords = (Sh::kMaxBlocks + 31) / 32;
+    extern __shared__ __align__(16) uint8_t score_smem[];   // [stages][stage blocks][heads * 4 D + 16]
+    __shared__ uint64_t full_bar[kScoreStages], empty_bar[kScoreStages];
+    __shared__ unsigned there[kScoreStages][kWords];        // blocks of the stage that exist
     __shared__ uint32_t abort_word;
-    __shared__ float size_of[kScoreWarps];
+    __shared__ float size_of[kWarps];
     const PagedView& kv = p.kv;
-    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
+    const int heads = p.heads, subs = kWarps / heads, stage_blocks = subs * 16;
+    const uint32_t copy_bytes = heads * 4 * D, row_bytes = copy_bytes + 16;
+    const int b = blockIdx.z, head0 = blockIdx.y * heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
     const int group = p.q_heads / kv.kv_heads;
-    if (lane == 0) {
-        for (int s = 0; s < kScoreStages; ++s) ptx::mbar_init(ptx::smem_u32(&bars[warp][s]), 1);
-        if (warp == 0) abort_word = 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kScoreStages; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), heads * subs);
+        }
+        abort_word = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
     }
@@ -349,115 +365,134 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
     __syncthreads();
     const int ctx = kv.length(b);
     const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
-    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
-    const int last = min(blocks, (static_cast<int>(blockIdx.x) + 1) * p.cta_blocks);
-    const int begin = blockIdx.x * p.cta_blocks + warp * kBatch;
-    constexpr int kStep = kScoreWarps * kBatch;
-    const int* table = kv.table + static_cast<size_t>(b) * kv.max_blocks;
-    uint8_t* mine = score_smem + warp * kScoreStages * kBatch * kRowBytes;
-    const auto page_of = [&](int base) -> int {   // lane i < 16 brings block i of a batch
-        const int block = base + lane;
-        if (lane >= kBatch || block >= last) return -2;
-        const int page = table[block];
-        if (page >= 0 && page < kv.num_blocks) return page;
-        atomicOr(kv.status, kCodeDecodeBounds);
-        return -1;
-    };
-    const auto issue = [&](int stage, int page) -> unsigned {
-        const unsigned present = __ballot_sync(0xffffffffu, page >= 0);
-        const uint32_t bar = ptx::smem_u32(&bars[warp][stage]);
-        if (lane == 0) ptx::mbar_expect_tx(bar, __popc(present) * 4 * D);
-        __syncwarp();
-        if (page >= 0)
-            bulk_load(ptx::smem_u32(mine + (stage * kBatch + lane) * kRowBytes),
-                      static_cast<const bf16*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * D, 4 * D, bar);
-        return present;
-    };
-    unsigned there[kScoreStages];
+    const int begin = blockIdx.x * p.cta_blocks, last = min(blocks, begin + p.cta_blocks);
+    float size = 0.0F;
+    if (warp == kWarps) {
+        // ---------------------------------------------------------------- copies: lane i brings blocks i, i + 32, ...
+        const int* table = kv.table + static_cast<size_t>(b) * kv.max_blocks;
+        int next[kWords];
+        const auto fetch = [&](int base) {
 #pragma unroll
-    for (int s = 0; s < kScoreStages; ++s) there[s] = begin + s * kStep < last ? issue(s, page_of(begin + s * kStep)) : 0u;
-    // B fragments: columns are heads, rows k: q- for the low half, q+ for the high half
-    uint32_t qb[2 * KS][2];
-    const auto load_heads = [&](int g0) {
-        const int g = g0 + (lane >> 2);
-        const bf16* q = static_cast<const bf16*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + min(g, group - 1)) * D;
-        const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0F, 0.0F);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(q + 16 * k + 8 * h + 2 * quad);
-                const __nv_bfloat162 neg = __hmin2_nan(v, zero), pos = __hmax2_nan(v, zero);   // (a NaN in q reaches every score)
-                qb[k][h] = *reinterpret_cast<const uint32_t*>(&neg);
-                qb[KS + k][h] = *reinterpret_cast<const uint32_t*>(&pos);
-            }
-    };
-    load_heads(0);
-    __nv_bfloat162 most = __floats2bfloat162_rn(0.0F, 0.0F), least = most;
-    int stage = 0, phase = 0;
-    for (int base = begin; base < last; base += kStep) {
-        const int ahead = base + kScoreStages * kStep;
-        const int next_page = ahead < last ? page_of(ahead) : -2;     // in flight while this batch is scored
-        if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bars[warp][stage]), phase, &abort_word, kv.status, kCodeScore))) break;
-        unsigned present = 0;
-#pragma unroll
-        for (int s = 0; s < kScoreStages; ++s)
-            if (s == stage) present = there[s];
-        const uint32_t rows = ptx::smem_u32(mine + stage * kBatch * kRowBytes) + (lane & 15) * kRowBytes + (lane >> 4) * 16;
-        float best[2] = {-INFINITY, -INFINITY};   // rows lane / 4 and lane / 4 + 8
-#pragma unroll 1
-        for (int g0 = 0; g0 < group; g0 += 8) {
-            if (group > 8) load_heads(g0);
-            float c[2][4] = {};   // two chains: even and odd steps
-#pragma unroll
-            for (int k = 0; k < 2 * KS; ++k) {
-                uint32_t a[4];
-                ldmatrix_x4(rows + k * 32, a);
-                mma_bf16(c[k & 1], a, qb[k][0], qb[k][1]);
-                if (g0 == 0) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool ok = present >> ((lane >> 2) + 8 * (i & 1)) & 1u;   // (a row that was not loaded holds anything)
-                        const uint32_t word = ok ? a[i] : 0u;
-                        const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&word);
-                        if (k < KS) least = __hmin2(least, v);
-                        else most = __hmax2(most, v);
-                    }
+            for (int j = 0; j < kWords; ++j) {
+                const int at = lane + 32 * j;
+                next[j] = -2;
+                if (at < stage_blocks && base + at < last) {
+                    const int page = table[base + at];
+                    next[j] = page >= 0 && page < kv.num_blocks ? page : -1;
+                    if (next[j] < 0) atomicOr(kv.status, kCodeDecodeBounds);
                 }
             }
-            // columns 2 quad and 2 quad + 1 of the heads
+        };
+        fetch(begin);
+        int n = 0;
+        for (int base = begin; base < last; base += stage_blocks, ++n) {
+            int page[kWords];
+            unsigned count = 0, present[kWords];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float x = g0 + 2 * quad < group ? c[0][2 * r] + c[1][2 * r] : -INFINITY;
-                const float y = g0 + 2 * quad + 1 < group ? c[0][2 * r + 1] + c[1][2 * r + 1] : -INFINITY;
-                best[r] = fmaxf(best[r], fmaxf(x, y));
+            for (int j = 0; j < kWords; ++j) {
+                page[j] = next[j];
+                present[j] = __ballot_sync(0xffffffffu, page[j] >= 0);
+                count += __popc(present[j]);
             }
-        }
+            fetch(base + stage_blocks);      // in flight while this stage waits
+            const int s = n % kScoreStages;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[s]), ((n / kScoreStages) & 1) ^ 1, &abort_word, kv.status, kCodeScore))) break;
+            const uint32_t bar = ptx::smem_u32(&full_bar[s]);
+            if (lane == 0) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
-            best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
-            const int at = (lane >> 2) + 8 * r;
-            if (quad == 0 && base + at < last)
-                p.scores[row * p.score_stride + base + at] = present >> at & 1u ? best[r] : __uint_as_float(0x7fc00000u);
-        }
-        __syncwarp();
-        if (ahead < last) {
-            const unsigned now = issue(stage, next_page);
+                for (int j = 0; j < kWords; ++j) there[s][j] = present[j];
+                ptx::mbar_expect_tx(bar, count * copy_bytes);
+            }
+            __syncwarp();
 #pragma unroll
-            for (int s = 0; s < kScoreStages; ++s)
-                if (s == stage) there[s] = now;
+            for (int j = 0; j < kWords; ++j)
+                if (page[j] >= 0)
+                    bulk_load(ptx::smem_u32(score_smem + (static_cast<size_t>(s) * stage_blocks + lane + 32 * j) * row_bytes),
+                              static_cast<const bf16*>(p.bounds) + (static_cast<int64_t>(page[j]) * kv.kv_heads + head0) * 2 * D, copy_bytes, bar);
         }
-        if (++stage == kScoreStages) { stage = 0; phase ^= 1; }
+    } else if (warp < heads * subs) {
+        const int kvh = head0 + warp % heads, sub = warp / heads;
+        const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+        // B fragments: columns are heads, rows k: q- for the low half, q+ for the high half
+        uint32_t qb[2 * KS][2];
+        const auto load_heads = [&](int g0) {
+            const int g = g0 + (lane >> 2);
+            const bf16* q = static_cast<const bf16*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + min(g, group - 1)) * D;
+            const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0F, 0.0F);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(q + 16 * k + 8 * h + 2 * quad);
+                    const __nv_bfloat162 neg = __hmin2_nan(v, zero), pos = __hmax2_nan(v, zero);   // (a NaN in q reaches every score)
+                    qb[k][h] = *reinterpret_cast<const uint32_t*>(&neg);
+                    qb[KS + k][h] = *reinterpret_cast<const uint32_t*>(&pos);
+                }
+        };
+        load_heads(0);
+        __nv_bfloat162 most = __floats2bfloat162_rn(0.0F, 0.0F), least = most;
+        int n = 0;
+        for (int base = begin; base < last; base += stage_blocks, ++n) {
+            const int s = n % kScoreStages;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&full_bar[s]), (n / kScoreStages) & 1, &abort_word, kv.status, kCodeScore))) break;
+            const int first = base + sub * 16;
+            if (first < last) {
+                const unsigned present = there[s][sub >> 1] >> ((sub & 1) * 16);
+                const uint32_t rows = ptx::smem_u32(score_smem) + (s * stage_blocks + sub * 16 + (lane & 15)) * row_bytes +
+                                      (warp % heads) * 4 * D + (lane >> 4) * 16;
+                float best[2] = {-INFINITY, -INFINITY};   // rows lane / 4 and lane / 4 + 8
+#pragma unroll 1
+                for (int g0 = 0; g0 < group; g0 += 8) {
+                    if (group > 8) load_heads(g0);
+                    float c[2][4] = {};   // two chains: even and odd steps
+#pragma unroll
+                    for (int k = 0; k < 2 * KS; ++k) {
+                        uint32_t a[4];
+                        ldmatrix_x4(rows + k * 32, a);
+                        mma_bf16(c[k & 1], a, qb[k][0], qb[k][1]);
+                        if (g0 == 0) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const bool ok = present >> ((lane >> 2) + 8 * (i & 1)) & 1u;   // (a row that was not loaded holds anything)
+                                const uint32_t word = ok ? a[i] : 0u;
+                                const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&word);
+                                if (k < KS) least = __hmin2(least, v);
+                                else most = __hmax2(most, v);
+                            }
+                        }
+                    }
+                    // columns 2 quad and 2 quad + 1 of the heads
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float x = g0 + 2 * quad < group ? c[0][2 * r] + c[1][2 * r] : -INFINITY;
+                        const float y = g0 + 2 * quad + 1 < group ? c[0][2 * r + 1] + c[1][2 * r + 1] : -INFINITY;
+                        best[r] = fmaxf(best[r], fmaxf(x, y));
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 1));
+                    best[r] = fmaxf(best[r], __shfl_xor_sync(0xffffffffu, best[r], 2));
+                    const int at = (lane >> 2) + 8 * r;
+                    if (quad == 0 && first + at < last)
+                        p.scores[row * p.score_stride + first + at] = present >> at & 1u ? best[r] : __uint_as_float(0x7fc00000u);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty_bar[s]));
+        }
+        // (low <= high, so the largest |bound| is the largest high or the smallest low)
+        size = warp_max(fmaxf(fmaxf(__low2float(most), __high2float(most)), -fminf(__low2float(least), __high2float(least))));
     }
-    const float size = warp_max(fmaxf(fmaxf(__low2float(most), __high2float(most)), -fminf(__low2float(least), __high2float(least))));
-    // (low <= high, so the largest |bound| is the largest high or the smallest low)
-    if (lane == 0) size_of[warp] = size;
+    if (warp < kWarps && lane == 0) size_of[warp] = size;
     __syncthreads();
     if (abort_word)
         for (int i = 0; i < 200; ++i) __nanosleep(1000);  // let copies in flight land before the CTA exits
-    if (threadIdx.x == 0)
-        p.sizes[row * gridDim.x + blockIdx.x] = fmaxf(fmaxf(size_of[0], size_of[1]), fmaxf(size_of[2], size_of[3]));
+    if (threadIdx.x < heads) {
+        float most = 0.0F;
+        for (int i = threadIdx.x; i < heads * subs; i += heads) most = fmaxf(most, size_of[i]);
+        p.sizes[(static_cast<size_t>(b) * kv.kv_heads + head0 + threadIdx.x) * gridDim.x + blockIdx.x] = most;
+    }
 }
 
 // How the scores are taken: by which kernel, blocks per batch and per CTA, and the error of a score relative to
@@ -465,16 +500,27 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
 enum ScoreKind { kScoreAny, kScoreVec, kScoreMma };
 struct ScoreShape {
     ScoreKind kind;
-    int lanes, batch, cta_blocks;
+    int lanes, batch, cta_blocks, heads;
     float error;
 };
 ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
-    ScoreShape s{kScoreAny, 0, 0, 16, 9.5367431640625e-7F};   // 2^-20: at most 8 + 5 roundings of 2^-24
+    ScoreShape s{kScoreAny, 0, 0, 16, 1, 9.5367431640625e-7F};   // 2^-20: at most 8 + 5 roundings of 2^-24
     if (!aligned16(a.bounds) || !aligned16(a.q)) return s;
     if (a.dtype == SFB_BF16 && a.head_dim % 16 == 0) {
         s.kind = kScoreMma;
-        s.batch = 16;
         s.error = 6.103515625e-5F;   // 2^-14: 2 dim <= 512 products, each addition good to 2^-23 at least
+        const int warps = a.head_dim <= 128 ? 8 : 4;
+        s.heads = a.kv_heads < warps ? a.kv_heads : warps;
+        while (a.kv_heads % s.heads != 0) --s.heads;
+        s.batch = warps / s.heads * 16;
+        // one round of CTAs (two per SM below 128 elements a head) as long as that leaves a stage for each; ranges of at most
+        // 2048 blocks even out ragged contexts
+        const int64_t slots = (a.head_dim <= 64 ? 2LL : 1LL) * sm_count(), groups = static_cast<int64_t>(a.batch) * (a.kv_heads / s.heads);
+        const int64_t each = slots / groups > 0 ? slots / groups : 1;
+        int range = ceil_div(blocks, static_cast<int>(each < blocks ? each : blocks));
+        if (range > 2048) range = 2048;
+        s.cta_blocks = ceil_div(range, s.batch) * s.batch;
+        return s;
     } else if (a.dtype == SFB_F32 && a.head_dim % 8 == 0) {
         s.kind = kScoreVec;
         s.lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
@@ -494,9 +540,9 @@ ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
 }
 
 template <class Kernel>
-sfb_status launch_score(Kernel kernel, size_t smem, dim3 grid, const ScoreParams& p, cudaStream_t stream) {
+sfb_status launch_score(Kernel kernel, int threads, size_t smem, dim3 grid, const ScoreParams& p, cudaStream_t stream) {
     if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    SFB_CUDA(launch_dependent(kernel, grid, dim3(128), smem, stream, p));
+    SFB_CUDA(launch_dependent(kernel, grid, dim3(threads), smem, stream, p));
     return check_launch("sparse_scores");
 }
 
@@ -505,11 +551,12 @@ sfb_status launch_scores(const ScoreParams& p, const ScoreShape& shape, int batc
     const int group = p.q_heads / kv.kv_heads;
     const dim3 grid(ceil_div(p.score_stride, shape.cta_blocks), kv.kv_heads, batch);
     if (shape.kind == kScoreAny)
-        return dtype == SFB_F32 ? launch_score(score_kernel<float>, 0, grid, p, stream) : launch_score(score_kernel<bf16>, 0, grid, p, stream);
+        return dtype == SFB_F32 ? launch_score(score_kernel<float>, 128, 0, grid, p, stream) : launch_score(score_kernel<bf16>, 128, 0, grid, p, stream);
     if (shape.kind == kScoreMma) {
-        const size_t smem = static_cast<size_t>(kScoreWarps) * kScoreStages * 16 * (4 * kv.dim + 16);
+        const size_t smem = static_cast<size_t>(kScoreStages) * shape.batch * (shape.heads * 4 * kv.dim + 16);
+        const dim3 grid(ceil_div(p.score_stride, shape.cta_blocks), kv.kv_heads / shape.heads, batch);
         switch (kv.dim / 16) {
-#define SFB_SCORE_CASE(KS) case KS: return launch_score(score_mma_kernel<KS>, smem, grid, p, stream);
+#define SFB_SCORE_CASE(KS) case KS: return launch_score(score_mma_kernel<KS>, (ScoreMma<KS>::kWarps + 1) * 32, smem, grid, p, stream);
             SFB_SCORE_CASE(1) SFB_SCORE_CASE(2) SFB_SCORE_CASE(3) SFB_SCORE_CASE(4) SFB_SCORE_CASE(5) SFB_SCORE_CASE(6) SFB_SCORE_CASE(7)
             SFB_SCORE_CASE(8) SFB_SCORE_CASE(9) SFB_SCORE_CASE(10) SFB_SCORE_CASE(11) SFB_SCORE_CASE(12) SFB_SCORE_CASE(13)
             SFB_SCORE_CASE(14) SFB_SCORE_CASE(15) SFB_SCORE_CASE(16)
@@ -518,7 +565,7 @@ sfb_status launch_scores(const ScoreParams& p, const ScoreShape& shape, int batc
     }
     const size_t smem = sizeof(float) * 2 * kv.dim * static_cast<size_t>(shape.batch) * kScoreStages * kScoreWarps;
     const auto by_group = [&](auto k1, auto k2, auto k4) -> sfb_status {
-        return group == 1 ? launch_score(k1, smem, grid, p, stream) : group == 2 ? launch_score(k2, smem, grid, p, stream) : launch_score(k4, smem, grid, p, stream);
+        return group == 1 ? launch_score(k1, 128, smem, grid, p, stream) : group == 2 ? launch_score(k2, 128, smem, grid, p, stream) : launch_score(k4, 128, smem, grid, p, stream);
     };
     if (shape.lanes == 8) return by_group(score_vec_kernel<float, 8, 1>, score_vec_kernel<float, 8, 2>, score_vec_kernel<float, 8, 4>);
     if (shape.lanes == 16) return by_group(score_vec_kernel<float, 16, 1>, score_vec_kernel<float, 16, 2>, score_vec_kernel<float, 16, 4>);
@@ -543,7 +590,7 @@ __device__ __forceinline__ float score_of_key(uint64_t key) {
     return __uint_as_float(image >> 31 ? image & 0x7fffffffu : ~image);
 }
 
-// Score of one block in 64 bits, by one warp.
+// Score of one block in 64 bits, by one warp: a lane's elements of low and high are read once for all heads.
 template <class T>
 __device__ double exact_score(const SelectParams& p, int b, int kvh, int block) {
     const PagedView& kv = p.kv;
@@ -552,15 +599,33 @@ __device__ double exact_score(const SelectParams& p, int b, int kvh, int block) 
     double best = __longlong_as_double(0x7ff8000000000000ll);  // NaN: ranks last
     if (page < 0 || page >= kv.num_blocks) return best;
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group) * kv.dim;
-    const T* lo = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * kv.dim;
-    const T* hi = lo + kv.dim;
-    for (int g = 0; g < group; ++g) {
-        double s = 0.0;
-        for (int d = lane; d < kv.dim; d += 32) {
-            const float qv = to_float(q[g * kv.dim + d]);
-            if (qv != 0.0F) s += static_cast<double>(qv) * static_cast<double>(to_float(qv > 0.0F ? hi[d] : lo[d]));
+    const T* low = static_cast<const T*>(p.bounds) + (static_cast<int64_t>(page) * kv.kv_heads + kvh) * 2 * kv.dim;
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        lo[i] = d < kv.dim ? to_float(low[d]) : 0.0F;
+        hi[i] = d < kv.dim ? to_float(low[kv.dim + d]) : 0.0F;
+    }
+    for (int g0 = 0; g0 < group; g0 += 4) {
+        double s[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            s[g] = 0.0;
+            const T* qg = q + min(g0 + g, group - 1) * kv.dim;   // (heads past the group repeat its last)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = lane + 32 * i;
+                const float qv = d < kv.dim ? to_float(qg[d]) : 0.0F;
+                if (qv != 0.0F) s[g] += static_cast<double>(qv) * static_cast<double>(qv > 0.0F ? hi[i] : lo[i]);
+            }
         }
-        best = fmax(best, warp_sum(s));  // (fmax ignores NaN)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) best = fmax(best, s[g]);  // (fmax ignores NaN)
     }
     return best;
 }
@@ -590,56 +655,51 @@ select_kernel(const __grid_constant__ SelectParams p) {
         for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < n ? i : -1;
         return;
     }
-    extern __shared__ float cached[];
+    extern __shared__ uint32_t keys[];
     const float* scores = p.scores + row * p.score_stride;
-    if (p.cached) {
-        for (int i = threadIdx.x; i < n; i += kSelectThreads) cached[i] = scores[i];
-        scores = cached;   // (ordered by the barrier below)
-    }
     double* exact = p.exact + row * p.score_stride;
-    const int recent_from = n - p.recent, sink = p.sink;
+    const int recent_from = n - p.recent, sink = p.sink, group = p.q_heads / kv.kv_heads;
     const auto forced = [&](int i) { return i < sink || i >= recent_from; };
     // the error of the 32-bit scores
-    const int group = p.q_heads / kv.kv_heads;
     float norm = 0.0F, size = 0.0F;
     for (int g = warp; g < group; g += kSelectThreads / 32) {
         const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * p.q_heads + kvh * group + g) * kv.dim;
         float s = 0.0F;
-        for (int d = lane; d < kv.dim; d += 32) s += fabsf(to_float(q[d]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (lane + 32 * i < kv.dim) s += fabsf(to_float(q[lane + 32 * i]));
         s = warp_sum(s);
         norm = s > norm || s != s ? s : norm;
     }
     for (int i = threadIdx.x; i < (n + p.blocks_per_size - 1) / p.blocks_per_size; i += kSelectThreads)
         size = fmaxf(size, p.sizes[row * p.size_count + i]);
     size = warp_max(size);
+    if (p.cached) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < n; i += kSelectThreads) keys[i] = forced(i) ? kForced : static_cast<uint32_t>(order_key(scores[i]));
+    }
     if (lane == 0) { most[0][warp] = norm; most[1][warp] = size; }
     if (threadIdx.x < 2) counts[threadIdx.x] = 0;
     __syncthreads();
-    norm = size = 0.0F;
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
-        norm = most[0][w] > norm || most[0][w] != most[0][w] ? most[0][w] : norm;
-        size = fmaxf(size, most[1][w]);
+    {
+        const float a = lane < kSelectThreads / 32 ? most[0][lane] : 0.0F;
+        norm = __any_sync(0xffffffffu, a != a) ? __uint_as_float(0x7fc00000u) : warp_max(a);
+        size = warp_max(lane < kSelectThreads / 32 ? most[1][lane] : 0.0F);
     }
     const int n_forced = min(sink, n) + min(p.recent, n) - max(0, min(sink, n) - max(recent_from, 0));
     const float err2 = 2.0F * p.error * norm * size;  // 2 err
     if (p.cached && k > n_forced) {
         const bool settled = select_mask<kSelectThreads>(
-            sh, n, k - n_forced, [&](int i) -> uint64_t { return forced(i) ? 0 : order_key(scores[i]); },
-            [&](uint64_t& low, uint64_t& high) {   // whatever the tolerance lets change places with the k-th (NaN, infinity: all)
+            sh, keys, n, k - n_forced,
+            [&](uint32_t& low, uint32_t& high) {   // whatever the tolerance lets change places with the k-th (NaN, infinity: all)
                 const float from = score_of_key(low) - err2, to = score_of_key(high) + err2;
-                low = from > -INFINITY ? order_key(from) : 1;
-                high = to < INFINITY ? order_key(to) : ~0ull;
+                low = from > -INFINITY ? static_cast<uint32_t>(order_key(from)) : 1u;
+                high = to < INFINITY ? static_cast<uint32_t>(order_key(to)) : kForced - 1;
             },
             [&](int j) -> uint64_t { return order_key(exact_score<T>(p, b, kvh, sh.near[j])); });
         if (settled) {
-            walk_bits<kSelectThreads>(sh.walk, (n + 31) / 32,
-                [&](int w, unsigned& take, unsigned& none) {
-                    take = sh.words[w];
-                    none = 0;
-                    for (int i = w * 32; i < min(sink, w * 32 + 32); ++i) take |= 1u << (i & 31);
-                    for (int i = max(max(recent_from, 0), w * 32); i < min(n, w * 32 + 32); ++i) take |= 1u << (i & 31);
-                },
-                [&](int i, int rank) { if (rank < k) out[rank] = i; }, [](int, int) {});
+            walk_bits<kSelectThreads>(sh.scan, (n + 31) / 32, [&](int w, unsigned& take, unsigned& none) { take = sh.words[w]; none = 0; },
+                                      [&](int i, int rank) { if (rank < k) out[rank] = i; }, [](int, int) {});
             for (int i = k + threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = -1;
             return;
         }
@@ -784,7 +844,7 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
     float *scores = reinterpret_cast<float*>(ws + l.scores), *sizes = reinterpret_cast<float*>(ws + l.sizes);
     const ScoreShape shape = score_shape(*a, l.score_stride);
     {
-        const ScoreParams p{kv, a->q, a->bounds, scores, sizes, a->q_heads, l.score_stride, shape.batch, shape.cta_blocks};
+        const ScoreParams p{kv, a->q, a->bounds, scores, sizes, a->q_heads, l.score_stride, shape.batch, shape.cta_blocks, shape.heads};
         SFB_TRY(launch_scores(p, shape, a->batch, a->dtype, s));
     }
     {

@@ -29,15 +29,16 @@ struct AddParams {
 
 constexpr int kAddThreads = 256;
 constexpr int kAddHeads = 16;      // heads whose statistics are kept at once
+constexpr int kWarpPieces = 4;     // pieces of a row that one warp joins
 
-// Grid (group + position chunks, K/V head, sequence).  The first `group` CTAs join the splits of one query head each into its
-// output; the others add the weights of `chunk` positions.  Maxima and sums come from the pieces.
+// Grid (position chunks, K/V head, sequence).  A warp takes a query head: its maximum and sum out of the pieces, and, in
+// the first chunk's CTA, its output.  Then the CTA adds the weights of `chunk` positions, the first of which were
+// fetched before.
 template <class T>
 __global__ void __launch_bounds__(kAddThreads)
 add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
-    __shared__ float factor[kMaxPieces];           // of every piece (output CTAs)
-    __shared__ float half_sum[256];
     __shared__ float2 stats[kAddHeads];            // maximum, 1 / sum
+    __shared__ float sums[kAddThreads / 32][256];
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.q_heads / kv.kv_heads;
@@ -45,71 +46,107 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
     grid_dependency_wait();
     const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
     const int ctx = kv.length(b);
-    if (blockIdx.x < group) {
-        const int g = blockIdx.x;
-        const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g, ctx);
-        if (warp == 0) row_statistics(p.part, r, factor);
-        __syncthreads();
-        T* dst = static_cast<T*>(p.out) + (row0 + g) * kv.dim_v;
-        // two halves of the CTA take alternate pieces
-        const int half = threadIdx.x >> 7;
-        for (int d0 = 0; d0 < kv.dim_v; d0 += 128) {
-            const int d = d0 + (threadIdx.x & 127);
-            float a = 0.0F;
-            if (d < kv.dim_v)
-#pragma unroll 8
-                for (int i = half; i < r.count; i += 2) {
-                    const float f = factor[i];
-                    if (f != 0.0F) a = fmaf(p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + d], f, a);
-                }
-            half_sum[threadIdx.x] = a;
-            __syncthreads();
-            if (half == 0 && d < kv.dim_v) dst[d] = from_float<T>(a + half_sum[threadIdx.x + 128]);
-            __syncthreads();
-        }
-        return;
-    }
-    const int first = (blockIdx.x - group) * chunk, end = min(ctx, first + chunk);
-    if (first >= ctx) return;
+    const int first = blockIdx.x * chunk, end = min(ctx, first + chunk);
+    if (first >= ctx && blockIdx.x > 0) return;
+    const int ctas = max(1, (ctx + chunk - 1) / chunk);       // that got this far
     const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
     for (int g0 = 0; g0 < group; g0 += kAddHeads) {
         const int heads = min(kAddHeads, group - g0);
-        __syncthreads();
-        for (int g = warp; g < heads; g += kAddThreads / 32) {
-            const float2 s = row_statistics(p.part, row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx), nullptr);
-            if (lane == 0) stats[g] = s;
-        }
-        __syncthreads();
         // (later rounds of a group of more than kAddHeads heads add to what the first left)
         const float* before = g0 == 0 ? p.weights : p.weights_out;
         const float* logits = p.logits + (row0 + g0) * p.logit_stride;
+        const bool four = chunk > kAddThreads && p.wide;      // four consecutive positions a thread
+        float4 ahead[4], old = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+        const int t0 = first + 4 * threadIdx.x;
+        if (four && t0 + 4 <= end) {
+            if (before) old = *reinterpret_cast<const float4*>(before + wrow + t0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g < heads) ahead[g] = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t0);
+        }
+        __syncthreads();
+        for (int g = warp; g < heads; g += kAddThreads / 32) {
+            const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx);
+            const float2 s = row_statistics(p.part, r, nullptr);
+            if (lane == 0) stats[g] = s;
+            if (blockIdx.x != 0 || r.count > kWarpPieces) continue;
+            T* dst = static_cast<T*>(p.out) + (row0 + g0 + g) * kv.dim_v;
+            float a[8] = {};
+#pragma unroll 4
+            for (int i = 0; i < r.count; ++i) {
+                const size_t index = r.first + static_cast<size_t>(i) * r.step;
+                const float m = p.part.ml[index * p.part.ml_step];
+                const float f = m == -INFINITY ? 0.0F : exp2_fast(m - s.x);
+                const float* o = p.part.o + index * p.part.o_step;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (lane + 32 * j < kv.dim_v) a[j] = fmaf(o[lane + 32 * j], f, a[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (lane + 32 * j < kv.dim_v) dst[lane + 32 * j] = from_float<T>(a[j] * s.y);
+        }
+        __syncthreads();
+        // a row of many pieces is joined by a whole CTA, the rows of the group by one CTA each as far as there are
+        for (int g = 0; g < heads; ++g) {
+            const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx);
+            if (r.count <= kWarpPieces || (g0 + g) % ctas != static_cast<int>(blockIdx.x)) continue;
+            float a[8] = {};
+            for (int i = warp; i < r.count; i += kAddThreads / 32) {
+                const size_t index = r.first + static_cast<size_t>(i) * r.step;
+                const float m = p.part.ml[index * p.part.ml_step];
+                const float f = m == -INFINITY ? 0.0F : exp2_fast(m - stats[g].x);
+                const float* o = p.part.o + index * p.part.o_step;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (lane + 32 * j < kv.dim_v) a[j] = fmaf(o[lane + 32 * j], f, a[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sums[warp][lane + 32 * j] = a[j];
+            __syncthreads();
+            if (threadIdx.x < kv.dim_v) {
+                float total = 0.0F;
+#pragma unroll
+                for (int w = 0; w < kAddThreads / 32; ++w) total += sums[w][threadIdx.x];
+                static_cast<T*>(p.out)[(row0 + g0 + g) * kv.dim_v + threadIdx.x] = from_float<T>(total * stats[g].y);
+            }
+            __syncthreads();
+        }
         const auto add_one = [&](int t) {
             float w = 0.0F;
             for (int g = 0; g < heads; ++g) w = fmaf(exp2_fast(logits[g * p.logit_stride + t] - stats[g].x), stats[g].y, w);
             p.weights_out[wrow + t] = (before ? before[wrow + t] : 0.0F) + w;
         };
-        if (chunk == kAddThreads) {
-            if (first + threadIdx.x < end) add_one(first + threadIdx.x);
-        } else {   // four consecutive positions a thread
-            for (int t = first + 4 * threadIdx.x; t < end; t += 4 * kAddThreads) {
-                if (t + 4 > end || !p.wide) {
-                    for (int i = 0; i < 4; ++i)
-                        if (t + i < end) add_one(t + i);
-                    continue;
-                }
-                float4 w = make_float4(0.0F, 0.0F, 0.0F, 0.0F), sum = w;
-                if (before) w = *reinterpret_cast<const float4*>(before + wrow + t);
-#pragma unroll 4
-                for (int g = 0; g < heads; ++g) {
-                    const float4 x = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t);
-                    const float2 st = stats[g];
-                    sum.x = fmaf(exp2_fast(x.x - st.x), st.y, sum.x);
-                    sum.y = fmaf(exp2_fast(x.y - st.x), st.y, sum.y);
-                    sum.z = fmaf(exp2_fast(x.z - st.x), st.y, sum.z);
-                    sum.w = fmaf(exp2_fast(x.w - st.x), st.y, sum.w);
-                }
-                *reinterpret_cast<float4*>(p.weights_out + wrow + t) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
+        const auto add_four = [&](float4& sum, const float4& x, int g) {
+            const float2 st = stats[g];
+            sum.x = fmaf(exp2_fast(x.x - st.x), st.y, sum.x);
+            sum.y = fmaf(exp2_fast(x.y - st.x), st.y, sum.y);
+            sum.z = fmaf(exp2_fast(x.z - st.x), st.y, sum.z);
+            sum.w = fmaf(exp2_fast(x.w - st.x), st.y, sum.w);
+        };
+        if (!four) {
+            for (int t = first + threadIdx.x; t < end; t += kAddThreads) add_one(t);
+            continue;
+        }
+        for (int t = t0; t < end; t += 4 * kAddThreads) {
+            if (t + 4 > end) {
+                for (int i = t; i < end; ++i) add_one(i);
+                continue;
             }
+            float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F), w = old;
+            if (t != t0) {
+                w = sum;
+                if (before) w = *reinterpret_cast<const float4*>(before + wrow + t);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    if (g < heads) ahead[g] = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g < heads) add_four(sum, ahead[g], g);
+#pragma unroll 4
+            for (int g = 4; g < heads; ++g) add_four(sum, *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t), g);
+            *reinterpret_cast<float4*>(p.weights_out + wrow + t) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
         }
     }
     if (p.positions && first <= ctx - 1 && ctx - 1 < end && threadIdx.x == 0) p.positions[wrow + ctx - 1] = p.query_position[b];
@@ -152,7 +189,7 @@ struct EvictParams {
     int* positions_out;
     int* new_len;
     uint8_t* kept;         // [batch * kv_heads][max_context]
-    int* moves;            // per (sequence, K/V head): count, then max_moves destinations, then max_moves sources
+    int* moves;            // per (sequence, K/V head): old length, count, then max_moves destinations, then max_moves sources
     int max_moves, stride, budget, sink, recent, masked;   // masked: rows of at most kMaskItems slots
 };
 
@@ -204,9 +241,10 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     const int* positions = p.positions + row * p.stride;
     float* weights_out = p.weights_out + row * p.stride;
     int* positions_out = p.positions_out + row * p.stride;
-    int* to = p.moves + row * (1 + 2 * static_cast<size_t>(p.max_moves)) + 1;
+    int* to = p.moves + row * (2 + 2 * static_cast<size_t>(p.max_moves)) + 2;
     int* since = to + p.max_moves;
     uint8_t* kept_bits = p.kept + row * kv.limit;
+    if (threadIdx.x == 0) to[-2] = n;
     if (k == n) {
         if (threadIdx.x == 0) to[-1] = 0;
         for (int i = threadIdx.x; i < n; i += kEvictThreads) {
@@ -215,8 +253,14 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
         }
         return;
     }
+    extern __shared__ uint32_t keys[];   // masked: positions, then the weights' keys (kForced for safe rows)
     int newest = -1;
-    for (int i = threadIdx.x; i < n; i += kEvictThreads) newest = max(newest, positions[i]);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += kEvictThreads) {
+        const int at = positions[i];
+        newest = max(newest, at);
+        if (p.masked) keys[i] = static_cast<uint32_t>(at);
+    }
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) newest_of[warp] = newest;
     __syncthreads();
@@ -224,13 +268,19 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     const int64_t recent_from = static_cast<int64_t>(newest) - p.recent;
     const int sink = p.sink;
     // rows kept by their position are counted first; the rest of the budget goes to the largest weights of the others
-    const auto safe = [&](int i) { return positions[i] < sink || positions[i] > recent_from; };
-    extern __shared__ uint32_t keys[];   // masked: the weights' keys, 0 for safe rows
+    const auto is_safe = [&](int at) { return at < sink || at > recent_from; };
+    const auto safe = [&](int i) { return is_safe(positions[i]); };
     int n_safe = 0;
-    for (int i = threadIdx.x; i < n; i += kEvictThreads) {
-        const bool is_safe = safe(i);
-        n_safe += is_safe;
-        if (p.masked) keys[i] = is_safe ? 0u : static_cast<uint32_t>(order_key(weights[i]));
+    if (p.masked) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < n; i += kEvictThreads) {   // (its own entries)
+            const uint32_t key = static_cast<uint32_t>(order_key(weights[i]));
+            const bool s = is_safe(static_cast<int>(keys[i]));
+            keys[i] = s ? kForced : key;
+            n_safe += s;
+        }
+    } else {
+        for (int i = threadIdx.x; i < n; i += kEvictThreads) n_safe += safe(i);
     }
     n_safe = __reduce_add_sync(0xffffffffu, n_safe);
     __syncthreads();
@@ -242,21 +292,18 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     bool settled = false;
     if (p.masked && n_safe <= k) {
         if (room > 0) {
-            settled = select_mask<kEvictThreads>(sh, n, room, [&](int i) -> uint64_t { return keys[i]; }, [](uint64_t&, uint64_t&) {},
-                                                 [&](int j) -> uint64_t { return keys[sh.near[j]]; });
+            settled = select_mask<kEvictThreads>(sh, keys, n, room, [](uint32_t&, uint32_t&) {}, [&](int j) -> uint64_t { return keys[sh.near[j]]; });
         } else {
-            for (int w = threadIdx.x; w < (n + 31) / 32; w += kEvictThreads) sh.words[w] = 0;
+            for (int i0 = warp * 32; i0 < n; i0 += kEvictThreads) {
+                const unsigned word = __ballot_sync(0xffffffffu, i0 + lane < n && keys[i0 + lane] == kForced);
+                if (lane == 0) sh.words[i0 >> 5] = word;
+            }
             settled = true;
             __syncthreads();
         }
     }
     if (settled) {
-        for (int i0 = warp * 32; i0 < n; i0 += kEvictThreads) {
-            const unsigned word = __ballot_sync(0xffffffffu, i0 + lane < n && keys[i0 + lane] == 0u);
-            if (lane == 0) sh.words[i0 >> 5] |= word;
-        }
-        __syncthreads();
-        const uint64_t totals = walk_bits<kEvictThreads>(sh.walk, (n + 31) / 32,
+        const unsigned totals = walk_bits<kEvictThreads>(sh.scan, (n + 31) / 32,
             [&](int w, unsigned& hole, unsigned& tail) {
                 const int at = w * 32;
                 const unsigned front = at + 32 <= k ? ~0u : (at >= k ? 0u : (1u << (k - at)) - 1);
@@ -264,7 +311,8 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
                 tail = sh.words[w] & ~front;
             },
             [&](int i, int rank) { if (rank < p.max_moves) to[rank] = i; }, [&](int i, int rank) { if (rank < p.max_moves) since[rank] = i; });
-        holes = min(min(static_cast<int>(totals & 0xffffffffu), static_cast<int>(totals >> 32)), p.max_moves);   // (both counts are equal)
+        holes = min(min(static_cast<int>(totals & 0xffffu), static_cast<int>(totals >> 16)), p.max_moves);   // (both counts are equal)
+#pragma unroll 4
         for (int i = threadIdx.x; i < k; i += kEvictThreads)
             if (sh.words[i >> 5] >> (i & 31) & 1u) {
                 weights_out[i] = weights[i];
@@ -280,15 +328,11 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
         weights_out[to[j]] = weights[since[j]];
         positions_out[to[j]] = positions[since[j]];
     }
-    __syncthreads();
-    for (int i = k + threadIdx.x; i < n; i += kEvictThreads) {
-        weights_out[i] = 0.0F;
-        positions_out[i] = -1;
-    }
-    if (threadIdx.x == 0) to[-1] = holes;
+    if (threadIdx.x == 0) to[-1] = holes;   // (slots behind the new length are cleared with the moves)
 }
 
-// One warp per moved row; new_len is written here, after every reader of context_len (it may be the same array).
+// One warp per moved row; the entries behind the new length are cleared here, and new_len is written here, where
+// nothing reads context_len (it may be the same array).
 template <class V>
 __global__ void __launch_bounds__(256)
 evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_units) {
@@ -296,7 +340,7 @@ evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_unit
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependents_may_launch();
     grid_dependency_wait();
-    const int* to = p.moves + (static_cast<size_t>(b) * kv.kv_heads + kvh) * (1 + 2 * static_cast<size_t>(p.max_moves)) + 1;
+    const int* to = p.moves + (static_cast<size_t>(b) * kv.kv_heads + kvh) * (2 + 2 * static_cast<size_t>(p.max_moves)) + 2;
     const int* since = to + p.max_moves;
     const int count = to[-1];
     V* keys = static_cast<V*>(const_cast<void*>(kv.k_pool));
@@ -307,7 +351,13 @@ evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_unit
         for (int i = lane; i < k_units; i += 32) keys[dst * k_units + i] = keys[src * k_units + i];
         for (int i = lane; i < v_units; i += 32) values[dst * v_units + i] = values[src * v_units + i];
     }
-    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) p.new_len[b] = min(max(kv.lens[b], 0), min(p.budget, kv.limit));
+    const int n = to[-2], k = min(n, p.budget);
+    const size_t row = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
+    for (int i = k + blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+        p.weights_out[row + i] = 0.0F;
+        p.positions_out[row + i] = -1;
+    }
+    if (blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0) p.new_len[b] = k;
 }
 
 int evict_max_moves(const sfb_evict_args& a) {
@@ -318,7 +368,7 @@ int evict_max_moves(const sfb_evict_args& a) {
 }
 
 size_t evict_moves_bytes(const sfb_evict_args& a) {
-    return round_up16(sizeof(int) * static_cast<size_t>(a.batch) * a.kv_heads * (1 + 2 * static_cast<size_t>(evict_max_moves(a))));
+    return round_up16(sizeof(int) * static_cast<size_t>(a.batch) * a.kv_heads * (2 + 2 * static_cast<size_t>(evict_max_moves(a))));
 }
 
 sfb_status check_evict(const sfb_evict_args* a) {
@@ -413,11 +463,11 @@ sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream 
                         l.logit_stride, a->q_heads, a->weight_stride,
                         a->weight_stride % 4 == 0 && aligned16(a->weights) && aligned16(a->weights_out)};
     const int group = a->q_heads / a->kv_heads;
-    // few CTAs: one position a thread; many: long chunks, so that the statistics are read less often
+    // few CTAs: one position a thread; many: four, and at last sixteen, so that the statistics are read less often
     const int64_t pairs = static_cast<int64_t>(a->kv_heads) * a->batch;
     int chunk = kAddThreads;
-    while (chunk < 16 * kAddThreads && pairs * ceil_div(p.kv.limit, chunk) > 4LL * sm_count()) chunk *= 4;
-    const dim3 grid(group + ceil_div(p.kv.limit, chunk), a->kv_heads, a->batch);
+    while (chunk < 16 * kAddThreads && pairs * ceil_div(p.kv.limit, chunk) > 8LL * sm_count()) chunk *= 4;
+    const dim3 grid(ceil_div(p.kv.limit, chunk), a->kv_heads, a->batch);
     if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(add_weights_kernel<float>, grid, dim3(kAddThreads), 0, s, add, chunk));
     else SFB_CUDA(launch_dependent(add_weights_kernel<bf16>, grid, dim3(kAddThreads), 0, s, add, chunk));
     return check_launch("decode_weights_add");
@@ -446,7 +496,7 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
     SFB_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(uint32_t) * kMaskItems)));
     SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
     SFB_TRY(check_launch("evict_select"));
-    const dim3 grid(p.max_moves > 0 ? (p.max_moves > 64 * 8 ? 64 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
+    const dim3 grid(p.max_moves > 0 ? (p.max_moves > 256 * 8 ? 256 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
     const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool);
     const int per = wide ? 16 / static_cast<int>(dtype_size(a->dtype)) : 1;
     const int ku = a->head_dim / per, vu = a->head_dim_value / per;

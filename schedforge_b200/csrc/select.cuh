@@ -1,10 +1,10 @@
 // Selection of the k largest of n keys by one CTA, ties to the lower index.
 //
-// Keys are unsigned 64-bit words whose order is the order wanted; a key of 0 does not take part.  Rows of up to
-// kMaskItems keys: the keys are counted in 2048 equal bins of their range, what lies above the bin of the k-th is kept,
-// and the few keys inside it are ranked against one another (select_mask; bits in shared memory).  Where too
-// many keys share that bin, and for longer rows, the range is narrowed bin by bin until it holds one value
-// (select_threshold: at most six passes for 64 bits).
+// Rows of up to kMaskItems keys of 32 bits (select_mask): the keys are counted in 2048 equal bins of their range, what
+// lies above the bin of the k-th is kept, and the few keys inside it are ranked against one another; the result is one
+// bit per key in shared memory.  Where too many keys share that bin, and for longer rows, keys of 64 bits are narrowed
+// bin by bin until the range holds one value (select_threshold: at most six passes).
+// The order of the unsigned keys is the order wanted; a key of 0 does not take part.
 #pragma once
 
 #include "common.cuh"
@@ -51,10 +51,8 @@ struct Threshold {
 };
 
 // All threads of the CTA call it; 1 <= k <= number of keys that are not 0.  key(i) is evaluated several times.
-// enough: a bin of at most that many keys ends the search as well; the k-th key is then among the keys of
-// [sh.low, sh.high] and the result says how many of those are wanted.
 template <int THREADS, class Key>
-__device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key, unsigned enough = 0) {
+__device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key) {
     constexpr int kWarps = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t lo = ~0ull, hi = 0;
@@ -116,8 +114,8 @@ __device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key, u
             sh.rest = rest - static_cast<int>(above);
             sh.low = first;
             sh.high = high - first < span ? high : first + span;
-            sh.done = shift == 0 || sh.hist[bin] == static_cast<unsigned>(sh.rest) || sh.hist[bin] <= enough;
-            if (enough == 0 && sh.hist[bin] == static_cast<unsigned>(sh.rest)) sh.rest = 0;  // the whole bin is wanted
+            sh.done = shift == 0 || sh.hist[bin] == static_cast<unsigned>(sh.rest);
+            if (sh.hist[bin] == static_cast<unsigned>(sh.rest)) sh.rest = 0;  // the whole bin is wanted
         }
         __syncthreads();
         if (sh.done) break;
@@ -127,26 +125,85 @@ __device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key, u
     return found;
 }
 
-// Bits of the k largest keys in sh.words (n <= kMaskItems; keys of 0 get none).  widen(low, high) may extend the range of
-// keys that are ranked, and rank(j) gives the final key of near item j (index sh.near[j]; called by whole warps, all of
-// whose lanes return it): how keys known to a tolerance only are ranked exactly where it matters.  Returns false, with
-// nothing settled, where more than kNearItems keys are in that range.  All threads call it; sh is ready for use afterwards.
-template <int THREADS, class Key, class Widen, class Rank>
-__device__ bool select_mask(SelectShared& sh, int n, int k, Key key, Widen widen, Rank rank) {
+constexpr uint32_t kForced = 0xffffffffu;   // a 32-bit key that is kept whatever the others are (no number's image)
+
+// Bits of the kept keys in sh.words: the forced ones and the k largest of the others (n <= kMaskItems; 1 <= k <= number of
+// other keys that are not 0).  keys: shared memory, complete after the callers' last barrier.  widen(low, high) may
+// extend the range of keys that are ranked, and rank(j) gives the final key of near item j (index sh.near[j]; called by
+// whole warps, all lanes of which return it): how keys known to a tolerance are ranked exactly where it matters.
+// Returns false, with nothing settled, where more than kNearItems keys are in that range.  All threads call it.
+template <int THREADS, class Widen, class Rank>
+__device__ bool select_mask(SelectShared& sh, const uint32_t* keys, int n, int k, Widen widen, Rank rank) {
+    constexpr int kWarps = THREADS / 32, kPer = kSelectBins / THREADS;
+    static_assert(kPer >= 1 && kWarps <= 32, "one or more bins a thread");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    select_threshold<THREADS>(sh, n, k, key, kNearItems / 8);
-    uint64_t low = sh.low, high = sh.high;
-    widen(low, high);
+    uint32_t low = ~0u, high = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const uint32_t v = keys[i];
+        if (v != 0 && v != kForced) {
+            low = min(low, v);
+            high = max(high, v);
+        }
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) { sh.lo[warp] = low; sh.hi[warp] = high; }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sh.hist[threadIdx.x * kPer + j] = 0;
     if (threadIdx.x == 0) sh.near_count = sh.kept_count = 0;
     __syncthreads();
+    low = __reduce_min_sync(0xffffffffu, lane < kWarps ? static_cast<uint32_t>(sh.lo[lane]) : ~0u);
+    high = __reduce_max_sync(0xffffffffu, lane < kWarps ? static_cast<uint32_t>(sh.hi[lane]) : 0u);
+    int rest = k;
+    for (int pass = 0; pass < 4; ++pass) {
+        const int bits = 32 - __clz(high - low), shift = bits > 11 ? bits - 11 : 0;
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const uint32_t v = keys[i];
+            if (v >= low && v <= high && v != kForced) atomicAdd(&sh.hist[(v - low) >> shift], 1u);
+        }
+        __syncthreads();
+        // counts from the top: thread t owns kPer bins counted downwards from the last
+        unsigned count[kPer], own = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) own += count[j] = sh.hist[kSelectBins - 1 - (threadIdx.x * kPer + j)];
+        unsigned sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) sh.scan[warp] = sum;
+        __syncthreads();
+        unsigned above = __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u) + sum - own;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (above < static_cast<unsigned>(rest) && above + count[j] >= static_cast<unsigned>(rest)) {   // one thread, one bin
+                const uint32_t first = low + (static_cast<uint32_t>(kSelectBins - 1 - (threadIdx.x * kPer + j)) << shift);
+                const uint32_t span = (1u << shift) - 1;
+                sh.low = first;
+                sh.high = high - first < span ? high : first + span;
+                sh.rest = rest - static_cast<int>(above);
+                sh.done = shift == 0 || count[j] <= kNearItems / 8;
+            }
+            above += count[j];
+            sh.hist[kSelectBins - 1 - (threadIdx.x * kPer + j)] = 0;
+        }
+        __syncthreads();
+        low = static_cast<uint32_t>(sh.low);
+        high = static_cast<uint32_t>(sh.high);
+        rest = sh.rest;
+        if (sh.done) break;
+        __syncthreads();
+    }
+    widen(low, high);
     int kept = 0;
     for (int i0 = warp * 32; i0 < n; i0 += THREADS) {
         const int i = i0 + lane;
-        const uint64_t v = i < n ? key(i) : 0;
+        const uint32_t v = i < n ? keys[i] : 0;
         const unsigned word = __ballot_sync(0xffffffffu, v > high);
-        kept += __popc(word);
+        kept += __popc(word & __ballot_sync(0xffffffffu, v != kForced));
         if (lane == 0) sh.words[i0 >> 5] = word;
-        if (v != 0 && v >= low && v <= high) {
+        if (v != 0 && v >= low && v <= high && v != kForced) {
             const int at = atomicAdd(&sh.near_count, 1);
             if (at < kNearItems) sh.near[at] = i;
         }
@@ -158,7 +215,7 @@ __device__ bool select_mask(SelectShared& sh, int n, int k, Key key, Widen widen
     if (room >= near) {
         for (int j = threadIdx.x; j < near; j += THREADS) atomicOr(&sh.words[sh.near[j] >> 5], 1u << (sh.near[j] & 31));
     } else {
-        for (int j = warp; j < near; j += THREADS / 32) {
+        for (int j = warp; j < near; j += kWarps) {
             const uint64_t v = rank(j);
             if (lane == 0) sh.near_key[j] = v;
         }
@@ -179,49 +236,34 @@ __device__ bool select_mask(SelectShared& sh, int n, int k, Key key, Widen widen
 }
 
 // Walks the set bits of two masks of `words` words in ascending order: visit_a(index, rank), visit_b(index, rank).
-// Returns the totals (a in the low, b in the high half).
+// Returns the totals (a in the low, b in the high half; each below 2^16).
 template <int THREADS, class Words, class VisitA, class VisitB>
-__device__ __forceinline__ uint64_t walk_bits(unsigned long long* scan, int words, Words get, VisitA visit_a, VisitB visit_b) {
+__device__ __forceinline__ unsigned walk_bits(unsigned* scan, int words, Words get, VisitA visit_a, VisitB visit_b) {
     constexpr int kWarps = THREADS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stretch = ((words + kWarps - 1) / kWarps + 31) & ~31;
-    const int begin = min(words, warp * stretch), end = min(words, begin + stretch);
-    uint64_t sum = 0;
-    for (int w = begin + lane; w < end; w += 32) {
-        unsigned a, b;
-        get(w, a, b);
-        sum += static_cast<uint64_t>(__popc(b)) << 32 | static_cast<unsigned>(__popc(a));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) scan[warp] = sum;
-    __syncthreads();
-    uint64_t before = 0, total = 0;
-#pragma unroll 8
-    for (int w = 0; w < kWarps; ++w) {
-        const uint64_t v = scan[w];
-        if (w < warp) before += v;
-        total += v;
-    }
-    __syncthreads();
-    for (int w0 = begin; w0 < end; w0 += 32) {
-        const int w = w0 + lane;
+    unsigned before = 0;
+    for (int w0 = 0; w0 < words; w0 += THREADS) {
+        const int w = w0 + threadIdx.x;
         unsigned a = 0, b = 0;
-        if (w < end) get(w, a, b);
-        const uint64_t own = static_cast<uint64_t>(__popc(b)) << 32 | static_cast<unsigned>(__popc(a));
-        uint64_t incl = own;
+        if (w < words) get(w, a, b);
+        const unsigned own = static_cast<unsigned>(__popc(a)) | static_cast<unsigned>(__popc(b)) << 16;
+        unsigned incl = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        const uint64_t at = before + incl - own;
-        int ra = static_cast<int>(at & 0xffffffffu), rb = static_cast<int>(at >> 32);
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        const unsigned mine = lane < kWarps ? scan[lane] : 0u;
+        const unsigned at = before + __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u) + incl - own;
+        before += __reduce_add_sync(0xffffffffu, mine);
+        int ra = static_cast<int>(at & 0xffffu), rb = static_cast<int>(at >> 16);
         for (; a; a &= a - 1) visit_a(w * 32 + __ffs(a) - 1, ra++);
         for (; b; b &= b - 1) visit_b(w * 32 + __ffs(b) - 1, rb++);
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        __syncthreads();
     }
-    return total;
+    return before;
 }
 
 // Walks [0, n) in index order with the flags a(i) and b(i), each warp a contiguous stretch: visit(i, a, b, ra, rb) is
