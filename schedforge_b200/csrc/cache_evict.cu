@@ -29,16 +29,16 @@ struct AddParams {
 
 constexpr int kAddThreads = 256;
 constexpr int kAddHeads = 16;      // heads whose statistics are kept at once
-constexpr int kWarpPieces = 4;     // pieces of a row that one warp joins
 
-// Grid (position chunks, K/V head, sequence).  A warp takes a query head: its maximum and sum out of the pieces, and, in
-// the first chunk's CTA, its output.  Then the CTA adds the weights of `chunk` positions, the first of which were
-// fetched before.
+// Grid (group + position chunks, K/V head, sequence).  The first `group` CTAs join the pieces of one query head each into
+// its output; each of the others adds the weights of `chunk` positions (one or four a thread), whose logits are fetched
+// before the heads' maxima and sums have been worked out of the pieces.
 template <class T>
 __global__ void __launch_bounds__(kAddThreads)
 add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
+    __shared__ float factor[kMaxPieces];           // of every piece (output CTAs)
+    __shared__ float half_sum[128];
     __shared__ float2 stats[kAddHeads];            // maximum, 1 / sum
-    __shared__ float sums[kAddThreads / 32][256];
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.q_heads / kv.kv_heads;
@@ -46,107 +46,74 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
     grid_dependency_wait();
     const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
     const int ctx = kv.length(b);
-    const int first = blockIdx.x * chunk, end = min(ctx, first + chunk);
-    if (first >= ctx && blockIdx.x > 0) return;
-    const int ctas = max(1, (ctx + chunk - 1) / chunk);       // that got this far
+    if (blockIdx.x < group) {
+        const int g = blockIdx.x;
+        const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g, ctx);
+        if (warp == 0) row_statistics(p.part, r, factor);
+        __syncthreads();
+        T* dst = static_cast<T*>(p.out) + (row0 + g) * kv.dim_v;
+        const int half = threadIdx.x >> 7;         // the halves of the CTA take alternate pieces
+        for (int d0 = 0; d0 < kv.dim_v; d0 += 128) {
+            const int d = d0 + (threadIdx.x & 127);
+            float a = 0.0F;
+            if (d < kv.dim_v)
+#pragma unroll 8
+                for (int i = half; i < r.count; i += 2) {
+                    const float f = factor[i];
+                    if (f != 0.0F) a = fmaf(p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + d], f, a);
+                }
+            if (half) half_sum[threadIdx.x & 127] = a;
+            __syncthreads();
+            if (!half && d < kv.dim_v) dst[d] = from_float<T>(a + half_sum[threadIdx.x]);
+            __syncthreads();
+        }
+        return;
+    }
+    const int first = (blockIdx.x - group) * chunk, end = min(ctx, first + chunk);
+    if (first >= ctx) return;
     const size_t wrow = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
+    const bool four = chunk > kAddThreads;                    // positions a thread takes, next to each other
+    const int t = first + (four ? 4 : 1) * static_cast<int>(threadIdx.x);
+    const bool wide = four && p.wide && t + 4 <= end;
     for (int g0 = 0; g0 < group; g0 += kAddHeads) {
         const int heads = min(kAddHeads, group - g0);
         // (later rounds of a group of more than kAddHeads heads add to what the first left)
         const float* before = g0 == 0 ? p.weights : p.weights_out;
-        const float* logits = p.logits + (row0 + g0) * p.logit_stride;
-        const bool four = chunk > kAddThreads && p.wide;      // four consecutive positions a thread
-        float4 ahead[4], old = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-        const int t0 = first + 4 * threadIdx.x;
-        if (four && t0 + 4 <= end) {
-            if (before) old = *reinterpret_cast<const float4*>(before + wrow + t0);
+        const float* logits = p.logits + (row0 + g0) * p.logit_stride + t;
+        float4 ahead[4], sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F), old = sum;
+        if (wide) {
+            if (before) old = *reinterpret_cast<const float4*>(before + wrow + t);
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                if (g < heads) ahead[g] = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t0);
+                if (g < heads) ahead[g] = *reinterpret_cast<const float4*>(logits + g * p.logit_stride);
         }
         __syncthreads();
         for (int g = warp; g < heads; g += kAddThreads / 32) {
-            const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx);
-            const float2 s = row_statistics(p.part, r, nullptr);
+            const float2 s = row_statistics(p.part, row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx), nullptr);
             if (lane == 0) stats[g] = s;
-            if (blockIdx.x != 0 || r.count > kWarpPieces) continue;
-            T* dst = static_cast<T*>(p.out) + (row0 + g0 + g) * kv.dim_v;
-            float a[8] = {};
-#pragma unroll 4
-            for (int i = 0; i < r.count; ++i) {
-                const size_t index = r.first + static_cast<size_t>(i) * r.step;
-                const float m = p.part.ml[index * p.part.ml_step];
-                const float f = m == -INFINITY ? 0.0F : exp2_fast(m - s.x);
-                const float* o = p.part.o + index * p.part.o_step;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (lane + 32 * j < kv.dim_v) a[j] = fmaf(o[lane + 32 * j], f, a[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (lane + 32 * j < kv.dim_v) dst[lane + 32 * j] = from_float<T>(a[j] * s.y);
         }
         __syncthreads();
-        // a row of many pieces is joined by a whole CTA, the rows of the group by one CTA each as far as there are
-        for (int g = 0; g < heads; ++g) {
-            const RowPieces r = row_pieces(p.part, kv.kv_heads, p.q_heads, b, kvh * group + g0 + g, ctx);
-            if (r.count <= kWarpPieces || (g0 + g) % ctas != static_cast<int>(blockIdx.x)) continue;
-            float a[8] = {};
-            for (int i = warp; i < r.count; i += kAddThreads / 32) {
-                const size_t index = r.first + static_cast<size_t>(i) * r.step;
-                const float m = p.part.ml[index * p.part.ml_step];
-                const float f = m == -INFINITY ? 0.0F : exp2_fast(m - stats[g].x);
-                const float* o = p.part.o + index * p.part.o_step;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (lane + 32 * j < kv.dim_v) a[j] = fmaf(o[lane + 32 * j], f, a[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sums[warp][lane + 32 * j] = a[j];
-            __syncthreads();
-            if (threadIdx.x < kv.dim_v) {
-                float total = 0.0F;
-#pragma unroll
-                for (int w = 0; w < kAddThreads / 32; ++w) total += sums[w][threadIdx.x];
-                static_cast<T*>(p.out)[(row0 + g0 + g) * kv.dim_v + threadIdx.x] = from_float<T>(total * stats[g].y);
-            }
-            __syncthreads();
-        }
-        const auto add_one = [&](int t) {
-            float w = 0.0F;
-            for (int g = 0; g < heads; ++g) w = fmaf(exp2_fast(logits[g * p.logit_stride + t] - stats[g].x), stats[g].y, w);
-            p.weights_out[wrow + t] = (before ? before[wrow + t] : 0.0F) + w;
-        };
-        const auto add_four = [&](float4& sum, const float4& x, int g) {
-            const float2 st = stats[g];
-            sum.x = fmaf(exp2_fast(x.x - st.x), st.y, sum.x);
-            sum.y = fmaf(exp2_fast(x.y - st.x), st.y, sum.y);
-            sum.z = fmaf(exp2_fast(x.z - st.x), st.y, sum.z);
-            sum.w = fmaf(exp2_fast(x.w - st.x), st.y, sum.w);
-        };
-        if (!four) {
-            for (int t = first + threadIdx.x; t < end; t += kAddThreads) add_one(t);
-            continue;
-        }
-        for (int t = t0; t < end; t += 4 * kAddThreads) {
-            if (t + 4 > end) {
-                for (int i = t; i < end; ++i) add_one(i);
-                continue;
-            }
-            float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F), w = old;
-            if (t != t0) {
-                w = sum;
-                if (before) w = *reinterpret_cast<const float4*>(before + wrow + t);
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    if (g < heads) ahead[g] = *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t);
-            }
+        if (wide) {
+            const auto add = [&](const float4& x, int g) {
+                const float2 st = stats[g];
+                sum.x = fmaf(exp2_fast(x.x - st.x), st.y, sum.x);
+                sum.y = fmaf(exp2_fast(x.y - st.x), st.y, sum.y);
+                sum.z = fmaf(exp2_fast(x.z - st.x), st.y, sum.z);
+                sum.w = fmaf(exp2_fast(x.w - st.x), st.y, sum.w);
+            };
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                if (g < heads) add_four(sum, ahead[g], g);
+                if (g < heads) add(ahead[g], g);
 #pragma unroll 4
-            for (int g = 4; g < heads; ++g) add_four(sum, *reinterpret_cast<const float4*>(logits + g * p.logit_stride + t), g);
-            *reinterpret_cast<float4*>(p.weights_out + wrow + t) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
+            for (int g = 4; g < heads; ++g) add(*reinterpret_cast<const float4*>(logits + g * p.logit_stride), g);
+            *reinterpret_cast<float4*>(p.weights_out + wrow + t) = make_float4(old.x + sum.x, old.y + sum.y, old.z + sum.z, old.w + sum.w);
+        } else {
+            for (int i = 0; i < (four ? 4 : 1) && t + i < end; ++i) {
+                float w = 0.0F;
+#pragma unroll 4
+                for (int g = 0; g < heads; ++g) w = fmaf(exp2_fast(logits[g * p.logit_stride + i] - stats[g].x), stats[g].y, w);
+                p.weights_out[wrow + t + i] = (before ? before[wrow + t + i] : 0.0F) + w;
+            }
         }
     }
     if (p.positions && first <= ctx - 1 && ctx - 1 < end && threadIdx.x == 0) p.positions[wrow + ctx - 1] = p.query_position[b];
@@ -463,11 +430,10 @@ sfb_status sfb_k_attention_decode_weights(const sfb_weights_args* a, sfb_stream 
                         l.logit_stride, a->q_heads, a->weight_stride,
                         a->weight_stride % 4 == 0 && aligned16(a->weights) && aligned16(a->weights_out)};
     const int group = a->q_heads / a->kv_heads;
-    // few CTAs: one position a thread; many: four, and at last sixteen, so that the statistics are read less often
+    // one position a thread as long as that leaves at most eight CTAs per SM, else four
     const int64_t pairs = static_cast<int64_t>(a->kv_heads) * a->batch;
-    int chunk = kAddThreads;
-    while (chunk < 16 * kAddThreads && pairs * ceil_div(p.kv.limit, chunk) > 8LL * sm_count()) chunk *= 4;
-    const dim3 grid(ceil_div(p.kv.limit, chunk), a->kv_heads, a->batch);
+    const int chunk = pairs * ceil_div(p.kv.limit, kAddThreads) <= 8LL * sm_count() ? kAddThreads : 4 * kAddThreads;
+    const dim3 grid(group + ceil_div(p.kv.limit, chunk), a->kv_heads, a->batch);
     if (a->dtype == SFB_F32) SFB_CUDA(launch_dependent(add_weights_kernel<float>, grid, dim3(kAddThreads), 0, s, add, chunk));
     else SFB_CUDA(launch_dependent(add_weights_kernel<bf16>, grid, dim3(kAddThreads), 0, s, add, chunk));
     return check_launch("decode_weights_add");

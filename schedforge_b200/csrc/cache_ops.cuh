@@ -140,6 +140,12 @@ template <> struct Raw8<bf16> {
     }
 };
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Where the pieces of query row (b, head) lie: indices first + i * step, i < count.  ctx: the sequence's length.
 struct RowPieces {
     size_t first;
@@ -156,23 +162,34 @@ __device__ __forceinline__ RowPieces row_pieces(const Partials& part, int kv_hea
 }
 
 // Maximum and 1 / sum of a row (0 for an empty one) out of its pieces, by one warp; factors != nullptr: the factor of
-// every piece.
+// every piece.  Up to 64 pieces are read once, all at the same time.
 __device__ __forceinline__ float2 row_statistics(const Partials& part, const RowPieces& r, float* factors) {
     const int lane = threadIdx.x & 31;
-    float top = -INFINITY, sum = 0.0F;
-    for (int i = lane; i < r.count; i += 32) top = fmaxf(top, part.ml[(r.first + static_cast<size_t>(i) * r.step) * part.ml_step]);
+    const auto read = [&](int i) -> float2 {
+        const float* at = part.ml + (r.first + static_cast<size_t>(i) * r.step) * part.ml_step;
+        return i < r.count ? make_float2(at[0], at[1]) : make_float2(-INFINITY, 0.0F);
+    };
+    const float2 a = read(lane), b = read(lane + 32);
+    float top = fmaxf(a.x, b.x);
+    for (int i = lane + 64; i < r.count; i += 32) top = fmaxf(top, read(i).x);
     top = warp_max(top);
     if (top == -INFINITY) top = 0.0F;
-    for (int i = lane; i < r.count; i += 32) {
-        const float* ml = part.ml + (r.first + static_cast<size_t>(i) * r.step) * part.ml_step;
-        const float f = ml[0] == -INFINITY ? 0.0F : exp2f(ml[0] - top);
-        sum += ml[1] * f;
-        if (factors) factors[i] = f;
+    const float fa = a.x == -INFINITY ? 0.0F : exp2_fast(a.x - top), fb = b.x == -INFINITY ? 0.0F : exp2_fast(b.x - top);
+    float sum = a.y * fa + b.y * fb;
+    for (int i = lane + 64; i < r.count; i += 32) {
+        const float2 v = read(i);
+        sum += v.x == -INFINITY ? 0.0F : v.y * exp2_fast(v.x - top);
     }
     sum = warp_sum(sum);
     const float inv = sum == 0.0F ? 0.0F : 1.0F / sum;
-    if (factors)
-        for (int i = lane; i < r.count; i += 32) factors[i] *= inv;   // (its own entries)
+    if (factors) {
+        if (lane < r.count) factors[lane] = fa * inv;
+        if (lane + 32 < r.count) factors[lane + 32] = fb * inv;
+        for (int i = lane + 64; i < r.count; i += 32) {
+            const float2 v = read(i);
+            factors[i] = v.x == -INFINITY ? 0.0F : exp2_fast(v.x - top) * inv;
+        }
+    }
     return make_float2(top, inv);
 }
 
@@ -218,11 +235,6 @@ __device__ __forceinline__ void even_range(int batch, int64_t subs, int granule,
     }
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 #endif
 
 }  // namespace sfb
