@@ -32,7 +32,6 @@ template <class T>
 __global__ void __launch_bounds__(128)
 bounds_kernel(const __grid_constant__ PagedView kv, const int* __restrict__ start_len, T* __restrict__ bounds, int vec) {
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int end = kv.length(b), start = max(0, start_len[b]);
     if (start >= end) return;
@@ -90,7 +89,6 @@ score_kernel(const __grid_constant__ ScoreParams p) {
     __shared__ float size_of[4];
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int ctx = kv.length(b);
     const int blocks = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
@@ -181,7 +179,6 @@ score_vec_kernel(const __grid_constant__ ScoreParams p) {
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
     }
-    grid_dependents_may_launch();
     grid_dependency_wait();
     __syncthreads();
     const int ctx = kv.length(b);
@@ -360,7 +357,6 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
         ptx::fence_barrier_init();
         ptx::fence_proxy_async();
     }
-    grid_dependents_may_launch();
     grid_dependency_wait();
     __syncthreads();
     const int ctx = kv.length(b);
@@ -644,7 +640,6 @@ select_kernel(const __grid_constant__ SelectParams p) {
     __shared__ int counts[2];
     const PagedView& kv = p.kv;
     const int b = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int ctx = kv.length(b);
     const int n = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;

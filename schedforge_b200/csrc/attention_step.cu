@@ -52,7 +52,6 @@ step_kernel(const __grid_constant__ StepParams p) {
     const int chunks = (group + G - 1) / G;
     const int kvh = blockIdx.y / chunks, head0 = kvh * group + (blockIdx.y % chunks) * G;
     const int heads = min(G, (kvh + 1) * group - head0);
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int ctx = kv.length(b);
     const int* list = p.selected ? p.selected + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.budget : nullptr;
@@ -239,7 +238,6 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Merg
     __shared__ float other[128];
     const int row = blockIdx.x;
     const int node = row % p.nodes, head = (row / p.nodes) % p.q_heads, b = row / p.nodes / p.q_heads;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     if (p.node_count && node >= p.node_count[b]) return;
     RowPieces r;

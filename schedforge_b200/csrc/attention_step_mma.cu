@@ -99,7 +99,6 @@ step_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         ptx::prefetch_tensormap(&map_k);
         ptx::prefetch_tensormap(&map_v);
     }
-    grid_dependents_may_launch();
     grid_dependency_wait();
     if (warp == 4) even_range(p.batch, subs, kUnits, [&](int b) { return Walk::units_of(p, kv.length(b)); }, start);
     __syncthreads();

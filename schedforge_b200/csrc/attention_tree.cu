@@ -3,56 +3,62 @@
 //
 // The query rows of one (sequence, K/V head) are the group's heads times the nodes, contiguous in memory.  The keys are
 // the committed positions followed by the drafted nodes; a row sees all of the first and its ancestors of the second,
-// kept as one bit per (node, node).  A CTA takes 64 rows and a range of keys (split) in tiles of 64 keys: scores and
-// products as register-blocked 4x4 outer products out of shared memory, online softmax per row, partial results of the
-// splits merged afterwards.
+// kept as one bit per (node, node).  A CTA takes 64 rows and a range of keys (split) in tiles of 64 keys.  Scores and
+// products are register-blocked outer products out of shared memory: a thread has 8 rows (4 where the value dimension
+// is above 128) and 4 keys, so a four-element step costs 12 wide shared-memory reads for 128 multiply-adds, and the
+// fp32 pipe is the bound, not the reads.  A row belongs to 16 lanes of one warp, which exchange its maximum by shuffles and
+// its weights through shared memory without a CTA barrier.  Several CTAs per SM cover the loads of one another.
 #include "attention_tree.cuh"
 
 namespace sfb {
 namespace {
 
-constexpr int BM = 64, BN = 64, kThreads = 256;
+constexpr int BM = 64, BN = 64;
 constexpr int kPStride = BN + 4;
+
+template <int NV> struct TreeTile {
+    static constexpr int kRows = NV <= 2 ? 8 : 4;             // query rows of a thread
+    static constexpr int kThreads = BM / kRows * 16;
+};
 
 __host__ __device__ inline int padded(int dim) { return ((dim + 3) & ~3) + 4; }  // floats per Q / K row in shared memory
 
 size_t tree_smem(int dim, int nv) {
     return sizeof(float) * (static_cast<size_t>(BM + BN) * padded(dim) + static_cast<size_t>(BN) * nv * 64 + static_cast<size_t>(BM) * kPStride) +
-           sizeof(uint32_t) * 8 * SFB_MAX_TREE_NODES + sizeof(int) * SFB_MAX_TREE_NODES;
+           2 * sizeof(void*) * BN + sizeof(uint32_t) * 8 * SFB_MAX_TREE_NODES + sizeof(int) * SFB_MAX_TREE_NODES;
 }
 
-// Loads `rows` rows of dim elements into [64][stride] floats, zero beyond; row(r) gives the element offset or -1.
-template <class T, class Row>
-__device__ __forceinline__ void load_tile(float* dst, int stride, const T* src, int dim, bool vec, float factor, Row row) {
-    const int width = (dim + 3) & ~3;
-    for (int i = threadIdx.x; i < 64 * (width / 4); i += kThreads) {
-        const int r = i / (width / 4), d = (i % (width / 4)) * 4;
-        const int64_t at = row(r);
-        float v[4] = {0.0F, 0.0F, 0.0F, 0.0F};
-        if (at >= 0) {
-            const T* p = src + at * dim + d;
-            if (vec) {
-                if constexpr (sizeof(T) == 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(p);
-                    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-                } else {
-                    const uint2 f = *reinterpret_cast<const uint2*>(p);
-                    v[0] = __uint_as_float(f.x << 16); v[1] = __uint_as_float(f.x & 0xffff0000u);
-                    v[2] = __uint_as_float(f.y << 16); v[3] = __uint_as_float(f.y & 0xffff0000u);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (d + j < dim) v[j] = to_float(p[j]);
-            }
+template <class T>
+__device__ __forceinline__ float4 load4(const T* p, int left, bool vec) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(p);
+        else {
+            const uint2 f = *reinterpret_cast<const uint2*>(p);
+            return make_float4(__uint_as_float(f.x << 16), __uint_as_float(f.x & 0xffff0000u), __uint_as_float(f.y << 16),
+                               __uint_as_float(f.y & 0xffff0000u));
         }
-        *reinterpret_cast<float4*>(dst + r * stride + d) = make_float4(v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
+    }
+    return make_float4(to_float(p[0]), left > 1 ? to_float(p[1]) : 0.0F, left > 2 ? to_float(p[2]) : 0.0F, left > 3 ? to_float(p[3]) : 0.0F);
+}
+
+// 64 rows of dim elements into [64][stride] floats, zero where row(r) is nullptr and behind the row's end.
+template <int THREADS, class T, class Row>
+__device__ __forceinline__ void load_tile(float* dst, int stride, int dim, int width, bool vec, float factor, Row row) {
+    const int pieces = width / 4;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < 64 * pieces; i += THREADS) {
+        const int r = i / pieces, d = (i - r * pieces) * 4;
+        const T* src = row(r);
+        float4 v = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+        if (src && d < dim) v = load4(src + d, dim - d, vec);
+        *reinterpret_cast<float4*>(dst + r * stride + d) = make_float4(v.x * factor, v.y * factor, v.z * factor, v.w * factor);
     }
 }
 
 template <class T, int NV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(TreeTile<NV>::kThreads)
 tree_simt_kernel(const __grid_constant__ TreeParams p) {
+    constexpr int kThreads = TreeTile<NV>::kThreads, R = TreeTile<NV>::kRows;
     extern __shared__ float4 tree_smem_raw[];
     const PagedView& kv = p.kv;
     const int stride = padded(kv.dim);
@@ -60,32 +66,33 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     float* ks = qs + BM * stride;                          // [BN][stride]
     float* vs = ks + BN * stride;                          // [BN][NV * 64]
     float* ps = vs + BN * NV * 64;                         // [BM][kPStride]
-    uint32_t* seen = reinterpret_cast<uint32_t*>(ps + BM * kPStride);  // [nodes][8]
+    const T** k_rows = reinterpret_cast<const T**>(ps + BM * kPStride);   // [BN] the tile's rows in memory, nullptr: masked
+    const T** v_rows = k_rows + BN;
+    uint32_t* seen = reinterpret_cast<uint32_t*>(v_rows + BN);            // [nodes][8]
     int* parent = reinterpret_cast<int*>(seen + 8 * SFB_MAX_TREE_NODES);
     const int group = p.q_heads / kv.kv_heads, rows_all = group * p.nodes;
     const int row_tiles = (rows_all + BM - 1) / BM;
     const int tile = blockIdx.x % row_tiles, split = blockIdx.x / row_tiles;
     const int kvh = blockIdx.y, b = blockIdx.z;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int ctx = kv.length(b);
     const int count = tree_node_count(p, b);
     const int keys = ctx + count;
     const int k0 = min(keys, split * p.chunk), k1 = split == p.splits - 1 ? keys : min(keys, k0 + p.chunk);
     const int row0 = tile * BM;
-    const bool has_draft = k1 > ctx;
-    if (has_draft) tree_ancestors(p, b, count, parent, seen);
+    if (k1 > ctx) tree_ancestors(p, b, count, parent, seen);
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all * kv.dim;
-    load_tile(qs, stride, q, kv.dim, p.vec, p.scale_log2, [&](int r) -> int64_t { return row0 + r < rows_all ? row0 + r : -1; });
-
-    float o[4][NV * 4], m[4], l[4];
-    int node[4];
+    if (k0 < k1)
+        load_tile<kThreads, T>(qs, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, p.scale_log2,
+                               [&](int r) { return row0 + r < rows_all ? q + static_cast<size_t>(row0 + r) * kv.dim : nullptr; });
+    float o[R][NV * 4], m[R], l[R];
+    int node[R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.0F;
-        node[i] = (row0 + ty * 4 + i) % p.nodes;
+        node[i] = (row0 + ty * R + i) % p.nodes;
 #pragma unroll
         for (int j = 0; j < NV * 4; ++j) o[i][j] = 0.0F;
     }
@@ -93,64 +100,61 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     const T* draft_v = static_cast<const T*>(p.draft_v) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim_v;
     for (int t0 = k0; t0 < k1; t0 += BN) {
         __syncthreads();
-        // committed rows come from the pool, drafted ones from their own tensors; a tile may hold both
-        const int from_pool = min(max(ctx - t0, 0), BN), live = min(BN, k1 - t0);
-        const auto pool_row = [&](int r) -> int64_t { return r < min(from_pool, live) ? kv.row(b, kvh, t0 + r) : -1; };
-        if (from_pool > 0) {
-            load_tile(ks, stride, static_cast<const T*>(kv.k_pool), kv.dim, p.vec, 1.0F, pool_row);
-            load_tile(vs, NV * 64, static_cast<const T*>(kv.v_pool), kv.dim_v, p.vec, 1.0F, pool_row);
-        }
-        if (from_pool < live) {
-            if (from_pool > 0) __syncthreads();
-            const auto draft_row = [&](int r) -> int64_t { return r >= from_pool && r < live ? t0 + r - ctx : -2; };
-            // (-2 in a mixed tile: the row was loaded above and must stay)
-            const auto mixed = [&](float* dst, int st, const T* src, int dim) {
-                const int width = (dim + 3) & ~3;
-                for (int i = threadIdx.x; i < 64 * (width / 4); i += kThreads) {
-                    const int r = i / (width / 4), d = (i % (width / 4)) * 4;
-                    const int64_t at = draft_row(r);
-                    if (at == -2 && r < from_pool) continue;
-                    float v[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = at >= 0 && d + j < dim ? to_float(src[at * dim + d + j]) : 0.0F;
-                    *reinterpret_cast<float4*>(dst + r * st + d) = make_float4(v[0], v[1], v[2], v[3]);
+        // committed rows come from the pool, drafted ones from their own tensors
+        if (threadIdx.x < BN) {
+            const int key = t0 + threadIdx.x;
+            const T *kr = nullptr, *vr = nullptr;
+            if (key < min(k1, ctx)) {
+                const int64_t at = kv.row(b, kvh, key);
+                if (at >= 0) {
+                    kr = static_cast<const T*>(kv.k_pool) + at * kv.dim;
+                    vr = static_cast<const T*>(kv.v_pool) + at * kv.dim_v;
                 }
-            };
-            mixed(ks, stride, draft_k, kv.dim);
-            mixed(vs, NV * 64, draft_v, kv.dim_v);
+            } else if (key < k1) {
+                kr = draft_k + static_cast<size_t>(key - ctx) * kv.dim;
+                vr = draft_v + static_cast<size_t>(key - ctx) * kv.dim_v;
+            }
+            k_rows[threadIdx.x] = kr;
+            v_rows[threadIdx.x] = vr;
         }
         __syncthreads();
-        float s[4][4] = {};
+        load_tile<kThreads, T>(ks, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, 1.0F, [&](int r) { return k_rows[r]; });
+        load_tile<kThreads, T>(vs, NV * 64, kv.dim_v, NV * 64, p.vec, 1.0F, [&](int r) { return v_rows[r]; });
+        __syncthreads();
+        float s[R][4] = {};
+#pragma unroll 2
         for (int d = 0; d < kv.dim; d += 4) {
-            float4 qa[4], ka[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) qa[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * stride + d);
+            float4 ka[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) ka[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * stride + d);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < R; ++i) {
+                const float4 qa = *reinterpret_cast<const float4*>(qs + (ty * R + i) * stride + d);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    s[i][j] = fmaf(qa[i].x, ka[j].x, s[i][j]);
-                    s[i][j] = fmaf(qa[i].y, ka[j].y, s[i][j]);
-                    s[i][j] = fmaf(qa[i].z, ka[j].z, s[i][j]);
-                    s[i][j] = fmaf(qa[i].w, ka[j].w, s[i][j]);
+                    s[i][j] = fmaf(qa.x, ka[j].x, s[i][j]);
+                    s[i][j] = fmaf(qa.y, ka[j].y, s[i][j]);
+                    s[i][j] = fmaf(qa.z, ka[j].z, s[i][j]);
+                    s[i][j] = fmaf(qa.w, ka[j].w, s[i][j]);
                 }
+            }
         }
+        if (t0 + BN > ctx || t0 + BN > k1) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int key = t0 + tx + 16 * j;
-            const bool inside = key < k1;
-            const bool draft = key >= ctx;
-            const bool there = inside && (draft || kv.row(b, kvh, key) >= 0);
+            for (int j = 0; j < 4; ++j) {
+                const int key = t0 + tx + 16 * j;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool visible = there && (!draft || (seen[node[i] * 8 + ((key - ctx) >> 5)] >> ((key - ctx) & 31) & 1u));
-                if (!visible) s[i][j] = -INFINITY;
+                for (int i = 0; i < R; ++i)
+                    if (key >= k1 || (key >= ctx && !(seen[node[i] * 8 + ((key - ctx) >> 5)] >> ((key - ctx) & 31) & 1u))) s[i][j] = -INFINITY;
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 4; ++j)
+            if (!k_rows[tx + 16 * j])
+#pragma unroll
+                for (int i = 0; i < R; ++i) s[i][j] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
             float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
             for (int w = 1; w < 16; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
@@ -164,36 +168,41 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
             for (int j = 0; j < 4; ++j) {
                 const float e = s[i][j] == -INFINITY ? 0.0F : exp2f(s[i][j] - top);
                 l[i] += e;   // this lane's share of the row sum
-                ps[(ty * 4 + i) * kPStride + tx + 16 * j] = e;
+                ps[(ty * R + i) * kPStride + tx + 16 * j] = e;
             }
         }
-        __syncthreads();
-        for (int k = 0; k < live; ++k) {
-            float e[4];
+        __syncwarp();   // (a row's lanes are in one warp)
+#pragma unroll 2
+        for (int k = 0; k < BN; k += 4) {
+            float4 e[R];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = ps[(ty * 4 + i) * kPStride + k];
+            for (int i = 0; i < R; ++i) e[i] = *reinterpret_cast<const float4*>(ps + (ty * R + i) * kPStride + k);
 #pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const float4 v = *reinterpret_cast<const float4*>(vs + k * NV * 64 + c * 64 + tx * 4);
+            for (int c = 0; c < NV; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[i][c * 4] = fmaf(e[i], v.x, o[i][c * 4]);
-                    o[i][c * 4 + 1] = fmaf(e[i], v.y, o[i][c * 4 + 1]);
-                    o[i][c * 4 + 2] = fmaf(e[i], v.z, o[i][c * 4 + 2]);
-                    o[i][c * 4 + 3] = fmaf(e[i], v.w, o[i][c * 4 + 3]);
+                for (int u = 0; u < 4; ++u) {
+                    const float4 v = *reinterpret_cast<const float4*>(vs + (k + u) * NV * 64 + c * 64 + tx * 4);
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        const float w = u == 0 ? e[i].x : u == 1 ? e[i].y : u == 2 ? e[i].z : e[i].w;
+                        o[i][c * 4] = fmaf(w, v.x, o[i][c * 4]);
+                        o[i][c * 4 + 1] = fmaf(w, v.y, o[i][c * 4 + 1]);
+                        o[i][c * 4 + 2] = fmaf(w, v.z, o[i][c * 4 + 2]);
+                        o[i][c * 4 + 3] = fmaf(w, v.w, o[i][c * 4 + 3]);
+                    }
                 }
-            }
         }
+        __syncwarp();
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < R; ++i) {
 #pragma unroll
         for (int w = 1; w < 16; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-        const int r = row0 + ty * 4 + i;
+        const int r = row0 + ty * R + i;
         if (r >= rows_all || node[i] >= count) continue;
         const size_t row = (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all + r;
         if (p.splits == 1) {
-            const float inv = l[i] > 0.0F ? 1.0F / l[i] : (l[i] == 0.0F ? 0.0F : l[i]);
+            const float inv = l[i] == 0.0F ? 0.0F : 1.0F / l[i];
             T* dst = static_cast<T*>(p.out) + tree_out_row(p, b, kvh * group + r / p.nodes, node[i]) * kv.dim_v;
 #pragma unroll
             for (int c = 0; c < NV; ++c)
@@ -218,7 +227,7 @@ sfb_status launch_tree(const TreeParams& p, cudaStream_t stream) {
     SFB_CUDA(cudaFuncSetAttribute(tree_simt_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     const int rows = p.q_heads / p.kv.kv_heads * p.nodes;
     const dim3 grid(ceil_div(rows, BM) * p.splits, p.kv.kv_heads, p.batch);
-    SFB_CUDA(launch_dependent(tree_simt_kernel<T, NV>, grid, dim3(kThreads), smem, stream, p));
+    SFB_CUDA(launch_dependent(tree_simt_kernel<T, NV>, grid, dim3(TreeTile<NV>::kThreads), smem, stream, p));
     return check_launch("attention_tree");
 }
 
@@ -237,7 +246,7 @@ struct TreeLayout {
     size_t total;
 };
 
-// Splits of the key axis: tiles of 64 keys, as many splits as fill the GPU about twice, no split below 256 keys.
+// Splits of the key axis: tiles of 64 keys, about four CTAs per SM, no split below 128 keys.
 TreeLayout tree_layout(const sfb_tree_args& a) {
     TreeLayout l{};
     const int covered = a.max_blocks * a.block_tokens;
@@ -245,8 +254,8 @@ TreeLayout tree_layout(const sfb_tree_args& a) {
     const int64_t base = static_cast<int64_t>(a.batch) * a.kv_heads * ceil_div(a.q_heads / a.kv_heads * a.nodes, BM);
     int splits = a.splits;
     if (splits <= 0) {
-        const int64_t wanted = (2LL * sm_count() + base - 1) / base;
-        const int most = ceil_div(limit, 256);
+        const int64_t wanted = (4LL * sm_count() + base - 1) / base;
+        const int most = ceil_div(limit, 128);
         splits = static_cast<int>(wanted < most ? wanted : most);
     }
     if (splits > 128) splits = 128;

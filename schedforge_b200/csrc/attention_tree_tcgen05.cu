@@ -157,7 +157,6 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
         ptx::tmem_relinquish();
     }
-    grid_dependents_may_launch();
     grid_dependency_wait();
     if (warp == 10) {
         even_range(t_.batch, static_cast<int64_t>(kv.kv_heads) * p.row_groups, 1,
@@ -561,7 +560,6 @@ __global__ void __launch_bounds__(256)
 tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
     constexpr int V = D / 32;
     const TreeParams& t = p.t;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31;
     const int slices = rows_cta / 8;

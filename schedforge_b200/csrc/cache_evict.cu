@@ -42,7 +42,6 @@ add_weights_kernel(const __grid_constant__ AddParams p, int chunk) {
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = p.q_heads / kv.kv_heads;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const size_t row0 = static_cast<size_t>(b) * p.q_heads + kvh * group;
     const int ctx = kv.length(b);
@@ -200,7 +199,6 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     __shared__ int newest_of[32];
     const PagedView& kv = p.kv;
     const int b = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int n = kv.length(b), k = min(n, p.budget);
     const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
@@ -305,7 +303,6 @@ __global__ void __launch_bounds__(256)
 evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_units) {
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int* to = p.moves + (static_cast<size_t>(b) * kv.kv_heads + kvh) * (2 + 2 * static_cast<size_t>(p.max_moves)) + 2;
     const int* since = to + p.max_moves;
@@ -365,7 +362,6 @@ __global__ void __launch_bounds__(256)
 accept_kernel(const __grid_constant__ AcceptParams p, int k_units, int v_units) {
     const PagedView& kv = p.kv;
     const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dependents_may_launch();
     grid_dependency_wait();
     const int start = kv.lens[b];
     int count = p.path_len[b];

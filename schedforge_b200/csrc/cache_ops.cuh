@@ -1,5 +1,9 @@
-// Shared pieces of the serving operators over the paged cache: guarded cache access, the split bookkeeping of the
-// decode kernels and the merge of their partial results.
+// Shared pieces of the serving operators over the paged cache: guarded cache access, the bookkeeping of cut work and the
+// joining of partial results.
+//
+// The kernels are launched with launch_dependent() and wait for the kernel before at once; none announces its dependents
+// early: blocks that came in ahead of time only took room from the ones they waited for (one eviction step 11.8 us with
+// griddepcontrol.launch_dependents at the start of its kernels, 9.2 us without).
 #pragma once
 
 #include "attention_decode.cuh"
