@@ -6,8 +6,7 @@
 // kept as one bit per (node, node).  A CTA takes 64 rows and a range of keys (split) in tiles of 64 keys.  Scores and
 // products are register-blocked outer products out of shared memory: a thread has 8 rows (4 where the value dimension
 // is above 128) and 4 keys, so a four-element step costs 12 wide shared-memory reads for 128 multiply-adds, and the
-// fp32 pipe is the bound, not the reads.  A row belongs to 16 lanes of one warp, which exchange its maximum by shuffles and
-// its weights through shared memory without a CTA barrier.  Several CTAs per SM cover the loads of one another.
+// fp32 pipe is the bound, not the reads.  A row belongs to 16 lanes of one warp, which exchange its maximum by shuffles.
 #include "attention_tree.cuh"
 
 namespace sfb {
@@ -23,9 +22,9 @@ template <int NV> struct TreeTile {
 
 __host__ __device__ inline int padded(int dim) { return ((dim + 3) & ~3) + 4; }  // floats per Q / K row in shared memory
 
-size_t tree_smem(int dim, int nv) {
+size_t tree_smem(int dim, int nv, int nodes) {
     return sizeof(float) * (static_cast<size_t>(BM + BN) * padded(dim) + static_cast<size_t>(BN) * nv * 64 + static_cast<size_t>(BM) * kPStride) +
-           2 * sizeof(void*) * BN + sizeof(uint32_t) * 8 * SFB_MAX_TREE_NODES + sizeof(int) * SFB_MAX_TREE_NODES;
+           4 * sizeof(void*) * BN + sizeof(uint32_t) * 9 * nodes;
 }
 
 template <class T>
@@ -41,10 +40,24 @@ __device__ __forceinline__ float4 load4(const T* p, int left, bool vec) {
     return make_float4(to_float(p[0]), left > 1 ? to_float(p[1]) : 0.0F, left > 2 ? to_float(p[2]) : 0.0F, left > 3 ? to_float(p[3]) : 0.0F);
 }
 
-// 64 rows of dim elements into [64][stride] floats, zero where row(r) is nullptr and behind the row's end.
-template <int THREADS, class T, class Row>
+// 64 rows of dim elements into [64][stride] floats, zero where row(r) is nullptr and behind the row's end.  ASYNC
+// (float32, 16-byte aligned rows, factor 1): by cp.async, to be waited for.
+template <int THREADS, class T, bool ASYNC, class Row>
 __device__ __forceinline__ void load_tile(float* dst, int stride, int dim, int width, bool vec, float factor, Row row) {
     const int pieces = width / 4;
+    if constexpr (ASYNC && sizeof(T) == 4) {
+        if (vec) {
+#pragma unroll 8
+            for (int i = threadIdx.x; i < 64 * pieces; i += THREADS) {
+                const int r = i / pieces, d = (i - r * pieces) * 4;
+                const T* src = row(r);
+                const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * stride + d));
+                if (src && d < dim) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(src + d) : "memory");
+                else *reinterpret_cast<float4*>(dst + r * stride + d) = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+            }
+            return;
+        }
+    }
 #pragma unroll 8
     for (int i = threadIdx.x; i < 64 * pieces; i += THREADS) {
         const int r = i / pieces, d = (i - r * pieces) * 4;
@@ -66,10 +79,10 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     float* ks = qs + BM * stride;                          // [BN][stride]
     float* vs = ks + BN * stride;                          // [BN][NV * 64]
     float* ps = vs + BN * NV * 64;                         // [BM][kPStride]
-    const T** k_rows = reinterpret_cast<const T**>(ps + BM * kPStride);   // [BN] the tile's rows in memory, nullptr: masked
-    const T** v_rows = k_rows + BN;
-    uint32_t* seen = reinterpret_cast<uint32_t*>(v_rows + BN);            // [nodes][8]
-    int* parent = reinterpret_cast<int*>(seen + 8 * SFB_MAX_TREE_NODES);
+    const T** k_rows = reinterpret_cast<const T**>(ps + BM * kPStride);   // [2][BN] rows of this and the next tile, nullptr: masked
+    const T** v_rows = k_rows + 2 * BN;
+    uint32_t* seen = reinterpret_cast<uint32_t*>(v_rows + 2 * BN);        // [nodes][8]
+    int* parent = reinterpret_cast<int*>(seen + 8 * p.nodes);
     const int group = p.q_heads / kv.kv_heads, rows_all = group * p.nodes;
     const int row_tiles = (rows_all + BM - 1) / BM;
     const int tile = blockIdx.x % row_tiles, split = blockIdx.x / row_tiles;
@@ -84,7 +97,7 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     if (k1 > ctx) tree_ancestors(p, b, count, parent, seen);
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all * kv.dim;
     if (k0 < k1)
-        load_tile<kThreads, T>(qs, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, p.scale_log2,
+        load_tile<kThreads, T, false>(qs, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, p.scale_log2,
                                [&](int r) { return row0 + r < rows_all ? q + static_cast<size_t>(row0 + r) * kv.dim : nullptr; });
     float o[R][NV * 4], m[R], l[R];
     int node[R];
@@ -98,28 +111,46 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     }
     const T* draft_k = static_cast<const T*>(p.draft_k) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim;
     const T* draft_v = static_cast<const T*>(p.draft_v) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim_v;
-    for (int t0 = k0; t0 < k1; t0 += BN) {
-        __syncthreads();
-        // committed rows come from the pool, drafted ones from their own tensors
-        if (threadIdx.x < BN) {
-            const int key = t0 + threadIdx.x;
-            const T *kr = nullptr, *vr = nullptr;
-            if (key < min(k1, ctx)) {
-                const int64_t at = kv.row(b, kvh, key);
-                if (at >= 0) {
-                    kr = static_cast<const T*>(kv.k_pool) + at * kv.dim;
-                    vr = static_cast<const T*>(kv.v_pool) + at * kv.dim_v;
-                }
-            } else if (key < k1) {
-                kr = draft_k + static_cast<size_t>(key - ctx) * kv.dim;
-                vr = draft_v + static_cast<size_t>(key - ctx) * kv.dim_v;
+    // committed rows come from the pool, drafted ones from their own tensors
+    const auto find_rows = [&](int t0, int buffer) {
+        if (threadIdx.x >= BN) return;
+        const int key = t0 + threadIdx.x;
+        const T *kr = nullptr, *vr = nullptr;
+        if (key < min(k1, ctx)) {
+            const int64_t at = kv.row(b, kvh, key);
+            if (at >= 0) {
+                kr = static_cast<const T*>(kv.k_pool) + at * kv.dim;
+                vr = static_cast<const T*>(kv.v_pool) + at * kv.dim_v;
             }
-            k_rows[threadIdx.x] = kr;
-            v_rows[threadIdx.x] = vr;
+        } else if (key < k1) {
+            kr = draft_k + static_cast<size_t>(key - ctx) * kv.dim;
+            vr = draft_v + static_cast<size_t>(key - ctx) * kv.dim_v;
         }
+        k_rows[buffer * BN + threadIdx.x] = kr;
+        v_rows[buffer * BN + threadIdx.x] = vr;
+    };
+    // K of the next tile is fetched under the softmax and the P.V of this one, V under the scores of the next
+    const auto fetch_k = [&](int buffer) {
+        load_tile<kThreads, T, true>(ks, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, 1.0F, [&](int r) { return k_rows[buffer * BN + r]; });
+    };
+    const auto fetch_v = [&](int buffer) {
+        load_tile<kThreads, T, true>(vs, NV * 64, kv.dim_v, NV * 64, p.vec, 1.0F, [&](int r) { return v_rows[buffer * BN + r]; });
+    };
+    const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    const auto wait_but_one = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
+    if (k0 < k1) {
+        find_rows(k0, 0);
         __syncthreads();
-        load_tile<kThreads, T>(ks, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, 1.0F, [&](int r) { return k_rows[r]; });
-        load_tile<kThreads, T>(vs, NV * 64, kv.dim_v, NV * 64, p.vec, 1.0F, [&](int r) { return v_rows[r]; });
+        fetch_k(0);
+        commit();
+        fetch_v(0);
+        commit();
+    }
+    int buffer = 0;
+    for (int t0 = k0; t0 < k1; t0 += BN, buffer ^= 1) {
+        const bool more = t0 + BN < k1;
+        if (more) find_rows(t0 + BN, buffer ^ 1);
+        wait_but_one();      // K
         __syncthreads();
         float s[R][4] = {};
 #pragma unroll 2
@@ -150,9 +181,12 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (!k_rows[tx + 16 * j])
+            if (!k_rows[buffer * BN + tx + 16 * j])
 #pragma unroll
                 for (int i = 0; i < R; ++i) s[i][j] = -INFINITY;
+        __syncthreads();
+        if (more) fetch_k(buffer ^ 1);
+        commit();
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float top = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
@@ -171,7 +205,8 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
                 ps[(ty * R + i) * kPStride + tx + 16 * j] = e;
             }
         }
-        __syncwarp();   // (a row's lanes are in one warp)
+        wait_but_one();      // V
+        __syncthreads();
 #pragma unroll 2
         for (int k = 0; k < BN; k += 4) {
             float4 e[R];
@@ -192,7 +227,9 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
                     }
                 }
         }
-        __syncwarp();
+        __syncthreads();
+        if (more) fetch_v(buffer ^ 1);
+        commit();
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -223,7 +260,7 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
 
 template <class T, int NV>
 sfb_status launch_tree(const TreeParams& p, cudaStream_t stream) {
-    const size_t smem = tree_smem(p.kv.dim, NV);
+    const size_t smem = tree_smem(p.kv.dim, NV, p.nodes);
     SFB_CUDA(cudaFuncSetAttribute(tree_simt_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     const int rows = p.q_heads / p.kv.kv_heads * p.nodes;
     const dim3 grid(ceil_div(rows, BM) * p.splits, p.kv.kv_heads, p.batch);
