@@ -1,5 +1,5 @@
-// Attention of a tree of drafted tokens over a paged cache: the entry point, the split rule and the CUDA-core kernel
-// (float32, and bf16 with head dimensions the tensor-core kernel does not take).
+// Attention of a tree of drafted tokens over a paged cache: the entry point, the split rule and the CUDA-core kernel (types,
+// head dimensions and alignments that the tensor-core kernels do not take).
 //
 // The query rows of one (sequence, K/V head) are the group's heads times the nodes, contiguous in memory.  The keys are
 // the committed positions followed by the drafted nodes; a row sees all of the first and its ancestors of the second,
@@ -288,7 +288,7 @@ TreeLayout tree_layout(const sfb_tree_args& a) {
     TreeLayout l{};
     const int covered = a.max_blocks * a.block_tokens;
     const int limit = (a.max_context < covered ? a.max_context : covered) + a.nodes;
-    const int64_t base = static_cast<int64_t>(a.batch) * a.kv_heads * ceil_div(a.q_heads / a.kv_heads * a.nodes, BM);
+    const int64_t base = static_cast<int64_t>(a.batch) * a.kv_heads * ceil_div(a.q_heads / a.kv_heads * a.nodes, tree_tf32_shape(a) ? 128 : BM);
     int splits = a.splits;
     if (splits <= 0) {
         const int64_t wanted = (4LL * sm_count() + base - 1) / base;
@@ -344,9 +344,11 @@ sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* a, sfb_stream stream)
     p.batch = a->batch; p.q_heads = a->q_heads; p.nodes = a->nodes; p.token_major = a->token_major;
     p.splits = l.splits; p.chunk = l.chunk;
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
-    p.vec = a->head_dim % 4 == 0 && a->head_dim_value % 4 == 0 && aligned16(a->q) && aligned16(a->k_pool) && aligned16(a->v_pool);
+    p.vec = a->head_dim % 4 == 0 && a->head_dim_value % 4 == 0 && aligned16(a->q) && aligned16(a->k_pool) && aligned16(a->v_pool) && aligned16(a->draft_k) &&
+            aligned16(a->draft_v);
     if (tensor) return tree_tcgen05(*a, p, s);
-    SFB_TRY(a->dtype == SFB_F32 ? tree_simt<float>(p, s) : tree_simt<bf16>(p, s));
+    if (p.vec && aligned16(a->out) && tree_tf32_shape(*a)) SFB_TRY(tree_tf32(p, s));
+    else SFB_TRY(a->dtype == SFB_F32 ? tree_simt<float>(p, s) : tree_simt<bf16>(p, s));
     if (l.splits == 1) return SFB_OK;
     const Partials part{p.partials, p.partials + 2, nullptr, l.splits, a->head_dim_value + 2, a->head_dim_value + 2};
     return merge_partials({part, p.kv, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, a->token_major}, a->dtype, s);

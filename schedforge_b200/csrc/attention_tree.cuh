@@ -15,6 +15,11 @@ struct TreeParams {
     float scale_log2;
 };
 
+// float32, head dimensions that are multiples of 8 up to 128 (attention_tree_tf32.cu); the same layout of splits as the
+// CUDA-core kernel, with row tiles of 128.
+bool tree_tf32_shape(const sfb_tree_args& a);
+sfb_status tree_tf32(const TreeParams& p, cudaStream_t stream);
+
 // bf16, head_dim = head_dim_value = 128 or 64 (attention_tree_tcgen05.cu).
 bool tree_tcgen05_shape(const sfb_tree_args& a);        // types and sizes
 bool tree_tcgen05_supported(const sfb_tree_args& a);    // and addresses

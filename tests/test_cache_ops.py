@@ -110,6 +110,9 @@ TREE_CASES = [
     ("f32", 6, 2, 20, 12, 4, 7, [9, 64, 65], [7, 0, 7], 1, 0),          # dims and blocks that are no multiples of anything
     ("f32", 8, 8, 64, 64, 16, 27, [500, 130], [27, 20], 0, 3),
     ("f32", 8, 1, 256, 200, 32, 33, [70], [33], 0, 0),
+    ("f32", 8, 2, 128, 128, 16, 40, [300, 0, 64, 63], [40, 40, 33, 1], 1, 0),
+    ("f32", 4, 1, 72, 40, 16, 70, [129, 640], [70, 64], 0, 2),           # three tiles of 128 query rows, two of draft keys
+    ("f32", 2, 2, 8, 8, 16, 3, [70], [3], 0, 0),
     ("bf16", 8, 2, 64, 64, 16, 1, [300, 0, 17], [1, 1, 1], 0, 0),       # one token
     ("bf16", 8, 2, 128, 128, 16, 9, [300, 0, 17, 128], [9, 9, 4, 2], 0, 0),
     ("bf16", 32, 8, 128, 128, 16, 64, [700, 1000], [64, 50], 1, 0),     # two row tiles of 128
