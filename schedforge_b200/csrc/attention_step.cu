@@ -265,6 +265,37 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Merg
     }
 }
 
+// The same with one warp per output row, for many rows.
+template <class T>
+__global__ void __launch_bounds__(256) merge_rows_kernel(const __grid_constant__ MergeParams p, int rows) {
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const int node = row % p.nodes, head = (row / p.nodes) % p.q_heads, b = row / p.nodes / p.q_heads;
+    grid_dependency_wait();
+    if (p.node_count && node >= p.node_count[b]) return;
+    RowPieces r;
+    if (p.part.span) r = row_pieces(p.part, p.kv.kv_heads, p.q_heads, b, head, p.kv.length(b));
+    else r = {static_cast<size_t>(row) * p.part.splits, 1, p.part.splits};
+    if (p.part.span && r.count == 1) return;   // written by the attention kernel itself
+    const float2 stats = row_statistics(p.part, r, nullptr);
+    T* dst = static_cast<T*>(p.out) + (p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
+                                                     : static_cast<size_t>(row)) * p.dim_v;
+    float a[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < r.count; ++i) {
+        const size_t index = r.first + static_cast<size_t>(i) * r.step;
+        const float m = p.part.ml[index * p.part.ml_step];
+        const float f = m == -INFINITY ? 0.0F : exp2_fast(m - stats.x);
+        const float* o = p.part.o + index * p.part.o_step;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < p.dim_v) a[j] = f == 0.0F ? a[j] : fmaf(o[lane + 32 * j], f, a[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (lane + 32 * j < p.dim_v) dst[lane + 32 * j] = from_float<T>(a[j] * stats.y);
+}
+
 }  // namespace
 
 sfb_status check_cache(const void* k_pool, const void* v_pool, const int* table, int batch, int kv_heads, int dim, int dim_v,
@@ -343,7 +374,14 @@ sfb_status step_attention(const StepParams& p, const StepPlan& plan, int dtype, 
 }
 
 sfb_status merge_partials(const MergeParams& p, int dtype, cudaStream_t stream) {
+    // a CTA per row while that leaves at most four per SM (all pieces in flight at once), else a warp per row
     const int64_t rows = static_cast<int64_t>(p.batch) * p.q_heads * p.nodes;
+    if (rows > 4LL * sm_count()) {
+        const dim3 grid(static_cast<unsigned>(ceil_div64(rows, 8)));
+        if (dtype == SFB_F32) SFB_CUDA(launch_dependent(merge_rows_kernel<float>, grid, dim3(256), 0, stream, p, static_cast<int>(rows)));
+        else SFB_CUDA(launch_dependent(merge_rows_kernel<bf16>, grid, dim3(256), 0, stream, p, static_cast<int>(rows)));
+        return check_launch("attention_merge");
+    }
     const dim3 grid(static_cast<unsigned>(rows));
     if (dtype == SFB_F32) SFB_CUDA(launch_dependent(merge_kernel<float>, grid, dim3(256), 0, stream, p));
     else SFB_CUDA(launch_dependent(merge_kernel<bf16>, grid, dim3(256), 0, stream, p));

@@ -311,7 +311,7 @@ sfb_status check_tree(const sfb_tree_args* a) {
     SFB_REQUIRE(a->nodes > 0, "tree attention: no nodes");
     SFB_REQUIRE(a->max_context >= 0, "tree attention: negative max_context");
     if (a->nodes > SFB_MAX_TREE_NODES) return fail(SFB_UNSUPPORTED, "tree attention: more than 256 nodes");
-    if (static_cast<int64_t>(a->q_heads) * a->nodes > (1 << 24)) return fail(SFB_UNSUPPORTED, "tree attention: more than 2^24 query rows per sequence");
+    if (static_cast<int64_t>(a->batch) * a->q_heads * a->nodes > (1 << 28)) return fail(SFB_UNSUPPORTED, "tree attention: more than 2^28 query rows");
     return SFB_OK;
 }
 
