@@ -6,9 +6,8 @@
 // count falls to a fifth of the CUDA-core form (attention_tree.cu), which had no issue slots left to cover its
 // loads (16 sequences of up to 1500 tokens, 27 nodes, 64-dimensional heads: 68 us there).
 // A CTA takes 128 query rows of one (sequence, K/V head) and a split of the keys in tiles of 64.  A warp owns 32 rows (16
-// where a head dimension is above 64): scores, softmax and P stay in its registers, since the lane that holds two
-// adjacent scores of a row may call them any two columns of the next product as long as V's rows follow.  K of the next
-// tile is fetched (cp.async) under the softmax and P.V of this one, V under the scores of the next.
+// where a head dimension is above 64); P goes through its own part of shared memory, so that both products are rolled loops:
+// fully unrolled they spent a third of the time waiting for instructions.  K of the next tile is fetched (cp.async) under the softmax and P.V of this one, V under the scores of the next.
 #include "attention_tree.cuh"
 
 namespace sfb {
@@ -28,11 +27,29 @@ __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
+// Four column tiles of all row tiles; the three products of one accumulator are 4 * M instructions apart, since each waits
+// for the one before (back to back they took twice the time).
+template <int M, class Acc>
+__device__ __forceinline__ void multiply(Acc acc, const uint32_t (&ah)[M][4], const uint32_t (&al)[M][4], const uint32_t (&bh)[4][2],
+                                         const uint32_t (&bl)[4][2]) {
+#pragma unroll
+    for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int t = 0; t < M; ++t) {
+                if (kind == 0) mma_tf32(acc(t, n), al[t], bh[n][0], bh[n][1]);
+                else if (kind == 1) mma_tf32(acc(t, n), ah[t], bl[n][0], bl[n][1]);
+                else mma_tf32(acc(t, n), ah[t], bh[n][0], bh[n][1]);
+            }
+}
+
 __host__ __device__ inline int k_stride(int dim) { return dim + 4; }                      // an odd multiple of 4: rows on different banks
-__host__ __device__ inline int v_stride(int dim_v) { return (dim_v + 15) / 16 * 16 + 4; }  // 4 mod 16: pairs of rows on different banks
+__host__ __device__ inline int v_stride(int dim_v) { return (dim_v + 31) / 32 * 32 + 8; }  // 8 mod 32: four rows on different banks
+constexpr int kPStride = BN + 4;
 
 size_t smem_bytes(int dim, int dim_v, int nodes) {
-    return sizeof(float) * (static_cast<size_t>(BM + BN) * k_stride(dim) + static_cast<size_t>(BN) * v_stride(dim_v)) +
+    return sizeof(float) * (static_cast<size_t>(BM + BN) * k_stride(dim) + static_cast<size_t>(BN) * v_stride(dim_v) + static_cast<size_t>(BM) * kPStride) +
            4 * sizeof(void*) * BN + sizeof(uint32_t) * 9 * nodes;
 }
 
@@ -47,12 +64,14 @@ __global__ void __launch_bounds__(Tile<WIDE>::kThreads)
 tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     constexpr int M = Tile<WIDE>::kM, kThreads = Tile<WIDE>::kThreads, kNT = BN / 8;
     extern __shared__ float4 tree_smem_raw[];
+    __shared__ int missing[2];   // the tile has keys without a block
     const PagedView& kv = p.kv;
     const int sk = k_stride(kv.dim), sv = v_stride(kv.dim_v);
     float* qs = reinterpret_cast<float*>(tree_smem_raw);   // [BM][sk]
     float* ks = qs + BM * sk;                              // [BN][sk]
     float* vs = ks + BN * sk;                              // [BN][sv]
-    const float** k_rows = reinterpret_cast<const float**>(vs + BN * sv);   // [2][BN] rows of this and the next tile, nullptr: masked
+    float* ps = vs + BN * sv;                              // [BM][kPStride]
+    const float** k_rows = reinterpret_cast<const float**>(ps + BM * kPStride);   // [2][BN] rows of this and the next tile, nullptr: masked
     const float** v_rows = k_rows + 2 * BN;
     uint32_t* seen = reinterpret_cast<uint32_t*>(v_rows + 2 * BN);          // [nodes][8]
     int* parent = reinterpret_cast<int*>(seen + 8 * p.nodes);
@@ -77,7 +96,8 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
             const float *kr = nullptr, *vr = nullptr;
             if (key < min(k1, ctx)) {
                 const int64_t at = kv.row(b, kvh, key);
-                if (at >= 0) {
+                if (at < 0) missing[buffer] = 1;
+                else {
                     kr = static_cast<const float*>(kv.k_pool) + at * kv.dim;
                     vr = static_cast<const float*>(kv.v_pool) + at * kv.dim_v;
                 }
@@ -101,6 +121,8 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     };
     const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     const auto wait_but_one = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
+    if (threadIdx.x < 2) missing[threadIdx.x] = 0;
+    __syncthreads();
     if (k0 < k1) {
         find_rows(k0, 0);
         __syncthreads();
@@ -131,6 +153,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
 #pragma unroll
         for (int n = 0; n < WIDE; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.0F;
     const bool busy = warp_row < rows_all;   // the warp has rows
+    float* my_p = ps + warp * 16 * M * kPStride;
     const int nv = kv.dim_v / 8;
     int buffer = 0;
     for (int t0 = k0; t0 < k1; t0 += BN, buffer ^= 1) {
@@ -144,7 +167,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
             for (int t = 0; t < M; ++t)
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.0F;
-#pragma unroll 2
+#pragma unroll 1
             for (int d = 0; d < kv.dim; d += 8) {
                 uint32_t ah[M][4], al[M][4];
 #pragma unroll
@@ -156,17 +179,15 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
                     split(qa[8 * sk + 4], ah[t][3], al[t][3]);
                 }
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) {
-                    const float* ka = ks + (8 * n + r4) * sk + d + quad;
-                    uint32_t bh0, bl0, bh1, bl1;
-                    split(ka[0], bh0, bl0);
-                    split(ka[4], bh1, bl1);
+                for (int n0 = 0; n0 < kNT; n0 += 4) {
+                    uint32_t bh[4][2], bl[4][2];
 #pragma unroll
-                    for (int t = 0; t < M; ++t) {
-                        mma_tf32(s[t][n], al[t], bh0, bh1);
-                        mma_tf32(s[t][n], ah[t], bl0, bl1);
-                        mma_tf32(s[t][n], ah[t], bh0, bh1);
+                    for (int n = 0; n < 4; ++n) {
+                        const float* ka = ks + (8 * (n0 + n) + r4) * sk + d + quad;
+                        split(ka[0], bh[n][0], bl[n][0]);
+                        split(ka[4], bh[n][1], bl[n][1]);
                     }
+                    multiply<M>([&](int t, int n) -> float (&)[4] { return s[t][n0 + n]; }, ah, al, bh, bl);
                 }
             }
             if (t0 + BN > ctx || t0 + BN > k1) {
@@ -181,13 +202,15 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
                                 s[i >> 1][n][2 * (i & 1) + e] = -INFINITY;
                     }
             }
+            if (missing[buffer]) {
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
+                for (int n = 0; n < kNT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (!k_rows[buffer * BN + 8 * n + 2 * quad + e])
+                    for (int e = 0; e < 2; ++e)
+                        if (!k_rows[buffer * BN + 8 * n + 2 * quad + e])
 #pragma unroll
-                        for (int i = 0; i < 2 * M; ++i) s[i >> 1][n][2 * (i & 1) + e] = -INFINITY;
+                            for (int i = 0; i < 2 * M; ++i) s[i >> 1][n][2 * (i & 1) + e] = -INFINITY;
+            }
         }
         __syncthreads();
         if (more) fetch(ks, sk, kv.dim, k_rows + (buffer ^ 1) * BN);
@@ -201,48 +224,47 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 top = fmaxf(top, m[i]);
-                const float alpha = top == -INFINITY ? 1.0F : exp2f(m[i] - top);
+                const float base = top == -INFINITY ? 0.0F : top;     // (2^-inf = 0 for masked keys)
+                const float alpha = exp2_fast(m[i] - base);
                 m[i] = top;
                 l[i] *= alpha;
 #pragma unroll
                 for (int n = 0; n < WIDE; ++n) { o[i >> 1][n][2 * (i & 1)] *= alpha; o[i >> 1][n][2 * (i & 1) + 1] *= alpha; }
 #pragma unroll
-                for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[i >> 1][n][2 * (i & 1) + e];
-                        x = x == -INFINITY ? 0.0F : exp2f(x - top);
-                        l[i] += x;   // this lane's share of the row sum
-                    }
+                for (int n = 0; n < kNT; ++n) {
+                    float2 e;
+                    e.x = exp2_fast(s[i >> 1][n][2 * (i & 1)] - base);
+                    e.y = exp2_fast(s[i >> 1][n][2 * (i & 1) + 1] - base);
+                    l[i] += e.x + e.y;   // this lane's share of the row sum
+                    *reinterpret_cast<float2*>(my_p + (16 * (i >> 1) + 8 * (i & 1) + r4) * kPStride + 8 * n + 2 * quad) = e;
+                }
             }
         }
         wait_but_one();      // V
         __syncthreads();
         if (busy) {
-            // column c < 4 of a step of eight keys is key 2c, column c + 4 is key 2c + 1
-#pragma unroll
-            for (int k = 0; k < kNT; ++k) {
+#pragma unroll 1
+            for (int k = 0; k < BN; k += 8) {
                 uint32_t ah[M][4], al[M][4];
 #pragma unroll
                 for (int t = 0; t < M; ++t) {
-                    split(s[t][k][0], ah[t][0], al[t][0]);
-                    split(s[t][k][2], ah[t][1], al[t][1]);
-                    split(s[t][k][1], ah[t][2], al[t][2]);
-                    split(s[t][k][3], ah[t][3], al[t][3]);
+                    const float* pa = my_p + (16 * t + r4) * kPStride + k + quad;
+                    split(pa[0], ah[t][0], al[t][0]);
+                    split(pa[8 * kPStride], ah[t][1], al[t][1]);
+                    split(pa[4], ah[t][2], al[t][2]);
+                    split(pa[8 * kPStride + 4], ah[t][3], al[t][3]);
                 }
 #pragma unroll
-                for (int n = 0; n < WIDE; ++n) {
-                    if (n >= nv) continue;
-                    const float* va = vs + (8 * k + 2 * quad) * sv + 8 * n + r4;
-                    uint32_t bh0, bl0, bh1, bl1;
-                    split(va[0], bh0, bl0);
-                    split(va[sv], bh1, bl1);
+                for (int n0 = 0; n0 < WIDE; n0 += 4) {
+                    if (n0 >= nv) continue;      // (columns of V's rows past dim_v feed outputs that are not stored)
+                    uint32_t bh[4][2], bl[4][2];
 #pragma unroll
-                    for (int t = 0; t < M; ++t) {
-                        mma_tf32(o[t][n], al[t], bh0, bh1);
-                        mma_tf32(o[t][n], ah[t], bl0, bl1);
-                        mma_tf32(o[t][n], ah[t], bh0, bh1);
+                    for (int n = 0; n < 4; ++n) {
+                        const float* va = vs + (k + quad) * sv + (n0 + n < nv ? 8 * (n0 + n) : 0) + r4;
+                        split(va[0], bh[n][0], bl[n][0]);
+                        split(va[4 * sv], bh[n][1], bl[n][1]);
                     }
+                    multiply<M>([&](int t, int n) -> float (&)[4] { return o[t][n0 + n]; }, ah, al, bh, bl);
                 }
             }
         }
