@@ -1002,6 +1002,31 @@ sfb_status sfb_paged_gather(sfb_paged_kv* cache, float* keys, float* values);
 sfb_status sfb_paged_decode(sfb_paged_kv* cache, const sfb_attention_config* config,
                             const float* q, float* out, double* milliseconds);
 
+/* Host forms of the serving operators on the same cache (no counterpart in the reference; one length for the batch).
+ * sfb_paged_decode_tree: attention of config.sequence_query drafted tokens per sequence (parents [batch, nodes], each -1 or
+ *   a smaller node) over the cache, whose length may be 0; q [B,Hq,nodes,D], draft keys/values [B,Hkv,nodes,D | Dv], out
+ *   [B,Hq,nodes,Dv].  The drafted tokens do not enter the cache.
+ * sfb_paged_accept: appends the nodes path[b, 0 .. tokens) of the same drafted keys/values.
+ * sfb_paged_decode_sparse: one query token per sequence over budget_pages pages (sink, recent and best-scored ones);
+ *   selected (may be NULL) receives [batch, kv_heads, budget_pages].  The pages' key bounds are kept with the cache and
+ *   brought up to date by the call.
+ * sfb_paged_decode_tracked: sfb_paged_decode for one query token that adds the attention weights to the cache's running
+ *   sums; tracking starts with the first call (weights 0, text positions 0, 1, ...), later appends continue the positions.
+ * sfb_paged_weights: the sums and text positions, [batch, kv_heads, length] each.
+ * sfb_paged_evict: cuts the cache to `budget` positions by those sums (a shorter cache stays as it is) and returns the
+ *   freed pages; slots are no longer in text order afterwards, so sfb_paged_truncate drops slots, not the newest text. */
+sfb_status sfb_paged_decode_tree(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q,
+                                 const float* draft_keys, const float* draft_values, const int* parents, float* out,
+                                 double* milliseconds);
+sfb_status sfb_paged_accept(sfb_paged_kv* cache, const float* draft_keys, const float* draft_values, int nodes,
+                            const int* path, int tokens);
+sfb_status sfb_paged_decode_sparse(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q, int budget_pages,
+                                   int sink_pages, int recent_pages, float* out, int* selected, double* milliseconds);
+sfb_status sfb_paged_decode_tracked(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q, float* out,
+                                    double* milliseconds);
+sfb_status sfb_paged_weights(sfb_paged_kv* cache, float* weights, int* positions);
+sfb_status sfb_paged_evict(sfb_paged_kv* cache, int budget, int sink_tokens, int recent_tokens);
+
 /* MoeConfig, include/schedforge/moe_compiler.h:71-77. */
 typedef struct sfb_moe_config {
     int tokens, hidden, intermediate, experts, top_k;

@@ -328,6 +328,54 @@ class PagedKVCache:
         L.check(L.load().sfb_paged_decode(self._h, C.byref(config), _fp(q), _fp(out), C.byref(ms)))
         return out, ms.value
 
+    def decode_tree(self, config, q, draft_keys, draft_values, parents):
+        """Attention of config.sequence_query drafted tokens (parents [B, nodes]) over the cache: (out, ms)."""
+        q, draft_keys, draft_values, parents = _f32(q), _f32(draft_keys), _f32(draft_values), _i32(parents)
+        if parents.shape != (config.batch, config.sequence_query):
+            raise ValueError("parents: one per sequence and node")
+        out = np.empty((config.batch, config.query_heads, config.sequence_query, config.head_dim_value), np.float32)
+        ms = C.c_double(0)
+        L.check(L.load().sfb_paged_decode_tree(self._h, C.byref(config), _fp(q), _fp(draft_keys), _fp(draft_values),
+                                               _ip(parents), _fp(out), C.byref(ms)))
+        return out, ms.value
+
+    def accept(self, draft_keys, draft_values, path):
+        """Appends the nodes of `path` [B, tokens] of the drafted keys/values [B, Hkv, nodes, D | Dv]."""
+        draft_keys, draft_values, path = _f32(draft_keys), _f32(draft_values), _i32(path)
+        if path.ndim != 2 or path.shape[0] != self.shape[0]:
+            raise ValueError("path: one row per sequence")
+        L.check(L.load().sfb_paged_accept(self._h, _fp(draft_keys), _fp(draft_values), draft_keys.shape[2], _ip(path),
+                                          path.shape[1]))
+
+    def decode_sparse(self, config, q, budget_pages, sink_pages=1, recent_pages=1):
+        """One query token per sequence over the pages that matter to it: (out, selected pages, ms)."""
+        q = _f32(q)
+        out = np.empty((config.batch, config.query_heads, config.sequence_query, config.head_dim_value), np.float32)
+        selected = np.empty((config.batch, config.kv_heads, max(int(budget_pages), 0)), np.int32)
+        ms = C.c_double(0)
+        L.check(L.load().sfb_paged_decode_sparse(self._h, C.byref(config), _fp(q), int(budget_pages), int(sink_pages),
+                                                 int(recent_pages), _fp(out), _ip(selected), C.byref(ms)))
+        return out, selected, ms.value
+
+    def decode_tracked(self, config, q):
+        """decode() for one query token that adds its attention weights to the cache's running sums."""
+        q = _f32(q)
+        out = np.empty((config.batch, config.query_heads, config.sequence_query, config.head_dim_value), np.float32)
+        ms = C.c_double(0)
+        L.check(L.load().sfb_paged_decode_tracked(self._h, C.byref(config), _fp(q), _fp(out), C.byref(ms)))
+        return out, ms.value
+
+    def weights(self):
+        """(accumulated weights, text positions), [B, Hkv, length] each."""
+        shape = (self.shape[0], self.shape[1], self.info()["length"])
+        weights, positions = np.zeros(shape, np.float32), np.zeros(shape, np.int32)
+        L.check(L.load().sfb_paged_weights(self._h, _fp(weights), _ip(positions)))
+        return weights, positions
+
+    def evict(self, budget, sink_tokens=0, recent_tokens=0):
+        """Cuts the cache to `budget` positions by the accumulated weights."""
+        L.check(L.load().sfb_paged_evict(self._h, int(budget), int(sink_tokens), int(recent_tokens)))
+
     def close(self):
         if self._h:
             L.load().sfb_paged_destroy(self._h)

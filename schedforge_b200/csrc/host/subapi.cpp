@@ -83,7 +83,47 @@ struct sfb_paged_kv {
     int length = 0;
     std::vector<int> page_table, free_pages;
     DeviceBuffer k_pool, v_pool, table, lens;
+    // key bounds of the pages (sfb_paged_decode_sparse), up to date for the first bounds_length positions
+    DeviceBuffer bounds;
+    int bounds_length = 0;
+    // accumulated attention weights and text positions, [batch, kv_heads, capacity] (sfb_paged_decode_tracked)
+    DeviceBuffer weights, positions;
+    bool tracked = false, evicted = false;
+    int next_position = 0;
     int pages() const { return (capacity + page_tokens - 1) / page_tokens; }
+    // pages for `tokens` more positions, from the back of the free list
+    void reserve(int tokens) {
+        if (tokens <= 0 || length + tokens > capacity) throw std::invalid_argument("paged KV capacity exceeded");
+        const int last_page = (length + tokens - 1) / page_tokens;
+        while (static_cast<int>(page_table.size()) <= last_page) {
+            if (free_pages.empty()) throw std::runtime_error("paged KV page allocator exhausted");
+            page_table.push_back(free_pages.back());
+            free_pages.pop_back();
+        }
+    }
+    void shorten(int new_length) {
+        const int keep = new_length == 0 ? 0 : (new_length + page_tokens - 1) / page_tokens;
+        while (static_cast<int>(page_table.size()) > keep) {
+            free_pages.push_back(page_table.back());
+            page_table.pop_back();
+        }
+        length = new_length;
+        // the bounds of the last block may cover positions that are gone
+        bounds_length = std::min(bounds_length, new_length / page_tokens * page_tokens);
+        if (tracked && !evicted) next_position = new_length;
+    }
+    // slots [first, first + tokens): no weight yet, text positions from next_position on
+    void stamp(int first, int tokens, cudaStream_t s) {
+        const size_t pitch = static_cast<size_t>(capacity) * 4, rows = static_cast<size_t>(batch) * kv_heads;
+        std::vector<int> host(rows * tokens);
+        for (size_t r = 0; r < rows; ++r)
+            for (int t = 0; t < tokens; ++t) host[r * tokens + t] = next_position + t;
+        cuda_check(cudaMemset2DAsync(weights.as<float>() + first, pitch, 0, static_cast<size_t>(tokens) * 4, rows, s), "weight clear");
+        cuda_check(cudaMemcpy2DAsync(positions.as<int>() + first, pitch, host.data(), static_cast<size_t>(tokens) * 4,
+                                     static_cast<size_t>(tokens) * 4, rows, cudaMemcpyHostToDevice, s), "position upload");
+        cuda_check(cudaStreamSynchronize(s), "position sync");
+        next_position += tokens;
+    }
     void sync_table(cudaStream_t s, int start_length) {
         const int max_blocks = pages();
         std::vector<int> host(static_cast<size_t>(batch) * max_blocks, 0), len(batch, start_length);
@@ -181,12 +221,7 @@ sfb_status sfb_paged_append(sfb_paged_kv* cache, const float* keys, const float*
         auto& c = *cache;
         if (tokens <= 0 || c.length + tokens > c.capacity) throw std::invalid_argument("paged KV capacity exceeded");
         if (!keys || !values) throw std::invalid_argument("paged KV append shape mismatch");
-        const int last_page = (c.length + tokens - 1) / c.page_tokens;
-        while (static_cast<int>(c.page_table.size()) <= last_page) {
-            if (c.free_pages.empty()) throw std::runtime_error("paged KV page allocator exhausted");
-            c.page_table.push_back(c.free_pages.back());
-            c.free_pages.pop_back();
-        }
+        c.reserve(tokens);
         cudaStream_t s = nullptr;
         c.sync_table(s, c.length);
         const size_t rows = static_cast<size_t>(c.batch) * c.kv_heads * tokens;
@@ -195,6 +230,7 @@ sfb_status sfb_paged_append(sfb_paged_kv* cache, const float* keys, const float*
                                        c.lens.as<int>(), c.batch, c.kv_heads, tokens, c.dim, c.dim_v, c.page_tokens,
                                        c.pages(), c.pages() * c.batch, static_cast<sfb_dtype>(c.dtype), s));
         cuda_check(cudaStreamSynchronize(s), "append sync");
+        if (c.tracked) c.stamp(c.length, tokens, s);
         c.length += tokens;
     });
 }
@@ -204,12 +240,7 @@ sfb_status sfb_paged_truncate(sfb_paged_kv* cache, int new_length) {
         if (!cache) throw std::invalid_argument("null paged KV cache");
         auto& c = *cache;
         if (new_length < 0 || new_length > c.length) throw std::invalid_argument("invalid paged KV truncation length");
-        const int keep = new_length == 0 ? 0 : (new_length + c.page_tokens - 1) / c.page_tokens;
-        while (static_cast<int>(c.page_table.size()) > keep) {
-            c.free_pages.push_back(c.page_table.back());
-            c.page_table.pop_back();
-        }
-        c.length = new_length;
+        c.shorten(new_length);
     });
 }
 
@@ -310,6 +341,220 @@ sfb_status sfb_paged_decode(sfb_paged_kv* cache, const sfb_attention_config* con
             if (milliseconds) *milliseconds = ms;
         }
         fetch(dout.get(), no, c.dtype, out, s);
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// The guards of sfb_paged_decode for a call with `queries` query tokens per sequence.
+void check_paged_call(const sfb_paged_kv* cache, const sfb_attention_config* config, int least_length, bool one_query) {
+    if (!cache || !config) throw std::invalid_argument("paged attention query shape mismatch");
+    const auto& c = *cache;
+    const auto& a = *config;
+    if (c.length < least_length || c.length > a.sequence_kv) throw std::invalid_argument("paged KV length violates compiled guard");
+    if (c.batch != a.batch || c.kv_heads != a.kv_heads || c.dim != a.head_dim || c.dim_v != a.head_dim_value)
+        throw std::invalid_argument("paged KV shape violates compiled guard");
+    if (a.query_heads <= 0 || a.query_heads % a.kv_heads != 0 || a.sequence_query <= 0)
+        throw std::invalid_argument("invalid grouped-query attention configuration");
+    if (one_query && a.sequence_query != 1) throw std::invalid_argument("decode attention expects one query token per sequence");
+    if (static_cast<int>(c.page_table.size()) < (c.length + c.page_tokens - 1) / c.page_tokens)
+        throw std::invalid_argument("paged KV page table is incomplete");
+}
+
+template <class Args>
+void fill_cache(Args& d, const sfb_paged_kv& c) {
+    d.k_pool = c.k_pool.get(); d.v_pool = c.v_pool.get(); d.block_table = c.table.as<int>();
+    d.batch = c.batch; d.kv_heads = c.kv_heads; d.head_dim = c.dim; d.head_dim_value = c.dim_v;
+    d.block_tokens = c.page_tokens; d.max_blocks = c.pages(); d.num_blocks = c.pages() * c.batch; d.dtype = c.dtype;
+}
+
+}  // namespace
+
+extern "C" {
+
+sfb_status sfb_paged_decode_tree(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q, const float* draft_keys,
+                                 const float* draft_values, const int* parents, float* out, double* milliseconds) {
+    return guarded([&] {
+        if (!q || !draft_keys || !draft_values || !parents || !out) throw std::invalid_argument("paged attention query shape mismatch");
+        check_paged_call(cache, config, 0, false);
+        auto& c = *cache;
+        const auto& a = *config;
+        const int nodes = a.sequence_query;
+        for (int b = 0; b < a.batch; ++b)
+            for (int i = 0; i < nodes; ++i)
+                if (parents[b * nodes + i] < -1 || parents[b * nodes + i] >= i)
+                    throw std::invalid_argument("a tree node's parent has to come before it");
+        cudaStream_t s = nullptr;
+        c.sync_table(s, c.length);
+        const size_t rows = static_cast<size_t>(a.batch) * nodes;
+        Staged dq(q, rows * a.query_heads * c.dim, c.dtype, s), dk(draft_keys, rows * c.kv_heads * c.dim, c.dtype, s),
+            dv(draft_values, rows * c.kv_heads * c.dim_v, c.dtype, s), dout(nullptr, rows * a.query_heads * c.dim_v, c.dtype, s);
+        DeviceBuffer tree(rows * 4);
+        cuda_check(cudaMemcpyAsync(tree.get(), parents, rows * 4, cudaMemcpyHostToDevice, s), "upload");
+        sfb_tree_args d{};
+        fill_cache(d, c);
+        d.q = dq.get(); d.context_len = c.lens.as<int>(); d.draft_k = dk.get(); d.draft_v = dv.get(); d.parents = tree.as<int>();
+        d.out = dout.get(); d.q_heads = a.query_heads; d.nodes = nodes; d.max_context = c.length; d.scale = a.scale;
+        DeviceBuffer workspace(std::max<size_t>(sfb_attention_tree_workspace(&d), 16));
+        d.workspace = workspace.get();
+        Timer timer;
+        timer.start(s);
+        throw_on(sfb_k_attention_tree_paged(&d, s));
+        const double ms = timer.stop(s);
+        if (milliseconds) *milliseconds = ms;
+        fetch(dout.get(), rows * a.query_heads * c.dim_v, c.dtype, out, s);
+    });
+}
+
+sfb_status sfb_paged_accept(sfb_paged_kv* cache, const float* draft_keys, const float* draft_values, int nodes, const int* path,
+                            int tokens) {
+    return guarded([&] {
+        if (!cache) throw std::invalid_argument("null paged KV cache");
+        auto& c = *cache;
+        if (tokens <= 0 || c.length + tokens > c.capacity) throw std::invalid_argument("paged KV capacity exceeded");
+        if (!draft_keys || !draft_values || !path || nodes <= 0) throw std::invalid_argument("paged KV append shape mismatch");
+        for (int i = 0; i < c.batch * tokens; ++i)
+            if (path[i] < 0 || path[i] >= nodes) throw std::invalid_argument("accepted path names a node that is not in the tree");
+        c.reserve(tokens);
+        cudaStream_t s = nullptr;
+        c.sync_table(s, c.length);
+        const size_t rows = static_cast<size_t>(c.batch) * c.kv_heads * nodes;
+        Staged dk(draft_keys, rows * c.dim, c.dtype, s), dv(draft_values, rows * c.dim_v, c.dtype, s);
+        const std::vector<int> count(c.batch, tokens);
+        DeviceBuffer steps(static_cast<size_t>(c.batch) * tokens * 4), counts(static_cast<size_t>(c.batch) * 4);
+        cuda_check(cudaMemcpyAsync(steps.get(), path, static_cast<size_t>(c.batch) * tokens * 4, cudaMemcpyHostToDevice, s), "upload");
+        cuda_check(cudaMemcpyAsync(counts.get(), count.data(), count.size() * 4, cudaMemcpyHostToDevice, s), "upload");
+        sfb_accept_args d{};
+        d.draft_k = dk.get(); d.draft_v = dv.get(); d.k_pool = c.k_pool.get(); d.v_pool = c.v_pool.get();
+        d.block_table = c.table.as<int>(); d.start_len = c.lens.as<int>(); d.path = steps.as<int>(); d.path_len = counts.as<int>();
+        d.batch = c.batch; d.kv_heads = c.kv_heads; d.nodes = nodes; d.max_path = tokens; d.head_dim = c.dim; d.head_dim_value = c.dim_v;
+        d.block_tokens = c.page_tokens; d.max_blocks = c.pages(); d.num_blocks = c.pages() * c.batch; d.dtype = c.dtype;
+        throw_on(sfb_k_paged_kv_accept(&d, s));
+        cuda_check(cudaStreamSynchronize(s), "append sync");
+        if (c.tracked) c.stamp(c.length, tokens, s);
+        c.length += tokens;
+    });
+}
+
+sfb_status sfb_paged_decode_sparse(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q, int budget_pages,
+                                   int sink_pages, int recent_pages, float* out, int* selected, double* milliseconds) {
+    return guarded([&] {
+        if (!q || !out) throw std::invalid_argument("paged attention query shape mismatch");
+        check_paged_call(cache, config, 1, true);
+        auto& c = *cache;
+        const auto& a = *config;
+        if (budget_pages <= 0 || sink_pages < 0 || recent_pages < 0 || static_cast<int64_t>(sink_pages) + recent_pages > budget_pages)
+            throw std::invalid_argument("sparse decode: the sink and recent blocks have to fit into the budget");
+        cudaStream_t s = nullptr;
+        c.sync_table(s, c.length);
+        if (!c.bounds.get()) c.bounds.allocate(static_cast<size_t>(c.pages()) * c.batch * c.kv_heads * 2 * c.dim * dtype_size(c.dtype));
+        DeviceBuffer start(static_cast<size_t>(c.batch) * 4);
+        if (c.bounds_length < c.length) {
+            const std::vector<int> from(c.batch, c.bounds_length);
+            cuda_check(cudaMemcpyAsync(start.get(), from.data(), from.size() * 4, cudaMemcpyHostToDevice, s), "upload");
+            cuda_check(cudaStreamSynchronize(s), "upload sync");
+            sfb_bounds_args u{};
+            u.k_pool = c.k_pool.get(); u.bounds = c.bounds.get(); u.block_table = c.table.as<int>();
+            u.start_len = start.as<int>(); u.end_len = c.lens.as<int>();
+            u.batch = c.batch; u.kv_heads = c.kv_heads; u.head_dim = c.dim; u.max_tokens = c.length - c.bounds_length;
+            u.block_tokens = c.page_tokens; u.max_blocks = c.pages(); u.num_blocks = c.pages() * c.batch; u.dtype = c.dtype;
+            throw_on(sfb_k_paged_kv_bounds(&u, s));
+            c.bounds_length = c.length;
+        }
+        const size_t rows = static_cast<size_t>(a.batch) * a.query_heads, chosen = static_cast<size_t>(a.batch) * c.kv_heads * budget_pages;
+        Staged dq(q, rows * c.dim, c.dtype, s), dout(nullptr, rows * c.dim_v, c.dtype, s);
+        DeviceBuffer list(chosen * 4);
+        sfb_sparse_args d{};
+        fill_cache(d, c);
+        d.q = dq.get(); d.bounds = c.bounds.get(); d.context_len = c.lens.as<int>(); d.out = dout.get(); d.selected = list.as<int>();
+        d.q_heads = a.query_heads; d.max_context = c.length; d.budget_blocks = budget_pages; d.sink_blocks = sink_pages;
+        d.recent_blocks = recent_pages; d.scale = a.scale;
+        DeviceBuffer workspace(std::max<size_t>(sfb_attention_sparse_workspace(&d), 16));
+        d.workspace = workspace.get();
+        Timer timer;
+        timer.start(s);
+        throw_on(sfb_k_attention_decode_sparse(&d, s));
+        const double ms = timer.stop(s);
+        if (milliseconds) *milliseconds = ms;
+        if (selected) cuda_check(cudaMemcpyAsync(selected, list.get(), chosen * 4, cudaMemcpyDeviceToHost, s), "download");
+        fetch(dout.get(), rows * c.dim_v, c.dtype, out, s);
+    });
+}
+
+sfb_status sfb_paged_decode_tracked(sfb_paged_kv* cache, const sfb_attention_config* config, const float* q, float* out,
+                                    double* milliseconds) {
+    return guarded([&] {
+        if (!q || !out) throw std::invalid_argument("paged attention query shape mismatch");
+        check_paged_call(cache, config, 1, true);
+        auto& c = *cache;
+        const auto& a = *config;
+        cudaStream_t s = nullptr;
+        c.sync_table(s, c.length);
+        if (!c.tracked) {   // from here on every position has a weight and a text position
+            const size_t entries = static_cast<size_t>(c.batch) * c.kv_heads * c.capacity;
+            c.weights.allocate(entries * 4);
+            c.positions.allocate(entries * 4);
+            c.next_position = 0;
+            c.stamp(0, c.length, s);
+            c.tracked = true;
+        }
+        const size_t rows = static_cast<size_t>(a.batch) * a.query_heads;
+        Staged dq(q, rows * c.dim, c.dtype, s), dout(nullptr, rows * c.dim_v, c.dtype, s);
+        sfb_weights_args d{};
+        fill_cache(d, c);
+        d.q = dq.get(); d.context_len = c.lens.as<int>(); d.out = dout.get();
+        d.weights = d.weights_out = c.weights.as<float>();
+        d.q_heads = a.query_heads; d.max_context = c.length; d.weight_stride = c.capacity; d.scale = a.scale;
+        DeviceBuffer workspace(std::max<size_t>(sfb_attention_weights_workspace(&d), 16));
+        d.workspace = workspace.get();
+        Timer timer;
+        timer.start(s);
+        throw_on(sfb_k_attention_decode_weights(&d, s));
+        const double ms = timer.stop(s);
+        if (milliseconds) *milliseconds = ms;
+        fetch(dout.get(), rows * c.dim_v, c.dtype, out, s);
+    });
+}
+
+sfb_status sfb_paged_weights(sfb_paged_kv* cache, float* weights, int* positions) {
+    return guarded([&] {
+        if (!cache || !weights || !positions) throw std::invalid_argument("null paged KV cache");
+        auto& c = *cache;
+        if (!c.tracked) throw std::invalid_argument("paged KV cache has no accumulated attention weights");
+        if (c.length == 0) return;
+        const size_t width = static_cast<size_t>(c.length) * 4, pitch = static_cast<size_t>(c.capacity) * 4;
+        const size_t rows = static_cast<size_t>(c.batch) * c.kv_heads;
+        cuda_check(cudaMemcpy2D(weights, width, c.weights.get(), pitch, width, rows, cudaMemcpyDeviceToHost), "download");
+        cuda_check(cudaMemcpy2D(positions, width, c.positions.get(), pitch, width, rows, cudaMemcpyDeviceToHost), "download");
+    });
+}
+
+sfb_status sfb_paged_evict(sfb_paged_kv* cache, int budget, int sink_tokens, int recent_tokens) {
+    return guarded([&] {
+        if (!cache) throw std::invalid_argument("null paged KV cache");
+        auto& c = *cache;
+        if (!c.tracked) throw std::invalid_argument("paged KV cache has no accumulated attention weights");
+        if (budget <= 0 || sink_tokens < 0 || recent_tokens < 0 || static_cast<int64_t>(sink_tokens) + recent_tokens > budget)
+            throw std::invalid_argument("evict: the sink and recent tokens have to fit into the budget");
+        if (c.length <= budget) return;
+        cudaStream_t s = nullptr;
+        c.sync_table(s, c.length);
+        DeviceBuffer new_len(static_cast<size_t>(c.batch) * 4);
+        sfb_evict_args d{};
+        fill_cache(d, c);
+        d.context_len = c.lens.as<int>(); d.new_len = new_len.as<int>();
+        d.weights = d.weights_out = c.weights.as<float>();
+        d.positions = d.positions_out = c.positions.as<int>();
+        d.max_context = c.length; d.weight_stride = c.capacity; d.budget = budget; d.sink_tokens = sink_tokens; d.recent_tokens = recent_tokens;
+        DeviceBuffer workspace(std::max<size_t>(sfb_paged_kv_evict_workspace(&d), 16));
+        d.workspace = workspace.get();
+        throw_on(sfb_k_paged_kv_evict(&d, s));
+        cuda_check(cudaStreamSynchronize(s), "evict sync");
+        c.evicted = true;
+        c.bounds_length = 0;      // rows moved into earlier pages
+        c.shorten(budget);
     });
 }
 
