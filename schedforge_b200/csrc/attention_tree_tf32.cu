@@ -21,27 +21,71 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The instruction reads the upper 19 bits of a register.
+// hi is x rounded to 11 bits, so that of the 12 bits and the sign of lo the instruction, which reads the upper 19 bits
+// of a register, drops one at most.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-    hi = __float_as_uint(x) & 0xffffe000u;
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-// Four column tiles of all row tiles; the three products of one accumulator are 4 * M instructions apart, since each waits
-// for the one before (back to back they took twice the time).
-template <int M, class Acc>
-__device__ __forceinline__ void multiply(Acc acc, const uint32_t (&ah)[M][4], const uint32_t (&al)[M][4], const uint32_t (&bh)[4][2],
-                                         const uint32_t (&bl)[4][2]) {
+// acc(t, n) += the products of four column tiles n and all row tiles t over `steps` steps of eight, operands from
+// a(step, t, hi, lo) and b(step, n, hi, lo).  The instruction truncates its sums, so the large products run at most DEPTH
+// steps in an accumulator of their own before a rounded addition takes them over, and the small ones, which have 11 bits to
+// spare, meet them at the end.  (All three products in one accumulator running on over the tiles: 2.6e-6 off at logits of ten.)
+// Products of one accumulator are at least 4 * M instructions apart, since each waits for the one before.
+template <int M, int DEPTH, class Acc, class A, class B>
+__device__ __forceinline__ void multiply(Acc acc, int steps, A a, B b) {
+    float small[M][4][4];
 #pragma unroll
-    for (int kind = 0; kind < 3; ++kind)
+    for (int t = 0; t < M; ++t)
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int t = 0; t < M; ++t) {
-                if (kind == 0) mma_tf32(acc(t, n), al[t], bh[n][0], bh[n][1]);
-                else if (kind == 1) mma_tf32(acc(t, n), ah[t], bl[n][0], bl[n][1]);
-                else mma_tf32(acc(t, n), ah[t], bh[n][0], bh[n][1]);
-            }
+            for (int i = 0; i < 4; ++i) small[t][n][i] = 0.0F;
+#pragma unroll 1
+    for (int step0 = 0; step0 < steps; step0 += DEPTH) {
+        float big[M][4][4];
+#pragma unroll
+        for (int t = 0; t < M; ++t)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big[t][n][i] = 0.0F;
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+            const int step = step0 + u;
+            if (step >= steps) continue;
+            uint32_t ah[M][4], al[M][4], bh[4][2], bl[4][2];
+#pragma unroll
+            for (int t = 0; t < M; ++t) a(step, t, ah[t], al[t]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) b(step, n, bh[n], bl[n]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int t = 0; t < M; ++t) mma_tf32(small[t][n], al[t], bh[n][0], bh[n][1]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int t = 0; t < M; ++t) mma_tf32(big[t][n], ah[t], bh[n][0], bh[n][1]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int t = 0; t < M; ++t) mma_tf32(small[t][n], ah[t], bl[n][0], bl[n][1]);
+        }
+#pragma unroll
+        for (int t = 0; t < M; ++t)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc(t, n)[i] += big[t][n][i];
+    }
+#pragma unroll
+    for (int t = 0; t < M; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc(t, n)[i] += small[t][n][i];
 }
 
 __host__ __device__ inline int k_stride(int dim) { return dim + 4; }                      // an odd multiple of 4: rows on different banks
@@ -167,29 +211,21 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
             for (int t = 0; t < M; ++t)
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.0F;
-#pragma unroll 1
-            for (int d = 0; d < kv.dim; d += 8) {
-                uint32_t ah[M][4], al[M][4];
 #pragma unroll
-                for (int t = 0; t < M; ++t) {
-                    const float* qa = qs + (warp * 16 * M + 16 * t + r4) * sk + d + quad;
-                    split(qa[0], ah[t][0], al[t][0]);
-                    split(qa[8 * sk], ah[t][1], al[t][1]);
-                    split(qa[4], ah[t][2], al[t][2]);
-                    split(qa[8 * sk + 4], ah[t][3], al[t][3]);
-                }
-#pragma unroll
-                for (int n0 = 0; n0 < kNT; n0 += 4) {
-                    uint32_t bh[4][2], bl[4][2];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float* ka = ks + (8 * (n0 + n) + r4) * sk + d + quad;
-                        split(ka[0], bh[n][0], bl[n][0]);
-                        split(ka[4], bh[n][1], bl[n][1]);
-                    }
-                    multiply<M>([&](int t, int n) -> float (&)[4] { return s[t][n0 + n]; }, ah, al, bh, bl);
-                }
-            }
+            for (int n0 = 0; n0 < kNT; n0 += 4)
+                multiply<M, 1>([&](int t, int n) -> float (&)[4] { return s[t][n0 + n]; }, kv.dim / 8,
+                    [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+                        const float* qa = qs + (warp * 16 * M + 16 * t + r4) * sk + 8 * step + quad;
+                        split(qa[0], hi[0], lo[0]);
+                        split(qa[8 * sk], hi[1], lo[1]);
+                        split(qa[4], hi[2], lo[2]);
+                        split(qa[8 * sk + 4], hi[3], lo[3]);
+                    },
+                    [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+                        const float* ka = ks + (8 * (n0 + n) + r4) * sk + 8 * step + quad;
+                        split(ka[0], hi[0], lo[0]);
+                        split(ka[4], hi[1], lo[1]);
+                    });
             if (t0 + BN > ctx || t0 + BN > k1) {
 #pragma unroll
                 for (int n = 0; n < kNT; ++n)
@@ -243,29 +279,22 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
         wait_but_one();      // V
         __syncthreads();
         if (busy) {
-#pragma unroll 1
-            for (int k = 0; k < BN; k += 8) {
-                uint32_t ah[M][4], al[M][4];
 #pragma unroll
-                for (int t = 0; t < M; ++t) {
-                    const float* pa = my_p + (16 * t + r4) * kPStride + k + quad;
-                    split(pa[0], ah[t][0], al[t][0]);
-                    split(pa[8 * kPStride], ah[t][1], al[t][1]);
-                    split(pa[4], ah[t][2], al[t][2]);
-                    split(pa[8 * kPStride + 4], ah[t][3], al[t][3]);
-                }
-#pragma unroll
-                for (int n0 = 0; n0 < WIDE; n0 += 4) {
-                    if (n0 >= nv) continue;      // (columns of V's rows past dim_v feed outputs that are not stored)
-                    uint32_t bh[4][2], bl[4][2];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float* va = vs + (k + quad) * sv + (n0 + n < nv ? 8 * (n0 + n) : 0) + r4;
-                        split(va[0], bh[n][0], bl[n][0]);
-                        split(va[4 * sv], bh[n][1], bl[n][1]);
-                    }
-                    multiply<M>([&](int t, int n) -> float (&)[4] { return o[t][n0 + n]; }, ah, al, bh, bl);
-                }
+            for (int n0 = 0; n0 < WIDE; n0 += 4) {
+                if (n0 >= nv) continue;      // (columns of V's rows past dim_v feed outputs that are not stored)
+                multiply<M, 2>([&](int t, int n) -> float (&)[4] { return o[t][n0 + n]; }, BN / 8,
+                    [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+                        const float* pa = my_p + (16 * t + r4) * kPStride + 8 * step + quad;
+                        split(pa[0], hi[0], lo[0]);
+                        split(pa[8 * kPStride], hi[1], lo[1]);
+                        split(pa[4], hi[2], lo[2]);
+                        split(pa[8 * kPStride + 4], hi[3], lo[3]);
+                    },
+                    [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+                        const float* va = vs + (8 * step + quad) * sv + (n0 + n < nv ? 8 * (n0 + n) : 0) + r4;
+                        split(va[0], hi[0], lo[0]);
+                        split(va[4 * sv], hi[1], lo[1]);
+                    });
             }
         }
         __syncthreads();
