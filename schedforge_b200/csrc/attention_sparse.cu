@@ -641,20 +641,7 @@ select_kernel(const __grid_constant__ SelectParams p) {
     const PagedView& kv = p.kv;
     const int b = blockIdx.y, kvh = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependency_wait();
-    const int ctx = kv.length(b);
-    const int n = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
-    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
-    int* out = p.selected + row * p.budget;
-    const int k = min(p.budget, n);
-    if (k == n) {  // everything is kept
-        for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < n ? i : -1;
-        return;
-    }
-    extern __shared__ uint32_t keys[];
-    const float* scores = p.scores + row * p.score_stride;
-    double* exact = p.exact + row * p.score_stride;
-    const int recent_from = n - p.recent, sink = p.sink, group = p.q_heads / kv.kv_heads;
-    const auto forced = [&](int i) { return i < sink || i >= recent_from; };
+    const int ctx = kv.length(b), group = p.q_heads / kv.kv_heads;
     // the error of the 32-bit scores
     float norm = 0.0F, size = 0.0F;
     for (int g = warp; g < group; g += kSelectThreads / 32) {
@@ -666,6 +653,19 @@ select_kernel(const __grid_constant__ SelectParams p) {
         s = warp_sum(s);
         norm = s > norm || s != s ? s : norm;
     }
+    const int n = ctx > 0 ? kv.block_of(ctx - 1) + 1 : 0;
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    int* out = p.selected + row * p.budget;
+    const int k = min(p.budget, n);
+    if (k == n) {  // everything is kept
+        for (int i = threadIdx.x; i < p.budget; i += kSelectThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    extern __shared__ uint32_t keys[];
+    const float* scores = p.scores + row * p.score_stride;
+    double* exact = p.exact + row * p.score_stride;
+    const int recent_from = n - p.recent, sink = p.sink;
+    const auto forced = [&](int i) { return i < sink || i >= recent_from; };
     for (int i = threadIdx.x; i < (n + p.blocks_per_size - 1) / p.blocks_per_size; i += kSelectThreads)
         size = fmaxf(size, p.sizes[row * p.size_count + i]);
     size = warp_max(size);

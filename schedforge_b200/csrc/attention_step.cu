@@ -244,17 +244,29 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Merg
     if (p.part.span) r = row_pieces(p.part, p.kv.kv_heads, p.q_heads, b, head, p.kv.length(b));
     else r = {static_cast<size_t>(row) * p.part.splits, 1, p.part.splits};
     if (p.part.span && r.count == 1) return;   // written by the attention kernel itself
+    // the first eight pieces of each half are fetched before their factors are known
+    const int half = threadIdx.x >> 7;
+    float early[8];
+    {
+        const int d = threadIdx.x & 127;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            early[i] = half + 2 * i < r.count && d < p.dim_v ? p.part.o[(r.first + static_cast<size_t>(half + 2 * i) * r.step) * p.part.o_step + d] : 0.0F;
+    }
     if (threadIdx.x < 32) row_statistics(p.part, r, factor);
     __syncthreads();
     T* dst = static_cast<T*>(p.out) + (p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
                                                      : static_cast<size_t>(row)) * p.dim_v;
-    const int half = threadIdx.x >> 7;
     for (int d0 = 0; d0 < p.dim_v; d0 += 128) {
         const int d = d0 + (threadIdx.x & 127);
         float a = 0.0F;
+        if (d0 == 0)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (half + 2 * i < r.count && factor[half + 2 * i] != 0.0F) a = fmaf(factor[half + 2 * i], early[i], a);
         if (d < p.dim_v)
 #pragma unroll 8
-            for (int i = half; i < r.count; i += 2) {
+            for (int i = half + (d0 == 0 ? 16 : 0); i < r.count; i += 2) {
                 const float f = factor[i];
                 if (f != 0.0F) a = fmaf(f, p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + d], a);
             }

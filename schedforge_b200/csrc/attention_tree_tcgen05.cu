@@ -331,17 +331,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             for (int j = kTwoTiles ? 0 : t; ok && j < n; j += kTwoTiles ? 1 : 2, ++used) {
                 const int x = w.x + j;
                 const uint32_t g = n_kv + j;
-                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[t]), n_slot & 1, abort_flag, status, kCodeTree | 4);
-                if (!ok) break;
-                ++n_slot;
-                ptx::tc_fence_after();
                 const bool draft = x >= n_ctx;
-                const int key0 = draft ? (x - n_ctx) * KT : x * KT;
-                const int live = min(KT, (draft ? w.count : w.ctx) - key0);
-                uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-                bool masked = live < KT;
-                if (draft) {
-                    masked = true;
+                if (draft) {   // parents come in while the scores are computed
                     for (int i = r; i < w.count; i += 128) {
                         int up = t_.parents[static_cast<size_t>(w.b) * t_.nodes + i];
                         if (up < -1 || up >= i) {
@@ -351,6 +342,17 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         parent[i] = static_cast<uint8_t>(up);   // (-1 becomes 255; a parent is at most 254)
                     }
                     ptx::mbar_arrive(ptx::smem_u32(&par_full[t]));
+                }
+                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[t]), n_slot & 1, abort_flag, status, kCodeTree | 4);
+                if (!ok) break;
+                ++n_slot;
+                ptx::tc_fence_after();
+                const int key0 = draft ? (x - n_ctx) * KT : x * KT;
+                const int live = min(KT, (draft ? w.count : w.ctx) - key0);
+                uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+                bool masked = live < KT;
+                if (draft) {
+                    masked = true;
                     ok = ptx::mbar_wait(ptx::smem_u32(&par_full[t]), n_par & 1, abort_flag, status, kCodeTree | 4);
                     if (!ok) break;
                     ++n_par;

@@ -157,11 +157,11 @@ struct RowPieces {
 };
 __device__ __forceinline__ RowPieces row_pieces(const Partials& part, int kv_heads, int q_heads, int b, int head, int ctx) {
     if (!part.span) return {(static_cast<size_t>(b) * q_heads + head) * part.splits, 1, part.splits};
-    if (ctx == 0) return {0, 0, 0};
     const int group = q_heads / kv_heads, chunks = (group + kPieceHeads - 1) / kPieceHeads;
     const int in_group = head % group;
     const size_t pair = (static_cast<size_t>(b) * kv_heads + head / group) * chunks + in_group / kPieceHeads;
     const int2 span = part.span[pair];
+    if (ctx == 0) return {0, 0, 0};   // (nobody wrote the span; its load need not wait for the length)
     return {(span.x + pair) * kPieceHeads + in_group % kPieceHeads, kPieceHeads, min(span.y - span.x + 1, kMaxPieces)};
 }
 
