@@ -491,7 +491,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool whole = w.x == 0 && n == w.tiles;
             const int64_t pair = static_cast<int64_t>(w.b) * kv.kv_heads * p.row_groups + w.sub;
             if ((kTwoTiles || t == 0) && live_warp) {
-                const float inv = whole ? (row_sum > 0.0F ? 1.0F / row_sum : 0.0F) : 1.0F;
+                const float inv = whole ? (row_sum == 0.0F ? 0.0F : 1.0F / row_sum) : 1.0F;
                 f0 *= inv;
                 f1 *= inv;
                 const bool second = !kTwoTiles && n > 1;
@@ -571,26 +571,51 @@ tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
     const int b = static_cast<int>(pair / subs), sub = static_cast<int>(pair % subs);
     const int kvh = sub / p.row_groups, rg = sub % p.row_groups;
     const int row = rg * rows_cta + tile_row, node = row % t.nodes;
-    if (row >= p.rows_all || node >= tree_node_count(t, b)) return;
-    const int2 span = p.pair_span[pair];
+    if (row >= p.rows_all) return;
+    const int2 span = p.pair_span[pair];      // (not written where the sequence has no nodes; then the count is 0)
+    if (node >= tree_node_count(t, b)) return;
     if (span.x == span.y) return;   // written by the attention kernel itself
+    // up to kAtOnce pieces are read at the same time
+    constexpr int kAtOnce = 8;
+    const auto index = [&](int c) { return (c + pair) * rows_cta + tile_row; };
+    float2 ml[kAtOnce];
+    float part[kAtOnce][V];
     float top = -INFINITY;
-    for (int c = span.x; c <= span.y; ++c) top = fmaxf(top, p.part_ml[(c + pair) * rows_cta + tile_row].x);
-    float sum = 0.0F, acc[V] = {};
-    for (int c = span.x; c <= span.y; ++c) {
-        const float2 ml = p.part_ml[(c + pair) * rows_cta + tile_row];
-        if (ml.x == -INFINITY) continue;
-        const float f = exp2_fast(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
-        const float* part = p.part_o + ((c + pair) * rows_cta + tile_row) * D + lane * V;
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(part + i);
-            acc[i] = fmaf(v.x, f, acc[i]);
-            acc[i + 1] = fmaf(v.y, f, acc[i + 1]);
+    for (int i = 0; i < kAtOnce; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.0F);
+        if (span.x + i > span.y) continue;
+        ml[i] = p.part_ml[index(span.x + i)];
+        const float* at = p.part_o + index(span.x + i) * D + lane * V;
+#pragma unroll
+        for (int k = 0; k < V; k += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(at + k);
+            part[i][k] = v.x;
+            part[i][k + 1] = v.y;
         }
     }
-    const float inv = sum > 0.0F ? 1.0F / sum : 0.0F;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
+    for (int c = span.x + kAtOnce; c <= span.y; ++c) top = fmaxf(top, p.part_ml[index(c)].x);
+    float sum = 0.0F, acc[V] = {};
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+        if (ml[i].x == -INFINITY) continue;
+        const float f = exp2_fast(ml[i].x - top);
+        sum = fmaf(ml[i].y, f, sum);
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = fmaf(part[i][k], f, acc[k]);
+    }
+    for (int c = span.x + kAtOnce; c <= span.y; ++c) {
+        const float2 more = p.part_ml[index(c)];
+        if (more.x == -INFINITY) continue;
+        const float f = exp2_fast(more.x - top);
+        sum = fmaf(more.y, f, sum);
+        const float* at = p.part_o + index(c) * D + lane * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = fmaf(at[k], f, acc[k]);
+    }
+    const float inv = sum == 0.0F ? 0.0F : 1.0F / sum;
     bf16* dst = static_cast<bf16*>(t.out) + tree_out_row(t, b, kvh * (t.q_heads / t.kv.kv_heads) + row / t.nodes, node) * D + lane * V;
 #pragma unroll
     for (int i = 0; i < V; i += 2) *reinterpret_cast<__nv_bfloat162*>(dst + i) = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
