@@ -37,6 +37,14 @@ __device__ __forceinline__ int tree_node_count(const TreeParams& p, int b) {
     return n;
 }
 
+// Context length and node count of a sequence, both loads in flight together.
+__device__ __forceinline__ void tree_sizes(const TreeParams& p, int b, int& ctx, int& count, bool report) {
+    const int length = p.kv.lens[b], nodes = p.node_count ? p.node_count[b] : p.nodes;
+    ctx = min(max(length, 0), p.kv.limit);
+    count = min(max(nodes, 0), p.nodes);
+    if (report && (ctx != length || count != nodes)) atomicOr(p.kv.status, kCodeDecodeBounds);
+}
+
 __device__ __forceinline__ size_t tree_out_row(const TreeParams& p, int b, int head, int node) {
     return p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
                          : (static_cast<size_t>(b) * p.q_heads + head) * p.nodes + node;

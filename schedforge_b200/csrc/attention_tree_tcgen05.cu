@@ -70,8 +70,7 @@ struct Walk {
     int64_t left;
 
     __device__ __forceinline__ void read(const TreeTcParams& p) {
-        ctx = p.t.kv.length(b);
-        count = tree_node_count(p.t, b);
+        tree_sizes(p.t, b, ctx, count, false);
         tiles = tiles_of(ctx, count);
     }
     __device__ __forceinline__ int take() const { return static_cast<int>(left < tiles - x ? left : tiles - x); }
@@ -160,7 +159,11 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     grid_dependency_wait();
     if (warp == 10) {
         even_range(t_.batch, static_cast<int64_t>(kv.kv_heads) * p.row_groups, 1,
-                   [&](int b) { return tiles_of(kv.length(b), tree_node_count(t_, b)); }, start);
+                   [&](int b) {
+                       int ctx, count;
+                       tree_sizes(t_, b, ctx, count, blockIdx.x == 0);   // (the first CTA reports for all sequences)
+                       return tiles_of(ctx, count);
+                   }, start);
     }
     ptx::tc_fence_before();
     __syncthreads();
@@ -500,7 +503,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             tree_out_row(t_, w.b, kvh * (t_.q_heads / kv.kv_heads) + row / t_.nodes, node) * D;
                 float* part = p.part_o + (piece * ROWS + tile_row) * D;
                 if (!whole && live_row) p.part_ml[piece * ROWS + tile_row] = make_float2(m_used, row_sum);
-#pragma unroll 1
+#pragma unroll 2
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32], o2[32];
                     ptx::tmem_ld_32x32(o_addr + c * 32, o);

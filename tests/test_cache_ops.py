@@ -182,6 +182,8 @@ def test_tree_bad_parents_counts_lengths_and_blocks_are_cut_and_reported(dev, po
     got = tree_call(dev, port, cache, hq, nodes, counts, bad, q, dk, dv)
     assert status_word() & 0x200
     tree_check(got, cache, hq, counts, good, q, dk, dv)
+    tree_call(dev, port, cache, hq, nodes, [6, 6, 6, -1], parents, q, dk, dv)
+    assert status_word() & 0x200
     got = tree_call(dev, port, cache, hq, nodes, [6, 99, 6, -3], parents, q, dk, dv)   # cut to 6 and to 0
     assert status_word() & 0x200
     tree_check(got, cache, hq, [6, 6, 6, 0], parents, q, dk, dv)
