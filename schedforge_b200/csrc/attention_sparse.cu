@@ -736,7 +736,8 @@ select_kernel(const __grid_constant__ SelectParams p) {
             while (todo) {
                 const int i = i0 + __ffs(todo) - 1;
                 todo &= todo - 1;
-                const double v = exact_score<T>(p, b, kvh, i);
+                // (without any error the 32-bit scores are exact: a query or bounds of zeros, where all blocks tie)
+                const double v = err2 == 0.0F ? scores[i] : exact_score<T>(p, b, kvh, i);
                 if (lane == 0) exact[i] = v;
             }
         }

@@ -121,6 +121,9 @@ TREE_CASES = [
     ("bf16", 6, 2, 80, 96, 16, 12, [100, 47], [12, 5], 0, 0),           # not for the tensor-core kernel
     ("bf16", 3, 3, 128, 128, 24, 20, [100, 191], [20, 20], 0, 0),       # block of 24 tokens
     ("bf16", 4, 4, 64, 64, 16, 256, [40], [256], 0, 0),                 # the most nodes there can be
+    ("bf16", 4, 1, 128, 128, 8, 11, [300, 5], [11, 11], 0, 0),          # the smallest blocks TMA takes
+    ("bf16", 4, 1, 64, 64, 256, 11, [700, 129], [11, 2], 1, 0),         # blocks longer than a key tile
+    ("bf16", 4, 1, 128, 128, 1, 4, [37], [4], 0, 0),                    # blocks of one token
     ("bf16", 4, 2, 128, 128, 16, 130, [1500], [129], 0, 5),             # draft keys over more than one tile
 ]
 
@@ -400,6 +403,8 @@ def test_sparse_ties_go_to_the_lower_block_and_nan_scores_rank_last(dev):
     assert list(selected[0, 0]) == [0, 77]
     _, selected = sparse_call(dev, dd, q, inf, 2, 2999, 0, 0)
     assert list(selected[0, 0]) == [i for i in range(3000) if i != 78]
+    _, selected = sparse_call(dev, dd, 0.0 * q, bounds, 2, 5, 1, 1)     # a query of zeros: every score is zero
+    assert list(selected[0, 0]) == [0, 1, 2, 3, 2999]
 
 
 @gpu
