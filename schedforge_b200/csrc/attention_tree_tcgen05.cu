@@ -60,6 +60,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 __device__ __forceinline__ int tiles_of(int ctx, int count) {
     return count > 0 ? (ctx + KT - 1) / KT + (count + KT - 1) / KT : 0;
 }
@@ -441,26 +455,28 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     if (grow) m_used = tile_max;
                     const float neg_m = m_used == -INFINITY ? 0.0F : -m_used;
-                    float s0 = 0.0F, s1 = 0.0F, s2 = 0.0F, s3 = 0.0F;
+                    float2 s0 = make_float2(0.0F, 0.0F), s1 = s0;
+                    const float2 scale = make_float2(t_.scale_log2, t_.scale_log2), shift = make_float2(neg_m, neg_m);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t packed[16];
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float x0 = exp2_fast(fmaf(__uint_as_float(raw[c][i]), t_.scale_log2, neg_m));
-                            const float x1 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 1]), t_.scale_log2, neg_m));
-                            const float x2 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 2]), t_.scale_log2, neg_m));
-                            const float x3 = exp2_fast(fmaf(__uint_as_float(raw[c][i + 3]), t_.scale_log2, neg_m));
-                            s0 += x0; s1 += x1; s2 += x2; s3 += x3;
+                            float2 x = fma2(make_float2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), scale, shift);
+                            float2 y = fma2(make_float2(__uint_as_float(raw[c][i + 2]), __uint_as_float(raw[c][i + 3])), scale, shift);
+                            x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            s0 = add2(s0, x);
+                            s1 = add2(s1, y);
                             // the weights are rounded to bf16 for the product; the row sum keeps 32 bits
-                            const __nv_bfloat162 lo = __floats2bfloat162_rn(x0, x1), hi = __floats2bfloat162_rn(x2, x3);
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(y.x, y.y);
                             packed[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
                             packed[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
                         }
                         ptx::tmem_st_32x16(s_addr + c * 16, packed);
                     }
                     ptx::tmem_st_wait();
-                    row_sum += (s0 + s1) + (s2 + s3);
+                    row_sum += (s0.x + s0.y) + (s1.x + s1.y);
                 }
                 ptx::tc_fence_before();
                 ptx::mbar_arrive(ptx::smem_u32(&p_full[t]));
