@@ -28,64 +28,58 @@ __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-// acc(t, n) += the products of four column tiles n and all row tiles t over `steps` steps of eight, operands from
-// a(step, t, hi, lo) and b(step, n, hi, lo).  The instruction truncates its sums, so the large products run at most DEPTH
-// steps in an accumulator of their own before a rounded addition takes them over, and the small ones, which have 11 bits to
-// spare, meet them at the end.  (All three products in one accumulator running on over the tiles: 2.6e-6 off at logits of ten.)
-// Products of one accumulator are at least 4 * M instructions apart, since each waits for the one before.
-template <int M, int DEPTH, class Acc, class A, class B>
+// acc(t, n) += the products of N column tiles n and M row tiles t over `steps` steps of eight, operands from
+// a(step, t, hi, lo) and b(step, n, hi, lo).  The instruction truncates its sums, so an accumulator starts from zero every
+// DEPTH steps, takes the small products first, while truncation costs nothing, then the large ones, and a rounded addition
+// takes it over.  (All three products in one accumulator running on over the tiles: 2.6e-6 off at logits of ten.)
+// Four column tiles at a time, so that the products of one accumulator, each of which waits for the one before, are 4 * M
+// instructions apart.
+template <int M, int N, int DEPTH, class Acc, class A, class B>
 __device__ __forceinline__ void multiply(Acc acc, int steps, A a, B b) {
-    float small[M][4][4];
-#pragma unroll
-    for (int t = 0; t < M; ++t)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) small[t][n][i] = 0.0F;
 #pragma unroll 1
     for (int step0 = 0; step0 < steps; step0 += DEPTH) {
-        float big[M][4][4];
+        uint32_t ah[DEPTH][M][4], al[DEPTH][M][4];
 #pragma unroll
-        for (int t = 0; t < M; ++t)
+        for (int u = 0; u < DEPTH; ++u)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int t = 0; t < M; ++t) a(step0 + u, t, ah[u][t], al[u][t]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) big[t][n][i] = 0.0F;
+        for (int n0 = 0; n0 < N; n0 += 4) {
+            float sum[M][4][4];
+            uint32_t bh[DEPTH][4][2], bl[DEPTH][4][2];
 #pragma unroll
-        for (int u = 0; u < DEPTH; ++u) {
-            const int step = step0 + u;
-            if (step >= steps) continue;
-            uint32_t ah[M][4], al[M][4], bh[4][2], bl[4][2];
+            for (int t = 0; t < M; ++t)
 #pragma unroll
-            for (int t = 0; t < M; ++t) a(step, t, ah[t], al[t]);
+                for (int n = 0; n < 4; ++n) sum[t][n][0] = sum[t][n][1] = sum[t][n][2] = sum[t][n][3] = 0.0F;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) b(step, n, bh[n], bl[n]);
+            for (int u = 0; u < DEPTH; ++u)
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n) b(step0 + u, n0 + n, bh[u][n], bl[u][n]);
 #pragma unroll
-                for (int t = 0; t < M; ++t) mma_tf32(small[t][n], al[t], bh[n][0], bh[n][1]);
+            for (int u = 0; u < DEPTH; ++u) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int t = 0; t < M; ++t) mma_tf32(big[t][n], ah[t], bh[n][0], bh[n][1]);
+                    for (int t = 0; t < M; ++t) mma_tf32(sum[t][n], al[u][t], bh[u][n][0], bh[u][n][1]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int t = 0; t < M; ++t) mma_tf32(small[t][n], ah[t], bl[n][0], bl[n][1]);
+                    for (int t = 0; t < M; ++t) mma_tf32(sum[t][n], ah[u][t], bl[u][n][0], bl[u][n][1]);
+            }
+#pragma unroll
+            for (int u = 0; u < DEPTH; ++u)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int t = 0; t < M; ++t) mma_tf32(sum[t][n], ah[u][t], bh[u][n][0], bh[u][n][1]);
+#pragma unroll
+            for (int t = 0; t < M; ++t)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc(t, n0 + n)[i] += sum[t][n][i];
         }
-#pragma unroll
-        for (int t = 0; t < M; ++t)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc(t, n)[i] += big[t][n][i];
     }
-#pragma unroll
-    for (int t = 0; t < M; ++t)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc(t, n)[i] += small[t][n][i];
 }
 
 __host__ __device__ inline int k_stride(int dim) { return dim + 4; }                      // an odd multiple of 4: rows on different banks
@@ -107,6 +101,8 @@ template <int WIDE>
 __global__ void __launch_bounds__(Tile<WIDE>::kThreads)
 tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     constexpr int M = Tile<WIDE>::kM, kThreads = Tile<WIDE>::kThreads, kNT = BN / 8;
+    constexpr int kPieces = 2 * WIDE;      // lanes that copy a row, 16 bytes each
+    constexpr int kRowsAtOnce = kThreads / kPieces;
     extern __shared__ float4 tree_smem_raw[];
     __shared__ int missing[2];   // the tile has keys without a block
     const PagedView& kv = p.kv;
@@ -134,12 +130,16 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     const float* q = static_cast<const float*>(p.q) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all * kv.dim;
     const float* draft_k = static_cast<const float*>(p.draft_k) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim;
     const float* draft_v = static_cast<const float*>(p.draft_v) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim_v;
-    const auto find_rows = [&](int t0, int buffer) {
-        for (int i = threadIdx.x; i < BN; i += kThreads) {
-            const int key = t0 + i;
+    const auto find = [&](int t0) {   // the block of key t0 + thread, read long before it is needed
+        const int key = t0 + static_cast<int>(threadIdx.x);
+        return threadIdx.x < BN && key < min(k1, ctx) ? kv.page(b, key) : -1;
+    };
+    const auto note = [&](int t0, int page, int buffer) {
+        if (threadIdx.x < BN) {
+            const int i = threadIdx.x, key = t0 + i;
             const float *kr = nullptr, *vr = nullptr;
             if (key < min(k1, ctx)) {
-                const int64_t at = kv.row(b, kvh, key);
+                const int64_t at = kv.row_in(page, kvh, key);
                 if (at < 0) missing[buffer] = 1;
                 else {
                     kr = static_cast<const float*>(kv.k_pool) + at * kv.dim;
@@ -154,11 +154,15 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
         }
     };
     const auto fetch = [&](float* dst, int stride, int dim, const float** rows) {
-        const int pieces = dim / 4;
-#pragma unroll 8
-        for (int i = threadIdx.x; i < BN * pieces; i += kThreads) {
-            const int r = i / pieces, d = (i - r * pieces) * 4;
-            const float* src = rows[r];
+        const int d = 4 * (threadIdx.x % kPieces);
+        if (d >= dim) return;
+        const float* from[BN / kRowsAtOnce];   // (read together: the copies between them are barriers to the compiler)
+#pragma unroll
+        for (int i = 0; i < BN / kRowsAtOnce; ++i) from[i] = rows[threadIdx.x / kPieces + i * kRowsAtOnce];
+#pragma unroll
+        for (int i = 0; i < BN / kRowsAtOnce; ++i) {
+            const int r = threadIdx.x / kPieces + i * kRowsAtOnce;
+            const float* src = from[i];
             if (src) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst + r * stride + d))), "l"(src + d) : "memory");
             else *reinterpret_cast<float4*>(dst + r * stride + d) = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
         }
@@ -168,20 +172,25 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     if (threadIdx.x < 2) missing[threadIdx.x] = 0;
     __syncthreads();
     if (k0 < k1) {
-        find_rows(k0, 0);
+        note(k0, find(k0), 0);
         __syncthreads();
         fetch(ks, sk, kv.dim, k_rows);
         commit();
         fetch(vs, sv, kv.dim_v, v_rows);
         commit();
-        const int pieces = kv.dim / 4;
-#pragma unroll 8
-        for (int i = threadIdx.x; i < BM * pieces; i += kThreads) {
-            const int r = i / pieces, d = (i - r * pieces) * 4;
-            float4 v = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-            if (row0 + r < rows_all) v = *reinterpret_cast<const float4*>(q + static_cast<size_t>(row0 + r) * kv.dim + d);
-            *reinterpret_cast<float4*>(qs + r * sk + d) = make_float4(v.x * p.scale_log2, v.y * p.scale_log2, v.z * p.scale_log2, v.w * p.scale_log2);
+        const int d = 4 * (threadIdx.x % kPieces);
+        float4 v[BM / kRowsAtOnce];
+#pragma unroll
+        for (int i = 0; i < BM / kRowsAtOnce; ++i) {
+            const int r = row0 + threadIdx.x / kPieces + i * kRowsAtOnce;
+            v[i] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+            if (r < rows_all && d < kv.dim) v[i] = *reinterpret_cast<const float4*>(q + static_cast<size_t>(r) * kv.dim + d);
         }
+        if (d < kv.dim)
+#pragma unroll
+            for (int i = 0; i < BM / kRowsAtOnce; ++i)
+                *reinterpret_cast<float4*>(qs + (threadIdx.x / kPieces + i * kRowsAtOnce) * sk + d) =
+                    make_float4(v[i].x * p.scale_log2, v[i].y * p.scale_log2, v[i].z * p.scale_log2, v[i].w * p.scale_log2);
     }
     // row i of this lane: warp_row + 16 * (i / 2) + 8 * (i % 2) + r4
     float o[M][WIDE][4], m[2 * M], l[2 * M];
@@ -202,7 +211,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     int buffer = 0;
     for (int t0 = k0; t0 < k1; t0 += BN, buffer ^= 1) {
         const bool more = t0 + BN < k1;
-        if (more) find_rows(t0 + BN, buffer ^ 1);
+        const int next = more ? find(t0 + BN) : -1;
         wait_but_one();      // K
         __syncthreads();
         float s[M][kNT][4];
@@ -211,21 +220,19 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
             for (int t = 0; t < M; ++t)
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) s[t][n][0] = s[t][n][1] = s[t][n][2] = s[t][n][3] = 0.0F;
-#pragma unroll
-            for (int n0 = 0; n0 < kNT; n0 += 4)
-                multiply<M, 1>([&](int t, int n) -> float (&)[4] { return s[t][n0 + n]; }, kv.dim / 8,
-                    [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-                        const float* qa = qs + (warp * 16 * M + 16 * t + r4) * sk + 8 * step + quad;
-                        split(qa[0], hi[0], lo[0]);
-                        split(qa[8 * sk], hi[1], lo[1]);
-                        split(qa[4], hi[2], lo[2]);
-                        split(qa[8 * sk + 4], hi[3], lo[3]);
-                    },
-                    [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
-                        const float* ka = ks + (8 * (n0 + n) + r4) * sk + 8 * step + quad;
-                        split(ka[0], hi[0], lo[0]);
-                        split(ka[4], hi[1], lo[1]);
-                    });
+            multiply<M, kNT, 1>([&](int t, int n) -> float (&)[4] { return s[t][n]; }, kv.dim / 8,
+                [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+                    const float* qa = qs + (warp * 16 * M + 16 * t + r4) * sk + 8 * step + quad;
+                    split(qa[0], hi[0], lo[0]);
+                    split(qa[8 * sk], hi[1], lo[1]);
+                    split(qa[4], hi[2], lo[2]);
+                    split(qa[8 * sk + 4], hi[3], lo[3]);
+                },
+                [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+                    const float* ka = ks + (8 * n + r4) * sk + 8 * step + quad;
+                    split(ka[0], hi[0], lo[0]);
+                    split(ka[4], hi[1], lo[1]);
+                });
             if (t0 + BN > ctx || t0 + BN > k1) {
 #pragma unroll
                 for (int n = 0; n < kNT; ++n)
@@ -248,6 +255,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
                             for (int i = 0; i < 2 * M; ++i) s[i >> 1][n][2 * (i & 1) + e] = -INFINITY;
             }
         }
+        if (more) note(t0 + BN, next, buffer ^ 1);
         __syncthreads();
         if (more) fetch(ks, sk, kv.dim, k_rows + (buffer ^ 1) * BN);
         commit();
@@ -279,23 +287,19 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
         wait_but_one();      // V
         __syncthreads();
         if (busy) {
-#pragma unroll
-            for (int n0 = 0; n0 < WIDE; n0 += 4) {
-                if (n0 >= nv) continue;      // (columns of V's rows past dim_v feed outputs that are not stored)
-                multiply<M, 2>([&](int t, int n) -> float (&)[4] { return o[t][n0 + n]; }, BN / 8,
-                    [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-                        const float* pa = my_p + (16 * t + r4) * kPStride + 8 * step + quad;
-                        split(pa[0], hi[0], lo[0]);
-                        split(pa[8 * kPStride], hi[1], lo[1]);
-                        split(pa[4], hi[2], lo[2]);
-                        split(pa[8 * kPStride + 4], hi[3], lo[3]);
-                    },
-                    [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
-                        const float* va = vs + (8 * step + quad) * sv + (n0 + n < nv ? 8 * (n0 + n) : 0) + r4;
-                        split(va[0], hi[0], lo[0]);
-                        split(va[4 * sv], hi[1], lo[1]);
-                    });
-            }
+            multiply<M, WIDE, 2>([&](int t, int n) -> float (&)[4] { return o[t][n]; }, BN / 8,
+                [&](int step, int t, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+                    const float* pa = my_p + (16 * t + r4) * kPStride + 8 * step + quad;
+                    split(pa[0], hi[0], lo[0]);
+                    split(pa[8 * kPStride], hi[1], lo[1]);
+                    split(pa[4], hi[2], lo[2]);
+                    split(pa[8 * kPStride + 4], hi[3], lo[3]);
+                },
+                [&](int step, int n, uint32_t (&hi)[2], uint32_t (&lo)[2]) {   // (columns past dim_v feed outputs that are not stored)
+                    const float* va = vs + (8 * step + quad) * sv + (n < nv ? 8 * n : 0) + r4;
+                    split(va[0], hi[0], lo[0]);
+                    split(va[4 * sv], hi[1], lo[1]);
+                });
         }
         __syncthreads();
         if (more) fetch(vs, sv, kv.dim_v, v_rows + (buffer ^ 1) * BN);

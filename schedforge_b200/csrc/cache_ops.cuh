@@ -32,9 +32,10 @@ struct PagedView {
     }
     // Row of position `position` of sequence b and K/V head `head` in the [blocks][heads][tokens] pool; -1 where the
     // table names no block of the pool.
-    __device__ __forceinline__ int64_t row(int b, int head, int position) const {
+    __device__ __forceinline__ int64_t row(int b, int head, int position) const { return row_in(page(b, position), head, position); }
+    __device__ __forceinline__ int page(int b, int position) const { return table[static_cast<size_t>(b) * max_blocks + block_of(position)]; }
+    __device__ __forceinline__ int64_t row_in(int page, int head, int position) const {
         const int block = block_of(position);
-        const int page = table[static_cast<size_t>(b) * max_blocks + block];
         if (page < 0 || page >= num_blocks) {
             atomicOr(status, kCodeDecodeBounds);
             return -1;
