@@ -426,7 +426,7 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
                 }
         };
         load_heads(0);
-        __nv_bfloat162 most = __floats2bfloat162_rn(0.0F, 0.0F), least = most;
+        __nv_bfloat162 most = __floats2bfloat162_rn(0.0F, 0.0F);
         int n = 0;
         for (int base = begin; base < last; base += stage_blocks, ++n) {
             const int s = n % kScoreStages;
@@ -450,10 +450,8 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const bool ok = present >> ((lane >> 2) + 8 * (i & 1)) & 1u;   // (a row that was not loaded holds anything)
-                                const uint32_t word = ok ? a[i] : 0u;
-                                const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&word);
-                                if (k < KS) least = __hmin2(least, v);
-                                else most = __hmax2(most, v);
+                                const uint32_t word = ok ? a[i] & 0x7fff7fffu : 0u;
+                                most = __hmax2(most, *reinterpret_cast<const __nv_bfloat162*>(&word));
                             }
                         }
                     }
@@ -477,8 +475,7 @@ score_mma_kernel(const __grid_constant__ ScoreParams p) {
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&empty_bar[s]));
         }
-        // (low <= high, so the largest |bound| is the largest high or the smallest low)
-        size = warp_max(fmaxf(fmaxf(__low2float(most), __high2float(most)), -fminf(__low2float(least), __high2float(least))));
+        size = warp_max(fmaxf(__low2float(most), __high2float(most)));
     }
     if (warp < kWarps && lane == 0) size_of[warp] = size;
     __syncthreads();
@@ -535,9 +532,14 @@ ScoreShape score_shape(const sfb_sparse_args& a, int blocks) {
     return s;
 }
 
+// Three stages of at most 128 blocks and heads of 128, or 64 of 256, elements: 4 * dim + 16 bytes for each at most.
+constexpr int kScoreSmemLimit = kScoreStages * 128 * (4 * 128 + 16);
+static_assert(kScoreSmemLimit >= kScoreStages * 64 * (4 * 256 + 16) && kScoreSmemLimit >= kScoreStages * kScoreWarps * kScoreBatchBytes, "scores");
+
 template <class Kernel>
 sfb_status launch_score(Kernel kernel, int threads, size_t smem, dim3 grid, const ScoreParams& p, cudaStream_t stream) {
-    if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // (the same limit for every shape, since another thread may be launching the kernel)
+    if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kScoreSmemLimit));
     SFB_CUDA(launch_dependent(kernel, grid, dim3(threads), smem, stream, p));
     return check_launch("sparse_scores");
 }
@@ -682,7 +684,11 @@ select_kernel(const __grid_constant__ SelectParams p) {
         size = warp_max(lane < kSelectThreads / 32 ? most[1][lane] : 0.0F);
     }
     const int n_forced = min(sink, n) + min(p.recent, n) - max(0, min(sink, n) - max(recent_from, 0));
-    const float err2 = 2.0F * p.error * norm * size;  // 2 err
+    // 2 err: relative to the largest sum of products there can be, and 1e-34 for products below the normal numbers.  Where
+    // that sum could leave the range (or is NaN) a 32-bit score says nothing, and every block is ranked in 64 bits.
+    const float reach = norm * size;
+    const float err2 = reach < 1e37F ? 2.0F * p.error * reach + 1e-34F : INFINITY;
+    const bool zeros = norm == 0.0F || size == 0.0F;   // (then every score is exactly zero)
     if (p.cached && k > n_forced) {
         const bool settled = select_mask<kSelectThreads>(
             sh, keys, n, k - n_forced,
@@ -736,8 +742,7 @@ select_kernel(const __grid_constant__ SelectParams p) {
             while (todo) {
                 const int i = i0 + __ffs(todo) - 1;
                 todo &= todo - 1;
-                // (without any error the 32-bit scores are exact: a query or bounds of zeros, where all blocks tie)
-                const double v = err2 == 0.0F ? scores[i] : exact_score<T>(p, b, kvh, i);
+                const double v = zeros ? 0.0 : exact_score<T>(p, b, kvh, i);
                 if (lane == 0) exact[i] = v;
             }
         }
@@ -849,7 +854,7 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
         const dim3 grid(a->kv_heads, a->batch);
         const size_t smem = p.cached ? sizeof(float) * l.score_stride : 0;
         const auto go = [&](auto kernel) -> sfb_status {
-            if (smem > 0) SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            SFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(uint32_t) * kMaskItems)));
             SFB_CUDA(launch_dependent(kernel, grid, dim3(kSelectThreads), smem, s, p));
             return SFB_OK;
         };

@@ -408,6 +408,73 @@ def test_sparse_ties_go_to_the_lower_block_and_nan_scores_rank_last(dev):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,d", [("f32", 32), ("f32", 20), ("bf16", 64)])
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** -70, 2.0 ** -70), (2.0 ** 80, 2.0 ** 50), (2.0 ** -75, 1.0), (1.0, 2.0 ** 100)])
+def test_sparse_ranks_scores_outside_the_range_of_float32_by_their_64_bit_sums(dev, port, dtype, d, q_size, k_size):
+    """Products that vanish or overflow in 32 bits (keys are equal within a block, so sums cancel)."""
+    rng = np.random.default_rng(d)
+    cache = Cache(rng, [16 * 60], 1, d, d, 16, dtype, round_bf16=port.round_bf16)
+    for i in range(60):
+        row = cache.keys[0][:, 16 * i:16 * i + 1] * k_size
+        cache.keys[0][:, 16 * i:16 * i + 16] = row
+        cache.k_pool[cache.table[0, i]] = row
+    dd = Device(dev, cache)
+    bounds = dd.put(np.zeros((cache.num_blocks, 1, 2, d), np.float32))
+    bounds_call(dev, dd, bounds, [0], cache.lens, 960)
+    q = rounder(port, dtype)(rng.standard_normal((1, 3, d)).astype(np.float32)) * np.float32(q_size)
+    for budget, sink, recent in ((7, 1, 1), (1, 0, 0), (59, 0, 3)):
+        _, selected = sparse_call(dev, dd, q, bounds, 3, budget, sink, recent)
+        assert list(selected[0, 0]) == plain_select(cache, 0, 0, q[0].astype(np.float64), budget, sink, recent)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [("f32", 32), ("f32", 20), ("bf16", 64)])
+def test_sparse_ignores_an_element_whose_query_is_zero(dev, port, dtype, d):
+    """A block whose keys are all NaN in one element has low = inf and high = -inf there."""
+    rng = np.random.default_rng(d)
+    cache = Cache(rng, [16 * 60], 1, d, d, 16, dtype, round_bf16=port.round_bf16)
+    q = rounder(port, dtype)(rng.standard_normal((1, 3, d)).astype(np.float32))
+    q[:, :, 5] = 0.0
+    want = plain_select(cache, 0, 0, q[0].astype(np.float64), 9, 0, 0)
+    for i in range(0, 60, 3):
+        cache.k_pool[cache.table[0, i], :, :, 5] = np.nan
+    dd = Device(dev, cache)
+    bounds = dd.put(np.zeros((cache.num_blocks, 1, 2, d), np.float32))
+    bounds_call(dev, dd, bounds, [0], cache.lens, 960)
+    _, selected = sparse_call(dev, dd, q, bounds, 3, 9, 0, 0)
+    assert list(selected[0, 0]) == want
+    q[:, 1, 5] = 1.0                                          # now such a block's second head has no upper bound but -inf
+    q[:, 0], q[:, 2] = q[:, 1], q[:, 1]
+    _, selected = sparse_call(dev, dd, q, bounds, 3, 40, 0, 0)
+    assert list(selected[0, 0]) == [i for i in range(60) if i % 3]
+
+
+@gpu
+@pytest.mark.parametrize("blocks,block", [(3000, 16), (300, 16), (43000, 1)])
+def test_sparse_bf16_ties_go_to_the_lower_block_and_infinite_scores_count(dev, blocks, block):
+    rng = np.random.default_rng(blocks)
+    cache = Cache(rng, [block * blocks], 1, 16, 16, block, "f32")
+    cache.dtype = "bf16"
+    row = np.exp2(rng.integers(-3, 4, (1, 1, 1, 16))).astype(np.float32)
+    cache.k_pool[:] = row                                      # every block scores the same
+    dd = Device(dev, cache)
+    bounds = dd.put(np.zeros((cache.num_blocks, 1, 2, 16), np.float32))
+    bounds_call(dev, dd, bounds, [0], cache.lens, block * blocks)
+    q = np.ones((1, 2, 16), np.float32)
+    _, selected = sparse_call(dev, dd, q, bounds, 2, 250, 0, 1)
+    assert list(selected[0, 0]) == list(range(249)) + [blocks - 1]
+    inf = bounds.clone()
+    inf[cache.table[0, 77].item()] = float("inf")
+    inf[cache.table[0, 78].item()] = float("-inf")
+    _, selected = sparse_call(dev, dd, q, inf, 2, 2, 0, 0)
+    assert list(selected[0, 0]) == [0, 77]
+    _, selected = sparse_call(dev, dd, q, inf, 2, blocks - 1, 0, 0)
+    assert list(selected[0, 0]) == [i for i in range(blocks) if i != 78]
+    _, selected = sparse_call(dev, dd, 0.0 * q, bounds, 2, 5, 1, 1)
+    assert list(selected[0, 0]) == [0, 1, 2, 3, blocks - 1]
+
+
+@gpu
 def test_sparse_bad_lengths_and_blocks(dev, port):
     rng = np.random.default_rng(9)
     cache = Cache(rng, [320, 320, 320], 2, 64, 64, 16, "bf16", round_bf16=port.round_bf16)
