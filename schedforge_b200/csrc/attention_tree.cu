@@ -261,7 +261,9 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
 template <class T, int NV>
 sfb_status launch_tree(const TreeParams& p, cudaStream_t stream) {
     const size_t smem = tree_smem(p.kv.dim, NV, p.nodes);
-    SFB_CUDA(cudaFuncSetAttribute(tree_simt_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // (the same limit for every shape, since another thread may be launching the kernel)
+    static const int most = static_cast<int>(tree_smem(256, NV, SFB_MAX_TREE_NODES));
+    SFB_CUDA(cudaFuncSetAttribute(tree_simt_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     const int rows = p.q_heads / p.kv.kv_heads * p.nodes;
     const dim3 grid(ceil_div(rows, BM) * p.splits, p.kv.kv_heads, p.batch);
     SFB_CUDA(launch_dependent(tree_simt_kernel<T, NV>, grid, dim3(TreeTile<NV>::kThreads), smem, stream, p));

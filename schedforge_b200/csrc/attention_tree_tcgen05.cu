@@ -49,10 +49,13 @@ struct TreeTcParams {
     int rows_all, row_groups, box_rows;
     int64_t pairs;
     int pool_rows;
-    float* part_o;          // [grid + pairs][ROWS][D]
-    float2* part_ml;        // [grid + pairs][ROWS]
+    float* part_o;          // [2 * grid][ROWS][D], by piece_of
+    float2* part_ml;        // [2 * grid][ROWS]
     int2* pair_span;        // [pairs]: first and last CTA
 };
+
+// Place of a cut pair's piece: a CTA has at most one pair that began before it and one that begins in it and goes on.
+__device__ __forceinline__ int64_t piece_of(int cta, bool begins) { return 2 * static_cast<int64_t>(cta) + (begins ? 1 : 0); }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -514,7 +517,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 f0 *= inv;
                 f1 *= inv;
                 const bool second = !kTwoTiles && n > 1;
-                const int64_t piece = static_cast<int64_t>(blockIdx.x) + pair;
+                const int64_t piece = piece_of(blockIdx.x, w.x == 0);
                 bf16* dst = static_cast<bf16*>(t_.out) +
                             tree_out_row(t_, w.b, kvh * (t_.q_heads / kv.kv_heads) + row / t_.nodes, node) * D;
                 float* part = p.part_o + (piece * ROWS + tile_row) * D;
@@ -596,7 +599,7 @@ tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
     if (span.x == span.y) return;   // written by the attention kernel itself
     // up to kAtOnce pieces are read at the same time
     constexpr int kAtOnce = 8;
-    const auto index = [&](int c) { return (c + pair) * rows_cta + tile_row; };
+    const auto index = [&](int c) { return piece_of(c, c == span.x) * rows_cta + tile_row; };
     float2 ml[kAtOnce];
     float part[kAtOnce][V];
     float top = -INFINITY;
@@ -658,7 +661,7 @@ TcLayout tc_layout(const sfb_tree_args& a) {
     int ctas = sm_count();
     if (a.splits > 0 && l.pairs * a.splits < ctas) ctas = static_cast<int>(l.pairs * a.splits);
     l.grid = static_cast<int>(most < ctas ? most : ctas);
-    const size_t pieces = static_cast<size_t>(l.grid + l.pairs);
+    const size_t pieces = 2 * static_cast<size_t>(l.grid);
     l.ml = sizeof(float) * pieces * l.rows_cta * a.head_dim;
     l.span = l.ml + sizeof(float2) * pieces * l.rows_cta;
     l.total = l.span + sizeof(int2) * static_cast<size_t>(l.pairs);

@@ -332,7 +332,9 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
 template <int WIDE>
 sfb_status launch(const TreeParams& p, cudaStream_t stream) {
     const size_t smem = smem_bytes(p.kv.dim, p.kv.dim_v, p.nodes);
-    SFB_CUDA(cudaFuncSetAttribute(tree_tf32_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // (the same limit for every shape, since another thread may be launching the kernel)
+    static const int most = static_cast<int>(smem_bytes(8 * WIDE, 8 * WIDE, SFB_MAX_TREE_NODES));
+    SFB_CUDA(cudaFuncSetAttribute(tree_tf32_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     const int rows = p.q_heads / p.kv.kv_heads * p.nodes;
     const dim3 grid(ceil_div(rows, BM) * p.splits, p.kv.kv_heads, p.batch);
     SFB_CUDA(launch_dependent(tree_tf32_kernel<WIDE>, grid, dim3(Tile<WIDE>::kThreads), smem, stream, p));
