@@ -328,10 +328,11 @@ sfb_status sfb_k_paged_kv_gather(const void* k_pool, const void* v_pool, void* k
  * positions count as masked); either sets bit 0x200 of sfb_device_status.  bf16 or float32, head dimensions up to 256
  * of either kind, any block size and any number of query heads per K/V head.  A sequence with nothing to attend to
  * gives zeros.  Positions behind the live ones (the rest of a block, rows of dead nodes) may hold anything, NaN
- * included.  `workspace`: device memory of at least the bytes the function beside it reports for the same arguments, 16-byte
+ * included; a block shared by several sequences has to be full, and sfb_k_paged_kv_accept and sfb_k_paged_kv_evict write
+ * to blocks that no other sequence may hold.  `workspace`: device memory of at least the bytes the function beside it reports for the same arguments, 16-byte
  * aligned, contents irrelevant before and after; calls that can overlap on the GPU need separate ones.  `splits` <= 0
- * lets the library choose; `scale` <= 0 means 1/sqrt(head_dim).  Kernels are chosen by type, head dimension and
- * alignment only, so the same arguments give the same bits every time. */
+ * lets the library choose; `scale` <= 0 means 1/sqrt(head_dim).  Kernels are chosen by types, sizes and alignment, and no
+ * result depends on the order in which threads arrive, so the same arguments give the same bits every time. */
 
 /* Attention of a tree of drafted tokens over the cache (verification step of speculative decoding).  Every sequence
  * brings `nodes` drafted tokens, of which the first node_count[b] are live; node i hangs below node parents[i] < i, or
@@ -340,8 +341,9 @@ sfb_status sfb_k_paged_kv_gather(const void* k_pool, const void* v_pool, void* k
  *   out[b,h,i,:] = softmax over those of (scale * q . k) . v
  * The drafted tokens' keys and values are passed as the layer produced them and are not in the cache;
  * sfb_k_paged_kv_accept appends the accepted ones.  Rows of dead nodes are left as they were.  A parent outside
- * [-1, i) counts as -1, a node_count outside [0, nodes] is cut, both set bit 0x200.  Values of live nodes must be
- * finite: a NaN in one reaches every row of its tree.  nodes <= SFB_MAX_TREE_NODES, else SFB_UNSUPPORTED. */
+ * [-1, i) counts as -1, a node_count outside [0, nodes] is cut, both set bit 0x200.  Queries, keys and values of live
+ * positions and nodes have to be finite: a NaN or an infinity in a value reaches every row of its tree, and float32 products
+ * are taken of split operands, which turns an infinite one into a NaN.  nodes <= SFB_MAX_TREE_NODES, else SFB_UNSUPPORTED. */
 #define SFB_MAX_TREE_NODES 256
 typedef struct sfb_tree_args {
     const void* q;           /* [batch, q_heads, nodes, head_dim]                                    */

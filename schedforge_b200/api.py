@@ -328,11 +328,17 @@ class PagedKVCache:
         L.check(L.load().sfb_paged_decode(self._h, C.byref(config), _fp(q), _fp(out), C.byref(ms)))
         return out, ms.value
 
+    def _check_drafts(self, keys, values, nodes):
+        b, hkv, d, dv, _, _ = self.shape
+        if keys.shape != (b, hkv, nodes, d) or values.shape != (b, hkv, nodes, dv):
+            raise ValueError("drafted keys and values: [batch, kv_heads, nodes, dim] each")
+
     def decode_tree(self, config, q, draft_keys, draft_values, parents):
         """Attention of config.sequence_query drafted tokens (parents [B, nodes]) over the cache: (out, ms)."""
         q, draft_keys, draft_values, parents = _f32(q), _f32(draft_keys), _f32(draft_values), _i32(parents)
         if parents.shape != (config.batch, config.sequence_query):
             raise ValueError("parents: one per sequence and node")
+        self._check_drafts(draft_keys, draft_values, config.sequence_query)
         out = np.empty((config.batch, config.query_heads, config.sequence_query, config.head_dim_value), np.float32)
         ms = C.c_double(0)
         L.check(L.load().sfb_paged_decode_tree(self._h, C.byref(config), _fp(q), _fp(draft_keys), _fp(draft_values),
@@ -344,6 +350,7 @@ class PagedKVCache:
         draft_keys, draft_values, path = _f32(draft_keys), _f32(draft_values), _i32(path)
         if path.ndim != 2 or path.shape[0] != self.shape[0]:
             raise ValueError("path: one row per sequence")
+        self._check_drafts(draft_keys, draft_values, draft_keys.shape[2] if draft_keys.ndim == 4 else 0)
         L.check(L.load().sfb_paged_accept(self._h, _fp(draft_keys), _fp(draft_values), draft_keys.shape[2], _ip(path),
                                           path.shape[1]))
 

@@ -319,8 +319,8 @@ sfb_status check_cache(const void* k_pool, const void* v_pool, const int* table,
     SFB_REQUIRE(dtype == SFB_F32 || dtype == SFB_BF16, name + ": unknown dtype");
     if (dim > 256 || dim_v > 256) return fail(SFB_UNSUPPORTED, name + ": head dimension > 256");
     if (batch > 65535 || kv_heads > 4096) return fail(SFB_UNSUPPORTED, name + ": more than 65535 sequences or 4096 K/V heads");
-    if (static_cast<int64_t>(max_blocks) * block_tokens > (int64_t{1} << 30))
-        return fail(SFB_UNSUPPORTED, name + ": more than 2^30 positions in a block table");
+    if (static_cast<int64_t>(max_blocks) * block_tokens > (int64_t{1} << 29))   // (a warp adds up 32 sequences' units in 32 bits)
+        return fail(SFB_UNSUPPORTED, name + ": more than 2^29 positions in a block table");
     return SFB_OK;
 }
 

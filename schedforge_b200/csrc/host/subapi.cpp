@@ -93,7 +93,7 @@ struct sfb_paged_kv {
     int pages() const { return (capacity + page_tokens - 1) / page_tokens; }
     // pages for `tokens` more positions, from the back of the free list
     void reserve(int tokens) {
-        if (tokens <= 0 || length + tokens > capacity) throw std::invalid_argument("paged KV capacity exceeded");
+        if (tokens <= 0 || tokens > capacity - length) throw std::invalid_argument("paged KV capacity exceeded");
         const int last_page = (length + tokens - 1) / page_tokens;
         while (static_cast<int>(page_table.size()) <= last_page) {
             if (free_pages.empty()) throw std::runtime_error("paged KV page allocator exhausted");
@@ -413,7 +413,7 @@ sfb_status sfb_paged_accept(sfb_paged_kv* cache, const float* draft_keys, const 
     return guarded([&] {
         if (!cache) throw std::invalid_argument("null paged KV cache");
         auto& c = *cache;
-        if (tokens <= 0 || c.length + tokens > c.capacity) throw std::invalid_argument("paged KV capacity exceeded");
+        if (tokens <= 0 || tokens > c.capacity - c.length) throw std::invalid_argument("paged KV capacity exceeded");
         if (!draft_keys || !draft_values || !path || nodes <= 0) throw std::invalid_argument("paged KV append shape mismatch");
         for (int i = 0; i < c.batch * tokens; ++i)
             if (path[i] < 0 || path[i] >= nodes) throw std::invalid_argument("accepted path names a node that is not in the tree");
