@@ -16,6 +16,11 @@
 //   ROWS = 256: the two groups own two 128-row tiles and meet every key tile;
 //   ROWS = 128: both own the same rows and take alternate key tiles, each with its own running maximum and
 //               accumulator; the first group joins them at the end of a piece, out of tensor memory.
+// A slot's scores of the next tile are issued behind its P.V of this one, since P lies over them.  Taken in two steps of 64 keys
+// (two S/P areas a slot), one step's products run under the softmax of the other, at the price of N = 64 products, which read
+// Q from shared memory twice as often: 69 -> 61 us for 8 sequences of 8192 tokens, one node, 128 elements a head.  It does not
+// pay with two row tiles, where the other tile's products fill the time already (113 -> 123 us with 256 rows), nor at 64
+// elements a head, where the products are half as long (44 -> 50 us).
 // Positions past the context in a loaded block may hold anything: their scores are masked and their V rows are zeroed
 // in shared memory before the product (0 * NaN).  Warps without a live row skip the arithmetic.  Waits are bounded.
 #include "attention_tree.cuh"
@@ -27,7 +32,7 @@ namespace {
 constexpr int KT = 128;
 constexpr int kThreads = 384;
 constexpr int kHalfBytes = KT * 64 * 2;
-constexpr uint32_t kTmemCols = 512;   // S_t (P_t over its first half) at t * 128, O_t at 256 + t * D
+constexpr uint32_t kTmemCols = 512;   // S_th (P_th over its first half) at t * 128 + h * 64, O_t at 256 + t * D
 constexpr uint32_t kOCol = 256;
 constexpr uint32_t kCodeTree = 0x80;
 constexpr float kRescaleThreshold = 8.0F;  // log2 units
@@ -37,6 +42,8 @@ template <int D, int ROWS>
 struct Shape {
     static constexpr int kHalves = D / 64;
     static constexpr int kQTiles = ROWS / 128;
+    // A tile of keys is taken in one step or in two: see the head of the file.
+    static constexpr int kSteps = ROWS == 128 && D == 128 ? 2 : 1, kKeys = KT / kSteps;
     static constexpr int kQBytes = kHalves * kHalfBytes;   // one 128-row tile
     static constexpr int kTileBytes = kHalves * kHalfBytes;
     static constexpr int kStages = D == 64 ? 5 : (ROWS == 128 ? 3 : 2);
@@ -113,6 +120,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     using Sh = Shape<D, ROWS>;
     constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kTileBytes = Sh::kTileBytes;
     constexpr bool kTwoTiles = ROWS == 256;
+    constexpr int kSteps = Sh::kSteps, KH = Sh::kKeys;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* q_smem = smem;
@@ -123,13 +131,13 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     uint64_t* bars = reinterpret_cast<uint64_t*>(ml_smem + 128);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;
-    uint64_t* s_full = bars + 2;     // [2]
-    uint64_t* p_full = bars + 4;     // [2]
-    uint64_t* o_full = bars + 6;     // [2]
-    uint64_t* par_full = bars + 8;   // [2]
-    uint64_t* ml_full = bars + 10;   // group 1's maxima and sums are in shared memory
-    uint64_t* o_free = bars + 11;    // group 0 has read group 1's accumulator
-    uint64_t* k_full = bars + 12;
+    uint64_t* s_full = bars + 2;     // [2][2]: scores of slot t, step h; with two steps, h = 0 once more behind a piece's last tile
+    uint64_t* p_full = bars + 6;     // [2][2]
+    uint64_t* par_full = bars + 10;  // [2]
+    uint64_t* ml_full = bars + 12;   // group 1's maxima and sums are in shared memory
+    uint64_t* o_free = bars + 13;    // group 0 has read group 1's accumulator
+    uint64_t* o_full = bars + 14;    // [2]
+    uint64_t* k_full = bars + 16;
     uint64_t* k_empty = k_full + kStages;
     uint64_t* v_full = k_empty + kStages;
     uint64_t* v_empty = v_full + kStages;
@@ -147,8 +155,10 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         ptx::mbar_init(ptx::smem_u32(q_full), 1);
         ptx::mbar_init(ptx::smem_u32(q_empty), 1);
         for (int t = 0; t < 2; ++t) {
-            ptx::mbar_init(ptx::smem_u32(&s_full[t]), 1);
-            ptx::mbar_init(ptx::smem_u32(&p_full[t]), 128);
+            for (int h = 0; h < 2; ++h) {
+                ptx::mbar_init(ptx::smem_u32(&s_full[2 * t + h]), 1);
+                ptx::mbar_init(ptx::smem_u32(&p_full[2 * t + h]), 128);
+            }
             ptx::mbar_init(ptx::smem_u32(&o_full[t]), 1);
             ptx::mbar_init(ptx::smem_u32(&par_full[t]), 128);
         }
@@ -266,12 +276,12 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         } else if (warp == 9) {
             // ------------------------------------------------------------ MMA issue
             // (the whole warp walks along, so that the operands are uniform; one lane of it issues)
-            constexpr uint32_t idesc_qk = ptx::umma_idesc_bf16(128, KT, 0, 0);
+            constexpr uint32_t idesc_qk = ptx::umma_idesc_bf16(128, KH, 0, 0);
             constexpr uint32_t idesc_pv = ptx::umma_idesc_bf16(128, D, 0, 1);
             const uint64_t q_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(q_smem)), k_desc = ptx::umma_desc_k_sw128(ptx::smem_u32(k_smem)),
                            v_desc = ptx::umma_desc_mn_sw128(ptx::smem_u32(v_smem), kHalfBytes, 1024);
             const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
-            uint32_t n_kv = 0, n_seg = 0, slot_parity[2] = {0, 0};   // tiles and pieces so far, parity of each slot's uses
+            uint32_t n_kv = 0, n_seg = 0, p_parity = 0;   // tiles and pieces so far, parity of the uses of each P (bits)
             const auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
                 return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(bar), parity, abort_flag, status, kCodeTree | 2));
             };
@@ -281,44 +291,62 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const int items = kTwoTiles ? 2 * n : n;
                 ok = wait(q_full, n_seg & 1);
                 if (!ok) break;
-                // S_t = Q . K_j^T for item i (tile j, slot t)
-                const auto issue_qk = [&](int i, int t) -> bool {
+                // S_th = Q . K_jh^T for item i (tile j, slot t), step h
+                const auto issue_qk = [&](int i, int t, int h) -> bool {
                     const uint32_t g = n_kv + (kTwoTiles ? i >> 1 : i), stage = g % kStages;
-                    if (!wait(&k_full[stage], (g / kStages) & 1)) return false;
-                    ptx::tc_fence_after();
-                    // (a step along K only adds to the address field of the descriptors)
-                    const uint64_t qa = q_desc + (kTwoTiles ? t : 0) * (Sh::kQBytes >> 4), ka = k_desc + stage * (kTileBytes >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const int off = (kk / 4) * (kHalfBytes >> 4) + (kk % 4) * (32 >> 4);
-                        ptx::umma_bf16_warp(tmem + t * KT, qa + off, ka + off, idesc_qk, kk != 0);
+                    if (h == 0 && (!kTwoTiles || t == 0)) {   // (the others meet the tile that this one has waited for)
+                        if (!wait(&k_full[stage], (g / kStages) & 1)) return false;
+                        ptx::tc_fence_after();
                     }
-                    ptx::umma_commit_warp(ptx::smem_u32(&s_full[t]));
-                    if (!kTwoTiles || t == 1) ptx::umma_commit_warp(ptx::smem_u32(&k_empty[stage]));
-                    if (i == items - 1) ptx::umma_commit_warp(ptx::smem_u32(q_empty));
+                    // (a step along K only adds to the address field of the descriptors)
+                    const uint64_t qa = q_desc + (kTwoTiles ? t : 0) * (Sh::kQBytes >> 4), ka = k_desc + stage * (kTileBytes >> 4) + h * (KH * 128 >> 4);
+#pragma unroll
+                    for (int half = 0; half < kHalves; ++half)
+                        ptx::umma_bf16_x4_warp(tmem + t * KT + h * KH, qa + half * (kHalfBytes >> 4), ka + half * (kHalfBytes >> 4), idesc_qk, half != 0);
                     return true;
                 };
-                ok = issue_qk(0, 0);
-                if (ok && items > 1) ok = issue_qk(1, 1);
-                for (int i0 = 0; ok && i0 < items; i0 += 2) {
+                const auto after_qk = [&](int i, int t, int h) {
+                    if (h < kSteps - 1) return;
+                    if (!kTwoTiles || t == 1) ptx::umma_commit_warp(ptx::smem_u32(&k_empty[(n_kv + (kTwoTiles ? i >> 1 : i)) % kStages]));
+                    if (i == items - 1) ptx::umma_commit_warp(ptx::smem_u32(q_empty));
+                };
+#pragma unroll
+                for (int h = 0; h < kSteps; ++h)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const int i = i0 + t;
-                        if (!ok || i >= items) continue;
-                        const uint32_t g = n_kv + (kTwoTiles ? i >> 1 : i), stage = g % kStages;
-                        ok = wait(&v_full[stage], (g / kStages) & 1) && wait(&p_full[t], slot_parity[t]);
-                        if (!ok) continue;
-                        slot_parity[t] ^= 1;
-                        ptx::tc_fence_after();
-                        const uint64_t va = v_desc + stage * (kTileBytes >> 4);
-#pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)   // O_t += P_t . V_j
-                            ptx::umma_bf16_ts_warp(tmem + kOCol + t * D, tmem + t * KT + kk * 8, va + kk * (16 * 128 >> 4), idesc_pv, (i0 | kk) != 0);
-                        // the tensor pipe runs in order: P_t is consumed before S_t is overwritten
-                        if (i + 2 < items) ok = issue_qk(i + 2, t);
-                        if (!kTwoTiles || t == 1) ptx::umma_commit_warp(ptx::smem_u32(&v_empty[stage]));
-                        if (i + 2 >= items) ptx::umma_commit_warp(ptx::smem_u32(&o_full[t]));
+                        if (!ok || t >= items) continue;
+                        ok = issue_qk(t, t, h);
+                        ptx::umma_commit_warp(ptx::smem_u32(&s_full[2 * t + h]));
+                        after_qk(t, t, h);
                     }
+                for (int i0 = 0; ok && i0 < items; i0 += 2) {
+#pragma unroll
+                    for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int i = i0 + t, at = 2 * t + h;
+                            if (!ok || i >= items) continue;
+                            const uint32_t g = n_kv + (kTwoTiles ? i >> 1 : i), stage = g % kStages;
+                            if (h == 0 && (!kTwoTiles || t == 0)) ok = wait(&v_full[stage], (g / kStages) & 1);
+                            ok = ok && wait(&p_full[at], p_parity >> at & 1);
+                            if (!ok) continue;
+                            p_parity ^= 1u << at;
+                            ptx::tc_fence_after();
+                            // O_t += P_th . V_jh; then the scores of the slot's next tile (the tensor pipe runs in order: P_th is
+                            // consumed before S_th is overwritten)
+#pragma unroll
+                            for (int k = 0; k < KH / 64; ++k)
+                                ptx::umma_bf16_ts_x4_warp(tmem + kOCol + t * D, tmem + t * KT + h * KH + k * 32,
+                                                          v_desc + stage * (kTileBytes >> 4) + (h * KH + k * 64) * (128 >> 4), idesc_pv, (i0 | h | k) != 0);
+                            if (h == kSteps - 1 && (!kTwoTiles || t == 1) && i + 2 >= items) ptx::umma_commit_warp(ptx::smem_u32(&v_empty[stage]));
+                            if (i + 2 < items) ok = issue_qk(i + 2, t, h);
+                            if (i + 2 < items || h < kSteps - 1) ptx::umma_commit_warp(ptx::smem_u32(&s_full[at]));
+                            else ptx::umma_commit_warp(ptx::smem_u32(&o_full[t]));
+                            if (i + 2 < items) {
+                                after_qk(i + 2, t, h);
+                                if (h == kSteps - 1 && (!kTwoTiles || t == 1)) ptx::umma_commit_warp(ptx::smem_u32(&v_empty[stage]));
+                            }
+                        }
                 }
                 n_kv += n;
                 ++n_seg;
@@ -336,7 +364,7 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t s_addr = tmem_base + lane_base + t * KT;
         const uint32_t o_addr = tmem_base + lane_base + kOCol + t * D;
         uint8_t* parent = parent_smem + t * SFB_MAX_TREE_NODES;
-        uint32_t n_kv = 0, n_slot = 0, n_out = 0, n_seg = 0, n_par = 0;
+        uint32_t n_kv = 0, n_first = 0, n_second = 0, n_out = 0, n_seg = 0, n_par = 0;   // n_first, n_second: uses of s_full
         bool ok = true;
         while (ok && w.left > 0) {
             const int n = w.take();
@@ -363,9 +391,8 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     ptx::mbar_arrive(ptx::smem_u32(&par_full[t]));
                 }
-                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[t]), n_slot & 1, abort_flag, status, kCodeTree | 4);
+                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[2 * t]), n_first & 1, abort_flag, status, kCodeTree | 4);
                 if (!ok) break;
-                ++n_slot;
                 ptx::tc_fence_after();
                 const int key0 = draft ? (x - n_ctx) * KT : x * KT;
                 const int live = min(KT, (draft ? w.count : w.ctx) - key0);
@@ -413,80 +440,97 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     ptx::fence_proxy_async();
                 }
-                if (live_warp) {
-                    uint32_t raw[KT / 32][32];
-                    ptx::tmem_ld_32x32(s_addr, raw[0]);
-                    ptx::tmem_ld_32x32(s_addr + 32, raw[1]);
-                    ptx::tmem_ld_32x32(s_addr + 64, raw[2]);
-                    ptx::tmem_ld_32x32(s_addr + 96, raw[3]);
-                    ptx::tmem_ld_wait();
-                    if (masked) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (!(see[c] >> i & 1u)) raw[c][i] = 0xff800000u;  // -inf, and 2^-inf = 0 below
+                for (int h = 0; h < kSteps; ++h) {
+                    if (h == 1) {
+                        ok = ptx::mbar_wait(ptx::smem_u32(&s_full[2 * t + 1]), n_second & 1, abort_flag, status, kCodeTree | 4);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
                     }
-                    float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+                    if (live_warp) {
+                        uint32_t raw[KH / 32][32];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < KH / 32; ++c) ptx::tmem_ld_32x32(s_addr + h * KH + c * 32, raw[c]);
+                        ptx::tmem_ld_wait();
+                        if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            const uint32_t* v = &raw[c][i];
-                            mx0 = max3(mx0, __uint_as_float(v[0]), __uint_as_float(v[1]));
-                            mx1 = max3(mx1, __uint_as_float(v[2]), __uint_as_float(v[3]));
-                            mx2 = max3(mx2, __uint_as_float(v[4]), __uint_as_float(v[5]));
-                            mx3 = max3(mx3, __uint_as_float(v[6]), __uint_as_float(v[7]));
+                            for (int c = 0; c < KH / 32; ++c)
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (!(see[h * (KH / 32) + c] >> i & 1u)) raw[c][i] = 0xff800000u;  // -inf, and 2^-inf = 0 below
                         }
-                    const float tile_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * t_.scale_log2;
-                    // lazy running maximum: O_t is only touched when it outgrows the one in use by 2^8; every earlier
-                    // product of this slot has finished when S_t is complete
-                    const bool grow = tile_max > m_used + kRescaleThreshold;
-                    if (used > 0 && __any_sync(0xffffffffu, grow)) {
-                        const float alpha = grow ? exp2_fast(m_used - tile_max) : 1.0F;
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            ptx::tmem_ld_32x32(o_addr + c * 32, o);
-                            ptx::tmem_ld_wait();
+                        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            ptx::tmem_st_32x32(o_addr + c * 32, o);
+                        for (int c = 0; c < KH / 32; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                const uint32_t* v = &raw[c][i];
+                                mx0 = max3(mx0, __uint_as_float(v[0]), __uint_as_float(v[1]));
+                                mx1 = max3(mx1, __uint_as_float(v[2]), __uint_as_float(v[3]));
+                                mx2 = max3(mx2, __uint_as_float(v[4]), __uint_as_float(v[5]));
+                                mx3 = max3(mx3, __uint_as_float(v[6]), __uint_as_float(v[7]));
+                            }
+                        const float step_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * t_.scale_log2;
+                        // lazy running maximum: O_t is only touched when it outgrows the one in use by 2^8.  With one step to a
+                        // tile every earlier product of the slot has finished when S_t is complete; with two the one of the step
+                        // before may still run, and what is committed behind it is the other step's next scores.
+                        const bool grow = step_max > m_used + kRescaleThreshold;
+                        if ((used > 0 || h > 0) && __any_sync(0xffffffffu, grow)) {
+                            if (kSteps == 2) {
+                                ok = ptx::mbar_wait(ptx::smem_u32(&s_full[2 * t + 1 - h]), (h == 0 ? n_second : n_first + 1) & 1, abort_flag, status, kCodeTree | 4);
+                                ok = __all_sync(0xffffffffu, ok);
+                                if (!ok) break;
+                                ptx::tc_fence_after();
+                            }
+                            const float alpha = grow ? exp2_fast(m_used - step_max) : 1.0F;
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                ptx::tmem_ld_32x32(o_addr + c * 32, o);
+                                ptx::tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                ptx::tmem_st_32x32(o_addr + c * 32, o);
+                            }
+                            ptx::tmem_st_wait();
+                            row_sum *= alpha;
+                        }
+                        if (grow) m_used = step_max;
+                        const float neg_m = m_used == -INFINITY ? 0.0F : -m_used;
+                        float2 s0 = make_float2(0.0F, 0.0F), s1 = s0;
+                        const float2 scale = make_float2(t_.scale_log2, t_.scale_log2), shift = make_float2(neg_m, neg_m);
+#pragma unroll
+                        for (int c = 0; c < KH / 32; ++c) {
+                            uint32_t packed[16];
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                float2 x = fma2(make_float2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), scale, shift);
+                                float2 y = fma2(make_float2(__uint_as_float(raw[c][i + 2]), __uint_as_float(raw[c][i + 3])), scale, shift);
+                                x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                                s0 = add2(s0, x);
+                                s1 = add2(s1, y);
+                                // the weights are rounded to bf16 for the product; the row sum keeps 32 bits
+                                const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(y.x, y.y);
+                                packed[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
+                                packed[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+                            }
+                            ptx::tmem_st_32x16(s_addr + h * KH + c * 16, packed);
                         }
                         ptx::tmem_st_wait();
-                        row_sum *= alpha;
+                        row_sum += (s0.x + s0.y) + (s1.x + s1.y);
                     }
-                    if (grow) m_used = tile_max;
-                    const float neg_m = m_used == -INFINITY ? 0.0F : -m_used;
-                    float2 s0 = make_float2(0.0F, 0.0F), s1 = s0;
-                    const float2 scale = make_float2(t_.scale_log2, t_.scale_log2), shift = make_float2(neg_m, neg_m);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float2 x = fma2(make_float2(__uint_as_float(raw[c][i]), __uint_as_float(raw[c][i + 1])), scale, shift);
-                            float2 y = fma2(make_float2(__uint_as_float(raw[c][i + 2]), __uint_as_float(raw[c][i + 3])), scale, shift);
-                            x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-                            s0 = add2(s0, x);
-                            s1 = add2(s1, y);
-                            // the weights are rounded to bf16 for the product; the row sum keeps 32 bits
-                            const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(y.x, y.y);
-                            packed[i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
-                            packed[i / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
-                        }
-                        ptx::tmem_st_32x16(s_addr + c * 16, packed);
-                    }
-                    ptx::tmem_st_wait();
-                    row_sum += (s0.x + s0.y) + (s1.x + s1.y);
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(ptx::smem_u32(&p_full[2 * t + h]));
                 }
-                ptx::tc_fence_before();
-                ptx::mbar_arrive(ptx::smem_u32(&p_full[t]));
+                if (!ok) break;
+                ++n_first;
+                ++n_second;
             }
             if (ok && used > 0) {
                 ok = ptx::mbar_wait(ptx::smem_u32(&o_full[t]), n_out & 1, abort_flag, status, kCodeTree | 4);
                 ++n_out;
+                if (kSteps == 2) ++n_first;
                 ptx::tc_fence_after();
             }
             if (!ok) break;

@@ -220,23 +220,48 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
 // The same three, called by a whole converged warp of which one lane (always the same) issues: with the operands the
 // same in all lanes they stay in uniform registers, which a lone lane's do not (an instruction issued from
 // `if (lane == 0)` takes 75 to 100 cycles, one issued here about 35).
-__device__ __forceinline__ void umma_bf16_warp(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// Four steps of 16 along K: operands of 128-byte swizzled rows, 32 bytes a step (K-major) ...
+__device__ __forceinline__ void umma_bf16_x4_warp(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p, e;\n"
+        ".reg .pred p, q, e;\n"
+        ".reg .b64 a, b;\n"
         "elect.sync _|e, 0xffffffff;\n"
         "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 q, %4, %4;\n"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "add.s64 a, %1, 2;\n"
+        "add.s64 b, %2, 2;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n"
+        "add.s64 a, %1, 4;\n"
+        "add.s64 b, %2, 4;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n"
+        "add.s64 a, %1, 6;\n"
+        "add.s64 b, %2, 6;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n"
         "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_bf16_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// ... or A in tensor memory, eight columns a step, and B with its rows along K, 16 rows of 128 bytes a step.
+__device__ __forceinline__ void umma_bf16_ts_x4_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p, e;\n"
+        ".reg .pred p, q, e;\n"
+        ".reg .b32 a;\n"
+        ".reg .b64 b;\n"
         "elect.sync _|e, 0xffffffff;\n"
         "setp.ne.b32 p, %4, 0;\n"
+        "setp.eq.b32 q, %4, %4;\n"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "add.s32 a, %1, 8;\n"
+        "add.s64 b, %2, 128;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n"
+        "add.s32 a, %1, 16;\n"
+        "add.s64 b, %2, 256;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n"
+        "add.s32 a, %1, 24;\n"
+        "add.s64 b, %2, 384;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n"
         "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
