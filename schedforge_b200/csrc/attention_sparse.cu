@@ -869,7 +869,7 @@ sfb_status sfb_k_attention_decode_sparse(const sfb_sparse_args* a, sfb_stream st
     p.scale_log2 = (a->scale > 0.0F ? a->scale : 1.0F / sqrtf(static_cast<float>(a->head_dim))) * 1.4426950408889634F;
     SFB_TRY(step_attention(p, l.step, a->dtype, s));
     if (step_joined(l.step)) return SFB_OK;
-    return merge_partials({p.part, kv, a->out, nullptr, a->batch, a->q_heads, 1, a->head_dim_value, 1}, a->dtype, s);
+    return merge_partials({p.part, kv, a->out, nullptr, a->batch, a->q_heads, 1, a->head_dim_value, 1, 0}, a->dtype, s);
 }
 
 }  // extern "C"

@@ -231,6 +231,13 @@ sfb_status step_typed(const StepParams& p, cudaStream_t stream) {
     return launch_step<T, 32, true>(p, stream);
 }
 
+// Pieces of a row cut into splits of `chunk` keys.
+__device__ __forceinline__ int split_pieces(const MergeParams& p, int b) {
+    if (p.chunk == 0) return p.part.splits;
+    const int keys = p.kv.length(b) + min(p.node_count ? p.node_count[b] : p.nodes, p.nodes);
+    return min(p.part.splits, (keys + p.chunk - 1) / p.chunk);
+}
+
 // One CTA per output row; thread = output element (strided), the two halves of the CTA take alternate pieces.
 template <class T>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ MergeParams p) {
@@ -242,7 +249,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Merg
     if (p.node_count && node >= p.node_count[b]) return;
     RowPieces r;
     if (p.part.span) r = row_pieces(p.part, p.kv.kv_heads, p.q_heads, b, head, p.kv.length(b));
-    else r = {static_cast<size_t>(row) * p.part.splits, 1, p.part.splits};
+    else r = {static_cast<size_t>(row) * p.part.splits, 1, split_pieces(p, b)};
     if (p.part.span && r.count == 1) return;   // written by the attention kernel itself
     // the first eight pieces of each half are fetched before their factors are known
     const int half = threadIdx.x >> 7;
@@ -287,21 +294,39 @@ __global__ void __launch_bounds__(256) merge_rows_kernel(const __grid_constant__
     if (p.node_count && node >= p.node_count[b]) return;
     RowPieces r;
     if (p.part.span) r = row_pieces(p.part, p.kv.kv_heads, p.q_heads, b, head, p.kv.length(b));
-    else r = {static_cast<size_t>(row) * p.part.splits, 1, p.part.splits};
+    else r = {static_cast<size_t>(row) * p.part.splits, 1, split_pieces(p, b)};
     if (p.part.span && r.count == 1) return;   // written by the attention kernel itself
-    const float2 stats = row_statistics(p.part, r, nullptr);
     T* dst = static_cast<T*>(p.out) + (p.token_major ? (static_cast<size_t>(b) * p.nodes + node) * p.q_heads + head
                                                      : static_cast<size_t>(row)) * p.dim_v;
+    // up to kAtOnce pieces of the first 64 elements are fetched while the maximum is found
+    constexpr int kAtOnce = 8;
+    float early[kAtOnce][2];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            early[i][j] = i < r.count && lane + 32 * j < p.dim_v ? p.part.o[(r.first + static_cast<size_t>(i) * r.step) * p.part.o_step + lane + 32 * j] : 0.0F;
+    const float2 stats = row_statistics(p.part, r, nullptr);
+    const auto factor = [&](int i) -> float {
+        const float m = p.part.ml[(r.first + static_cast<size_t>(i) * r.step) * p.part.ml_step];
+        return m == -INFINITY ? 0.0F : exp2_fast(m - stats.x);
+    };
     float a[8] = {};
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+        if (i >= r.count) continue;
+        const float f = factor(i);
+        if (f == 0.0F) continue;
+        a[0] = fmaf(early[i][0], f, a[0]);
+        a[1] = fmaf(early[i][1], f, a[1]);
+    }
 #pragma unroll 4
-    for (int i = 0; i < r.count; ++i) {
-        const size_t index = r.first + static_cast<size_t>(i) * r.step;
-        const float m = p.part.ml[index * p.part.ml_step];
-        const float f = m == -INFINITY ? 0.0F : exp2_fast(m - stats.x);
-        const float* o = p.part.o + index * p.part.o_step;
+    for (int i = p.dim_v > 64 ? 0 : kAtOnce; i < r.count; ++i) {
+        const float f = factor(i);
+        const float* o = p.part.o + (r.first + static_cast<size_t>(i) * r.step) * p.part.o_step;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < p.dim_v) a[j] = f == 0.0F ? a[j] : fmaf(o[lane + 32 * j], f, a[j]);
+            if (lane + 32 * j < p.dim_v && (j >= 2 || i >= kAtOnce)) a[j] = f == 0.0F ? a[j] : fmaf(o[lane + 32 * j], f, a[j]);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)

@@ -94,11 +94,11 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     const int keys = ctx + count;
     const int k0 = min(keys, split * p.chunk), k1 = split == p.splits - 1 ? keys : min(keys, k0 + p.chunk);
     const int row0 = tile * BM;
+    if (k0 >= k1) return;     // (an empty split leaves no piece)
     if (k1 > ctx) tree_ancestors(p, b, count, parent, seen);
     const T* q = static_cast<const T*>(p.q) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all * kv.dim;
-    if (k0 < k1)
-        load_tile<kThreads, T, false>(qs, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, p.scale_log2,
-                               [&](int r) { return row0 + r < rows_all ? q + static_cast<size_t>(row0 + r) * kv.dim : nullptr; });
+    load_tile<kThreads, T, false>(qs, stride, kv.dim, (kv.dim + 3) & ~3, p.vec, p.scale_log2,
+                           [&](int r) { return row0 + r < rows_all ? q + static_cast<size_t>(row0 + r) * kv.dim : nullptr; });
     float o[R][NV * 4], m[R], l[R];
     int node[R];
 #pragma unroll
@@ -138,7 +138,7 @@ tree_simt_kernel(const __grid_constant__ TreeParams p) {
     };
     const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     const auto wait_but_one = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
-    if (k0 < k1) {
+    {
         find_rows(k0, 0);
         __syncthreads();
         fetch_k(0);
@@ -353,7 +353,7 @@ sfb_status sfb_k_attention_tree_paged(const sfb_tree_args* a, sfb_stream stream)
     else SFB_TRY(a->dtype == SFB_F32 ? tree_simt<float>(p, s) : tree_simt<bf16>(p, s));
     if (l.splits == 1) return SFB_OK;
     const Partials part{p.partials, p.partials + 2, nullptr, l.splits, a->head_dim_value + 2, a->head_dim_value + 2};
-    return merge_partials({part, p.kv, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, a->token_major}, a->dtype, s);
+    return merge_partials({part, p.kv, a->out, a->node_count, a->batch, a->q_heads, a->nodes, a->head_dim_value, a->token_major, l.chunk}, a->dtype, s);
 }
 
 }  // extern "C"

@@ -105,6 +105,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     constexpr int kRowsAtOnce = kThreads / kPieces;
     extern __shared__ float4 tree_smem_raw[];
     __shared__ int missing[2];   // the tile has keys without a block
+    __shared__ int row_of[BM];   // head in the group * 256 + node of every row, -1: none
     const PagedView& kv = p.kv;
     const int sk = k_stride(kv.dim), sv = v_stride(kv.dim_v);
     float* qs = reinterpret_cast<float*>(tree_smem_raw);   // [BM][sk]
@@ -125,7 +126,13 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     const int count = tree_node_count(p, b);
     const int keys = ctx + count;
     const int k0 = min(keys, split_id * p.chunk), k1 = split_id == p.splits - 1 ? keys : min(keys, k0 + p.chunk);
-    const int row0 = tile * BM, warp_row = row0 + warp * 16 * M;
+    // the rows of live nodes only, closely packed: a tree of half its nodes costs half the products
+    const int row0 = tile * BM, warp_row = warp * 16 * M, rows_live = group * count;
+    if (row0 >= rows_live || k0 >= k1) return;     // (an empty split leaves no piece)
+    for (int i = threadIdx.x; i < BM; i += kThreads) {
+        const int r = row0 + i;
+        row_of[i] = r < rows_live ? (r / count) * 256 + r % count : -1;
+    }
     if (k1 > ctx) tree_ancestors(p, b, count, parent, seen);
     const float* q = static_cast<const float*>(p.q) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all * kv.dim;
     const float* draft_k = static_cast<const float*>(p.draft_k) + (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.nodes * kv.dim;
@@ -171,7 +178,7 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     const auto wait_but_one = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
     if (threadIdx.x < 2) missing[threadIdx.x] = 0;
     __syncthreads();
-    if (k0 < k1) {
+    {
         note(k0, find(k0), 0);
         __syncthreads();
         fetch(ks, sk, kv.dim, k_rows);
@@ -182,9 +189,9 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
         float4 v[BM / kRowsAtOnce];
 #pragma unroll
         for (int i = 0; i < BM / kRowsAtOnce; ++i) {
-            const int r = row0 + threadIdx.x / kPieces + i * kRowsAtOnce;
+            const int at = row_of[threadIdx.x / kPieces + i * kRowsAtOnce];
             v[i] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-            if (r < rows_all && d < kv.dim) v[i] = *reinterpret_cast<const float4*>(q + static_cast<size_t>(r) * kv.dim + d);
+            if (at >= 0 && d < kv.dim) v[i] = *reinterpret_cast<const float4*>(q + static_cast<size_t>((at >> 8) * p.nodes + (at & 255)) * kv.dim + d);
         }
         if (d < kv.dim)
 #pragma unroll
@@ -199,13 +206,13 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     for (int i = 0; i < 2 * M; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.0F;
-        node[i] = (warp_row + 16 * (i >> 1) + 8 * (i & 1) + r4) % p.nodes;
+        node[i] = max(row_of[warp_row + 16 * (i >> 1) + 8 * (i & 1) + r4], 0) & 255;
     }
 #pragma unroll
     for (int t = 0; t < M; ++t)
 #pragma unroll
         for (int n = 0; n < WIDE; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.0F;
-    const bool busy = warp_row < rows_all;   // the warp has rows
+    const bool busy = row0 + warp_row < rows_live;   // the warp has rows
     float* my_p = ps + warp * 16 * M * kPStride;
     const int nv = kv.dim_v / 8;
     int buffer = 0;
@@ -309,14 +316,15 @@ tree_tf32_kernel(const __grid_constant__ TreeParams p) {
     for (int i = 0; i < 2 * M; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        const int r = warp_row + 16 * (i >> 1) + 8 * (i & 1) + r4;
-        if (r >= rows_all || node[i] >= count) continue;
-        const size_t row = (static_cast<size_t>(b) * kv.kv_heads + kvh) * rows_all + r;
+        const int at = row_of[warp_row + 16 * (i >> 1) + 8 * (i & 1) + r4];
+        if (at < 0) continue;
+        const int head = kvh * group + (at >> 8);
+        const size_t row = (static_cast<size_t>(b) * p.q_heads + head) * p.nodes + node[i];
         float* dst;
         float inv = 1.0F;
         if (p.splits == 1) {
             inv = l[i] == 0.0F ? 0.0F : 1.0F / l[i];
-            dst = static_cast<float*>(p.out) + tree_out_row(p, b, kvh * group + r / p.nodes, node[i]) * kv.dim_v;
+            dst = static_cast<float*>(p.out) + tree_out_row(p, b, head, node[i]) * kv.dim_v;
         } else {
             float* rec = p.partials + (row * p.splits + split_id) * (kv.dim_v + 2);
             if (quad == 0) { rec[0] = m[i]; rec[1] = l[i]; }

@@ -109,10 +109,11 @@ inline bool step_joined(const StepPlan& plan) { return !plan.mma && plan.splits 
 // Rows are (b, q_head, node); nodes == 1 and node_count == nullptr for single-token decode.
 struct MergeParams {
     Partials part;
-    PagedView kv;            // lengths and heads (arrangement by CTAs)
+    PagedView kv;            // lengths and heads
     void* out;
     const int* node_count;
     int batch, q_heads, nodes, dim_v, token_major;
+    int chunk;               // keys of a split, the last split the rest; only the splits that have keys left a piece.  0: all did
 };
 sfb_status merge_partials(const MergeParams& p, int dtype, cudaStream_t stream);
 
