@@ -659,6 +659,48 @@ def test_evict(dev, port, alias, dtype, hkv, d, dv, block, lens, budget, sink, r
         assert np.all(k_pool[page] == 0.25)
 
 
+@gpu
+@pytest.mark.parametrize("alias", [False, True])
+@pytest.mark.parametrize("kind", ["distinct", "few values", "equal"])
+@pytest.mark.parametrize("hkv,lens,budget,sink,recent", [
+    (2, [16384, 0, 5, 12001, 4097], 2048, 4, 256),
+    (1, [40960, 33], 20000, 3, 100),                             # the longest row that a bit mask holds
+    (3, [5000], 1, 1, 0),
+    (1, [8191, 4100], 8190, 0, 8190),                            # everything kept is recent, or one leaves
+    (8, [4200, 4133, 9000, 300], 4100, 64, 0),
+])
+def test_evict_long_rows(dev, alias, kind, hkv, lens, budget, sink, recent):
+    rng = np.random.default_rng(budget + hkv)
+    cache = Cache(rng, lens, hkv, 4, 4, 16, "f32", poison=0.25)
+    stride = max(lens) + 5
+    shape = (cache.batch, hkv, stride)
+    weights = {"distinct": rng.permutation(np.prod(shape)).reshape(shape), "few values": rng.integers(0, 40, shape),
+               "equal": np.full(shape, 3)}[kind].astype(np.float32)
+    positions = np.full(shape, 1 << 20, np.int32)
+    for b, n in enumerate(lens):
+        for h in range(hkv):
+            positions[b, h, :n] = np.arange(n)
+    positions[-1, 0, :min(lens[-1], 7)] = 0                       # positions that repeat
+    dd = Device(dev, cache)
+    w, p = dev.f32(weights), dev.i32(positions)
+    w_out, p_out = (w, p) if alias else (dev.f32(np.full_like(weights, 3.5)), dev.i32(np.full_like(positions, 33)))
+    new_len = dev.i32(np.full(cache.batch, -9))
+    status_word()
+    evict_call(dev, dd, w, w_out, p, p_out, new_len, stride, budget, sink, recent)
+    assert status_word() == 0
+    assert list(dev.np(new_len)) == [min(n, budget) for n in lens]
+    got_w, got_p, k_pool = dev.np(w_out), dev.np(p_out), dev.np(dd.k_pool)
+    for b, n in enumerate(lens):
+        k = min(n, budget)
+        new_k = cache.rows(k_pool, b, n)
+        for h in range(hkv):
+            source = plain_evict(weights[b, h], positions[b, h], n, budget, sink, recent)
+            assert np.array_equal(got_w[b, h, :k], weights[b, h][source])
+            assert np.array_equal(got_p[b, h, :k], positions[b, h][source])
+            assert np.all(got_w[b, h, k:n] == 0.0) and np.all(got_p[b, h, k:n] == -1)
+            assert np.array_equal(new_k[h, :k], cache.keys[b][h][source])
+
+
 # ---- refusals (no device needed) -------------------------------------------------------------------------------------------
 
 
