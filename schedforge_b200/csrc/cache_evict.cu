@@ -167,16 +167,17 @@ struct EvictParams {
     uint8_t* kept;         // [batch * kv_heads][max_context]
     int* moves;            // per (sequence, K/V head): old length, count, then max_moves destinations, then max_moves sources
     int max_moves, stride, budget, sink, recent, masked;   // masked: rows of at most kMaskItems slots
+    int wide_items;        // longest stretch of a row shared by a cluster
 };
 
 constexpr int kEvictThreads = 1024;
 
 // Lists the kept rows of a row too long, or with too many equal weights, for the bit mask: two walks in slot order,
 // which rows are kept (ties go to the lower slot), then the ranks of freed slots and moved rows.
-template <class Safe>
+template <int THREADS, class Safe>
 __device__ int evict_lists(const EvictParams& p, SelectShared& sh, const float* weights, const int* positions, float* weights_out,
                            int* positions_out, uint8_t* kept_bits, int* to, int* since, int n, int k, int room, const Threshold& t, Safe safe) {
-    walk_ranks<kEvictThreads>(sh.walk, n,
+    walk_ranks<THREADS>(sh.walk, n,
         [&](int i) {
             const bool s = safe(i);
             return (s ? 2 : 0) | (!s && room > 0 && t.cut != 0 && order_key(weights[i]) == t.low ? 1 : 0);
@@ -190,7 +191,7 @@ __device__ int evict_lists(const EvictParams& p, SelectShared& sh, const float* 
             kept_bits[i] = kept;
         });
     __syncthreads();
-    const uint64_t totals = walk_ranks<kEvictThreads>(sh.walk, n,
+    const uint64_t totals = walk_ranks<THREADS>(sh.walk, n,
         [&](int i) { return i < k ? (kept_bits[i] ? 0 : 1) : (kept_bits[i] ? 2 : 0); },
         [&](int i, bool hole, bool tail, int holes, int tails) {
             if (hole) { if (holes < p.max_moves) to[holes] = i; }
@@ -296,7 +297,7 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     } else {
         Threshold t{~0ull, 0};
         if (room > 0) t = select_threshold<kEvictThreads>(sh, n, room, [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); });
-        holes = evict_lists(p, sh, weights, positions, weights_out, positions_out, kept_bits, to, since, n, k, room, t, safe);
+        holes = evict_lists<kEvictThreads>(p, sh, weights, positions, weights_out, positions_out, kept_bits, to, since, n, k, room, t, safe);
     }
     __syncthreads();  // the lists, and every read of weights and positions that an aliased output may overwrite
     for (int j = threadIdx.x; j < holes; j += kEvictThreads) {
@@ -304,6 +305,137 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
         positions_out[to[j]] = positions[since[j]];
     }
     if (threadIdx.x == 0) to[-1] = holes;   // (slots behind the new length are cleared with the moves)
+}
+
+// The same with a cluster per row, for long rows: a CTA keeps the keys and positions of its stretch in shared memory.
+constexpr int kWideThreads = 512, kWideFrom = 16384;
+
+__global__ void __cluster_dims__(kWideCtas, 1, 1) __launch_bounds__(kWideThreads)
+evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
+    __shared__ WideShared wide;
+    __shared__ SelectShared sh;        // (rows with too many equal weights only)
+    __shared__ int newest_of[32];
+    __shared__ int newest_here;
+    auto cluster = cooperative_groups::this_cluster();
+    const PagedView& kv = p.kv;
+    const int b = blockIdx.y, kvh = blockIdx.x / kWideCtas, mine = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dependency_wait();
+    const int n = kv.length(b), k = min(n, p.budget);
+    const size_t row = static_cast<size_t>(b) * kv.kv_heads + kvh;
+    const float* weights = p.weights + row * p.stride;
+    const int* positions = p.positions + row * p.stride;
+    float* weights_out = p.weights_out + row * p.stride;
+    int* positions_out = p.positions_out + row * p.stride;
+    int* to = p.moves + row * (2 + 2 * static_cast<size_t>(p.max_moves)) + 2;
+    int* since = to + p.max_moves;
+    if (threadIdx.x == 0 && mine == 0) to[-2] = n;
+    if (k == n) {
+        if (threadIdx.x == 0 && mine == 0) to[-1] = 0;
+        for (int i = mine * kWideThreads + threadIdx.x; i < n; i += kWideCtas * kWideThreads) {
+            weights_out[i] = weights[i];
+            positions_out[i] = positions[i];
+        }
+        return;
+    }
+    extern __shared__ uint32_t keys[];   // of the stretch: the weights' keys (kForced for safe rows), then the positions
+    const int stretch = wide_stretch(n), base = min(n, mine * stretch), count = min(stretch, n - base);
+    int* at = reinterpret_cast<int*>(keys + p.wide_items);
+    int newest = -1;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count; i += kWideThreads) {   // (its own entries, here and below)
+        at[i] = positions[base + i];
+        keys[i] = static_cast<uint32_t>(order_key(weights[base + i]));
+        newest = max(newest, at[i]);
+    }
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) newest_of[warp] = newest;
+    __syncthreads();
+    if (warp == 0) {
+        newest = __reduce_max_sync(0xffffffffu, lane < kWideThreads / 32 ? newest_of[lane] : -1);
+        if (lane == 0) newest_here = newest;
+    }
+    cluster.sync();
+    newest = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&newest_here, lane % kWideCtas));
+    const int64_t recent_from = static_cast<int64_t>(newest) - p.recent;
+    const int sink = p.sink;
+    const auto is_safe = [&](int position) { return position < sink || position > recent_from; };
+    int n_safe = 0;
+    for (int i = threadIdx.x; i < count; i += kWideThreads)
+        if (is_safe(at[i])) {
+            keys[i] = kForced;
+            ++n_safe;
+        }
+    n_safe = __reduce_add_sync(0xffffffffu, n_safe);
+    __syncthreads();
+    if (lane == 0) newest_of[warp] = n_safe;
+    __syncthreads();
+    n_safe = __reduce_add_sync(0xffffffffu, lane < kWideThreads / 32 ? newest_of[lane] : 0);
+    const int room = k - static_cast<int>(offsets_before(cluster, wide, n_safe, 0).all_a);
+    bool settled = false;
+    if (room > 0) {
+        settled = select_mask_wide<kWideThreads>(cluster, wide, keys, count, base, room, [](uint32_t&, uint32_t&) {},
+                                                 [&](int j) -> uint64_t { return keys[wide.near[j] - base]; });
+    } else if (room == 0) {
+        for (int i0 = warp * 32; i0 < count; i0 += kWideThreads) {
+            const unsigned word = __ballot_sync(0xffffffffu, i0 + lane < count && keys[i0 + lane] == kForced);
+            if (lane == 0) wide.words[i0 >> 5] = word;
+        }
+        settled = true;
+        __syncthreads();
+    }
+    if (!settled) {        // (all CTAs of the cluster agree)
+        cluster.sync();    // the others' shared memory is not read any more
+        if (mine != 0) return;
+        const auto safe = [&](int i) { return is_safe(positions[i]); };
+        Threshold t{~0ull, 0};
+        if (room > 0) t = select_threshold<kWideThreads>(sh, n, room, [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); });
+        const int holes = evict_lists<kWideThreads>(p, sh, weights, positions, weights_out, positions_out, p.kept + row * kv.limit, to, since, n, k, room, t, safe);
+        __syncthreads();
+        for (int j = threadIdx.x; j < holes; j += kWideThreads) {
+            weights_out[to[j]] = weights[since[j]];
+            positions_out[to[j]] = positions[since[j]];
+        }
+        if (threadIdx.x == 0) to[-1] = holes;
+        return;
+    }
+    // freed slots before the new length and kept rows behind it
+    const int words = (count + 31) / 32;
+    const auto masks = [&](int w, unsigned& hole, unsigned& tail) {
+        const int first = base + w * 32, left = count - w * 32;
+        const unsigned live = left >= 32 ? ~0u : (1u << left) - 1;
+        const unsigned front = (first + 32 <= k ? ~0u : (first >= k ? 0u : (1u << (k - first)) - 1)) & live;
+        hole = ~wide.words[w] & front;
+        tail = wide.words[w] & ~front & live;
+    };
+    unsigned n_hole = 0, n_tail = 0;
+    for (int w = threadIdx.x; w < words; w += kWideThreads) {
+        unsigned hole, tail;
+        masks(w, hole, tail);
+        n_hole += __popc(hole);
+        n_tail += __popc(tail);
+    }
+    n_hole = __reduce_add_sync(0xffffffffu, n_hole);
+    n_tail = __reduce_add_sync(0xffffffffu, n_tail);
+    if (lane == 0) { wide.lo[warp] = n_hole; wide.hi[warp] = n_tail; }
+    cluster.sync();        // (also: every CTA is done with the safe rows' counts)
+    n_hole = __reduce_add_sync(0xffffffffu, lane < kWideThreads / 32 ? wide.lo[lane] : 0u);
+    n_tail = __reduce_add_sync(0xffffffffu, lane < kWideThreads / 32 ? wide.hi[lane] : 0u);
+    const WideOffsets before = offsets_before(cluster, wide, n_hole, n_tail);
+    walk_bits<kWideThreads>(wide.scan, words, masks,
+        [&](int i, int rank) { if (static_cast<int>(before.a) + rank < p.max_moves) to[before.a + rank] = base + i; },
+        [&](int i, int rank) { if (static_cast<int>(before.b) + rank < p.max_moves) since[before.b + rank] = base + i; });
+    for (int i = threadIdx.x; i < count; i += kWideThreads)
+        if (base + i < k && (wide.words[i >> 5] >> (i & 31) & 1u)) {
+            weights_out[base + i] = weights[base + i];
+            positions_out[base + i] = at[i];
+        }
+    const int holes = min(min(static_cast<int>(before.all_a), static_cast<int>(before.all_b)), p.max_moves);
+    if (threadIdx.x == 0 && mine == 0) to[-1] = holes;
+    cluster.sync();        // the lists, and every read of weights and positions that an aliased output may overwrite
+    for (int j = mine * kWideThreads + threadIdx.x; j < holes; j += kWideCtas * kWideThreads) {
+        weights_out[to[j]] = weights[since[j]];
+        positions_out[to[j]] = positions[since[j]];
+    }
 }
 
 // One warp per moved row; the entries behind the new length are cleared here, and new_len is written here, where
@@ -469,9 +601,22 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
     p.kept = static_cast<uint8_t*>(a->workspace) + evict_moves_bytes(*a);
     p.stride = a->weight_stride; p.budget = a->budget; p.sink = a->sink_tokens; p.recent = a->recent_tokens;
     p.masked = p.kv.limit <= kMaskItems;
+    // Long rows are shared by a cluster each: rows that one CTA's mask does not hold (65536 slots, 8 rows: 165 us by the walks
+    // over 64-bit keys, 30 by a cluster; 131072: 332 and 40), and, while two CTAs an SM hold them all, rows of more than 16384
+    // (32768 slots: 30 us by one CTA, 26 by a cluster; 24500: 28.5 and 24.9; 16384: 24.0 and 23.4; 6000: 17 and 21).
+    const int64_t rows = static_cast<int64_t>(a->batch) * a->kv_heads;
+    const bool wide_select = p.kv.limit <= kWideCtas * kWideItems &&
+                             (!p.masked || (p.kv.limit > kWideFrom && rows * kWideCtas <= 2LL * sm_count()));
     const size_t key_bytes = p.masked ? sizeof(uint32_t) * static_cast<size_t>(p.kv.limit) : 0;
     SFB_CUDA(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(uint32_t) * kMaskItems)));
-    SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
+    if (wide_select) {
+        p.wide_items = wide_stretch(p.kv.limit);
+        SFB_CUDA(cudaFuncSetAttribute(evict_select_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * static_cast<int>(sizeof(uint32_t)) * kWideItems));
+        SFB_CUDA(launch_dependent(evict_select_wide_kernel, dim3(a->kv_heads * kWideCtas, a->batch), dim3(kWideThreads),
+                                  2 * sizeof(uint32_t) * static_cast<size_t>(p.wide_items), s, p));
+    } else {
+        SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
+    }
     SFB_TRY(check_launch("evict_select"));
     const dim3 grid(p.max_moves > 0 ? (p.max_moves > 256 * 8 ? 256 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
     const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool);

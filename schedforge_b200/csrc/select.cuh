@@ -7,6 +7,10 @@
 // The order of the unsigned keys is the order wanted; a key of 0 does not take part.
 #pragma once
 
+#ifdef __CUDACC__
+#include <cooperative_groups.h>
+#endif
+
 #include "common.cuh"
 
 namespace sfb {
@@ -233,6 +237,183 @@ __device__ bool select_mask(SelectShared& sh, const uint32_t* keys, int n, int k
     }
     __syncthreads();
     return true;
+}
+
+// ---- one row by a cluster ----------------------------------------------------------------------------------------
+// select_mask for a row that the kWideCtas CTAs of a cluster share, each with a stretch of its entries: the counts of
+// the bins, the range, the near keys and the totals are read out of the others' shared memory.  Rows of up to kWideCtas *
+// kWideItems entries; the barriers of the cluster cost about 10 us in all, so it takes over where one CTA's walks cost more.
+constexpr int kWideCtas = 8;
+constexpr int kWideItems = 20480;     // longest stretch of a CTA
+
+struct alignas(16) WideShared {
+    unsigned hist[kSelectBins];
+    unsigned scan[33];
+    uint32_t lo[32], hi[32];
+    uint32_t range[2];            // of this CTA's keys
+    uint32_t low, high;
+    int rest, done;
+    int near_count, kept_count;   // of this CTA
+    unsigned counts[2];           // for offsets_before
+    int near[kNearItems], all[kNearItems];
+    uint64_t near_key[kNearItems], all_key[kNearItems];
+    unsigned words[kWideItems / 32];
+};
+
+// Stretch of CTA `rank`: a multiple of 32 entries, all but the last of the same length.
+__host__ __device__ inline int wide_stretch(int n) { return ((n + kWideCtas - 1) / kWideCtas + 31) & ~31; }
+
+// keys: this CTA's n entries, which are numbers base, base + 1, ... of the row.  Otherwise as select_mask; k counts over the
+// whole row and is the same in all CTAs, and so is what is returned.
+template <int THREADS, class Widen, class Rank>
+__device__ bool select_mask_wide(cooperative_groups::cluster_group& cluster, WideShared& sh, const uint32_t* keys, int n, int base, int k,
+                                 Widen widen, Rank rank) {
+    constexpr int kWarps = THREADS / 32, kPer = kSelectBins / THREADS;
+    static_assert(kPer == 4, "four bins a thread: one 16-byte read of each CTA");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = cluster.block_rank();
+    uint32_t low = ~0u, high = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const uint32_t v = keys[i];
+        if (v != 0 && v != kForced) {
+            low = min(low, v);
+            high = max(high, v);
+        }
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0) { sh.lo[warp] = low; sh.hi[warp] = high; }
+    uint4* bins = reinterpret_cast<uint4*>(sh.hist);
+    bins[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x == 0) sh.near_count = sh.kept_count = 0;
+    __syncthreads();
+    if (warp == 0) {
+        low = __reduce_min_sync(0xffffffffu, lane < kWarps ? sh.lo[lane] : ~0u);
+        high = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.hi[lane] : 0u);
+        if (lane == 0) { sh.range[0] = low; sh.range[1] = high; }
+    }
+    cluster.sync();
+    {
+        const uint32_t* other = cluster.map_shared_rank(sh.range, lane % kWideCtas);
+        low = __reduce_min_sync(0xffffffffu, other[0]);
+        high = __reduce_max_sync(0xffffffffu, other[1]);
+    }
+    int rest = k;
+    for (int pass = 0; pass < 4; ++pass) {
+        const int bits = 32 - __clz(high - low), shift = bits > 11 ? bits - 11 : 0;
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const uint32_t v = keys[i];
+            if (v >= low && v <= high && v != kForced) atomicAdd(&sh.hist[(v - low) >> shift], 1u);
+        }
+        cluster.sync();
+        // counts from the top: thread t owns four bins counted downwards from the last
+        uint4 sum4 = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < kWideCtas; ++c) {
+            const uint4 v = cluster.map_shared_rank(bins, c)[THREADS - 1 - threadIdx.x];
+            sum4.x += v.x; sum4.y += v.y; sum4.z += v.z; sum4.w += v.w;
+        }
+        const unsigned count[4] = {sum4.w, sum4.z, sum4.y, sum4.x};
+        const unsigned own = count[0] + count[1] + count[2] + count[3];
+        unsigned sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) sh.scan[warp] = sum;
+        __syncthreads();
+        unsigned above = __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u) + sum - own;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (above < static_cast<unsigned>(rest) && above + count[j] >= static_cast<unsigned>(rest)) {   // one thread, one bin
+                const uint32_t first = low + (static_cast<uint32_t>(kSelectBins - 1 - (threadIdx.x * kPer + j)) << shift);
+                const uint32_t span = (1u << shift) - 1;
+                sh.low = first;
+                sh.high = high - first < span ? high : first + span;
+                sh.rest = rest - static_cast<int>(above);
+                sh.done = shift == 0 || count[j] <= kNearItems / 8;
+            }
+            above += count[j];
+        }
+        __syncthreads();
+        low = sh.low;
+        high = sh.high;
+        rest = sh.rest;
+        if (sh.done) break;     // (the same in all CTAs: they add up the same counts)
+        cluster.sync();         // every CTA has read the bins
+        bins[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+    }
+    widen(low, high);
+    int kept = 0;
+    for (int i0 = warp * 32; i0 < n; i0 += THREADS) {
+        const int i = i0 + lane;
+        const uint32_t v = i < n ? keys[i] : 0;
+        const unsigned word = __ballot_sync(0xffffffffu, v > high);
+        kept += __popc(word & __ballot_sync(0xffffffffu, v != kForced));
+        if (lane == 0) sh.words[i0 >> 5] = word;
+        if (v != 0 && v >= low && v <= high && v != kForced) {
+            const int at = atomicAdd(&sh.near_count, 1);
+            if (at < kNearItems) sh.near[at] = base + i;
+        }
+    }
+    if (lane == 0 && kept) atomicAdd(&sh.kept_count, kept);
+    cluster.sync();
+    int all = 0, before = 0, room = k;     // near keys of the row, of the CTAs before this one
+#pragma unroll
+    for (int c = 0; c < kWideCtas; ++c) {
+        const int near = *cluster.map_shared_rank(&sh.near_count, c);
+        if (c < mine) before += near;
+        all += near;
+        room -= *cluster.map_shared_rank(&sh.kept_count, c);
+    }
+    const int near = sh.near_count;
+    if (all > kNearItems) return false;
+    if (room >= all) {
+        for (int j = threadIdx.x; j < near; j += THREADS) atomicOr(&sh.words[(sh.near[j] - base) >> 5], 1u << ((sh.near[j] - base) & 31));
+    } else {
+        for (int j = warp; j < near; j += kWarps) {
+            const uint64_t v = rank(j);
+            if (lane < kWideCtas) {    // into every CTA's list
+                cluster.map_shared_rank(sh.all, lane)[before + j] = sh.near[j];
+                cluster.map_shared_rank(sh.all_key, lane)[before + j] = v;
+            }
+            if (lane == 0) sh.near_key[j] = v;
+        }
+        cluster.sync();
+        for (int j = threadIdx.x; j < near; j += THREADS) {
+            const uint64_t v = sh.near_key[j];
+            const int i = sh.near[j];
+            int ahead = 0;
+            for (int o = 0; o < all; ++o) {
+                const uint64_t w = sh.all_key[o];
+                ahead += w > v || (w == v && sh.all[o] < i);
+            }
+            if (ahead < room) atomicOr(&sh.words[(i - base) >> 5], 1u << ((i - base) & 31));
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
+// Sums of a and b (this CTA's counts, the same in all its threads) over the CTAs before this one, and over all.
+struct WideOffsets {
+    unsigned a, b, all_a, all_b;
+};
+__device__ __forceinline__ WideOffsets offsets_before(cooperative_groups::cluster_group& cluster, WideShared& sh, unsigned a, unsigned b) {
+    if (threadIdx.x == 0) { sh.counts[0] = a; sh.counts[1] = b; }
+    cluster.sync();
+    WideOffsets o{0u, 0u, 0u, 0u};
+    const unsigned mine = cluster.block_rank();
+#pragma unroll
+    for (unsigned c = 0; c < kWideCtas; ++c) {
+        const unsigned* other = cluster.map_shared_rank(sh.counts, c);
+        const unsigned x = other[0], y = other[1];
+        if (c < mine) { o.a += x; o.b += y; }
+        o.all_a += x;
+        o.all_b += y;
+    }
+    return o;
 }
 
 // Walks the set bits of two masks of `words` words in ascending order: visit_a(index, rank), visit_b(index, rank).

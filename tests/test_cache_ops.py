@@ -668,6 +668,10 @@ def test_evict(dev, port, alias, dtype, hkv, d, dv, block, lens, budget, sink, r
     (3, [5000], 1, 1, 0),
     (1, [8191, 4100], 8190, 0, 8190),                            # everything kept is recent, or one leaves
     (8, [4200, 4133, 9000, 300], 4100, 64, 0),
+    (1, [16385, 16384], 16383, 2, 16000),                        # where a cluster takes over
+    (2, [65543, 90, 40961], 30000, 4, 30),
+    (1, [163840, 163839], 2048, 4, 256),                         # the longest rows of a cluster
+    (1, [163841, 20], 100000, 4, 256),                           # and longer ones
 ])
 def test_evict_long_rows(dev, alias, kind, hkv, lens, budget, sink, recent):
     rng = np.random.default_rng(budget + hkv)
