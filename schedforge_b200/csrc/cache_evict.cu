@@ -438,7 +438,9 @@ evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
     }
 }
 
-// One warp per moved row; the entries behind the new length are cleared here, and new_len is written here, where
+constexpr int kMoveRows = 4;
+
+// A warp moves four rows at once (one after the other, each with its chain of list, table and row, moved 125 MB in 130 us); the entries behind the new length are cleared here, and new_len is written here, where
 // nothing reads context_len (it may be the same array).
 template <class V>
 __global__ void __launch_bounds__(256)
@@ -451,11 +453,31 @@ evict_move_kernel(const __grid_constant__ EvictParams p, int k_units, int v_unit
     const int count = to[-1];
     V* keys = static_cast<V*>(const_cast<void*>(kv.k_pool));
     V* values = static_cast<V*>(const_cast<void*>(kv.v_pool));
-    for (int j = blockIdx.x * 8 + warp; j < count; j += gridDim.x * 8) {
-        const int64_t src = kv.row(b, kvh, since[j]), dst = kv.row(b, kvh, to[j]);
-        if (src < 0 || dst < 0) continue;
-        for (int i = lane; i < k_units; i += 32) keys[dst * k_units + i] = keys[src * k_units + i];
-        for (int i = lane; i < v_units; i += 32) values[dst * v_units + i] = values[src * v_units + i];
+    for (int j0 = (blockIdx.x * 8 + warp) * kMoveRows; j0 < count; j0 += gridDim.x * 8 * kMoveRows) {
+        int64_t src = -1, dst = -1;
+        if (lane < kMoveRows && j0 + lane < count) {
+            src = kv.row(b, kvh, since[j0 + lane]);
+            dst = kv.row(b, kvh, to[j0 + lane]);
+            if (dst < 0) src = -1;
+        }
+        int64_t from[kMoveRows], into[kMoveRows];
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r) {
+            from[r] = __shfl_sync(0xffffffffu, src, r);
+            into[r] = __shfl_sync(0xffffffffu, dst, r);
+        }
+        for (int i = lane; i < k_units + v_units; i += 32) {
+            const bool key = i < k_units;
+            V* pool = key ? keys : values;
+            const int width = key ? k_units : v_units, at = key ? i : i - k_units;
+            V unit[kMoveRows];
+#pragma unroll
+            for (int r = 0; r < kMoveRows; ++r)
+                if (from[r] >= 0) unit[r] = pool[from[r] * width + at];
+#pragma unroll
+            for (int r = 0; r < kMoveRows; ++r)
+                if (from[r] >= 0) pool[into[r] * width + at] = unit[r];
+        }
     }
     const int n = to[-2], k = min(n, p.budget);
     const size_t row = (static_cast<size_t>(b) * kv.kv_heads + kvh) * p.stride;
@@ -618,7 +640,10 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
         SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
     }
     SFB_TRY(check_launch("evict_select"));
-    const dim3 grid(p.max_moves > 0 ? (p.max_moves > 256 * 8 ? 256 : ceil_div(p.max_moves, 8)) : 1, a->kv_heads, a->batch);
+    // eight warps of four rows a CTA, about two rounds of eight CTAs an SM at most
+    const int most = static_cast<int>(16LL * sm_count() / rows > 0 ? 16LL * sm_count() / rows : 1);
+    const int wanted = ceil_div(p.max_moves, 8 * kMoveRows);
+    const dim3 grid(wanted < 1 ? 1 : wanted < most ? wanted : most, a->kv_heads, a->batch);
     const bool wide = wide_rows(a->head_dim, a->head_dim_value, a->dtype) && aligned16(a->k_pool) && aligned16(a->v_pool);
     const int per = wide ? 16 / static_cast<int>(dtype_size(a->dtype)) : 1;
     const int ku = a->head_dim / per, vu = a->head_dim_value / per;
