@@ -1,9 +1,10 @@
 // Single-token attention over a paged cache, CUDA-core form: any type, head dimension up to 256, block size and group.
 //
 // One CTA handles one (sequence, K/V head, up to eight query heads, split).  A key row is read by LPR lanes, eight
-// elements each, so that a warp has 32 / LPR rows in flight, four times over; every lane group runs its own online
-// softmax over the rows it meets (no synchronisation while streaming), and the groups, warps and splits are joined by
-// the log-sum-exp rule.  All heads of the CTA share each K and V byte.  Memory-bound for small groups; the K/V bytes
+// elements each, so that a warp has 32 / LPR rows in flight, four times over (twice where four float32 or eight bf16 heads
+// leave too few registers for four CTAs an SM: 295 -> 240 us for 16 ragged float32 sequences to 8192 tokens, 32/8 heads of
+// 128); the blocks of the next rows are looked up a round ahead.  Every lane group runs its own online softmax over the
+// rows it meets (no synchronisation while streaming), and the groups, warps and splits are joined by the log-sum-exp rule.  All heads of the CTA share each K and V byte.  Memory-bound for small groups; the K/V bytes
 // are read once per eight query heads.
 #include "cache_ops.cuh"
 
@@ -11,7 +12,6 @@ namespace sfb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kRows = 4;  // rows in flight per lane group
 
 // Eight elements of a row: lane `sub` of LPR owns [8 * sub, 8 * sub + 8) (VEC: dim % 8 == 0 and 16-byte aligned rows),
 // or every LPR-th element.
@@ -43,7 +43,7 @@ struct Piece {
 template <class T, int LPR, int G, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32)
 step_kernel(const __grid_constant__ StepParams p) {
-    constexpr int RPW = 32 / LPR;
+    constexpr int RPW = 32 / LPR, kRows = G * sizeof(T) >= 16 ? 2 : 4;
     extern __shared__ float merge_smem[];  // [kWarps][G][dim_v + 2]
     const PagedView& kv = p.kv;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPR, rg = lane / LPR;
@@ -71,31 +71,40 @@ step_kernel(const __grid_constant__ StepParams p) {
         m[g] = -INFINITY;
         l[g] = 0.0F;
     }
+    // block and position (-1: none) of the warp's rows base + u * RPW + rg, read one round ahead
+    int next_page[kRows], next_position[kRows];
+    const auto locate = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int r = base + u * RPW + rg;
+            next_page[u] = -1;
+            next_position[u] = -1;
+            if (r >= rows) continue;
+            const int e = kv.block_of(r);
+            const int logical = list ? list[e0 + e] : e0 + e;
+            // (a list entry of -1 ends the list; it cannot be met before `entries`, but is not followed either)
+            const int at = logical * kv.block_tokens + (r - e * kv.block_tokens);
+            if (logical < 0 || at >= ctx) continue;
+            next_position[u] = at;
+            next_page[u] = kv.page(b, at);
+        }
+    };
+    locate(warp * RPW * kRows);
     for (int base = warp * RPW * kRows; base < rows; base += kWarps * RPW * kRows) {
         Piece<T, LPR, VEC> kp[kRows], vp[kRows];
         int position[kRows];
         bool live[kRows];
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            const int r = base + u * RPW + rg;
-            live[u] = r < rows;
-            int64_t at = -1;
-            position[u] = 0;
-            if (live[u]) {
-                const int e = kv.block_of(r);
-                int logical = list ? list[e0 + e] : e0 + e;
-                // (a list entry of -1 ends the list; it cannot be met before `entries`, but is not followed either)
-                position[u] = logical * kv.block_tokens + (r - e * kv.block_tokens);
-                live[u] = logical >= 0 && position[u] < ctx;
-                if (live[u]) at = kv.row(b, kvh, position[u]);
-            }
-            const bool there = at >= 0;
-            kp[u].load(static_cast<const T*>(kv.k_pool) + (there ? at : 0) * kv.dim, sub, kv.dim, there);
-            vp[u].load(static_cast<const T*>(kv.v_pool) + (there ? at : 0) * kv.dim_v, sub, kv.dim_v, there);
-            if (live[u] && !there && p.logits && sub < heads)   // a position whose block is missing weighs nothing
+            position[u] = next_position[u];
+            const int64_t at = position[u] >= 0 ? kv.row_in(next_page[u], kvh, position[u]) : -1;
+            live[u] = at >= 0;
+            kp[u].load(static_cast<const T*>(kv.k_pool) + (live[u] ? at : 0) * kv.dim, sub, kv.dim, live[u]);
+            vp[u].load(static_cast<const T*>(kv.v_pool) + (live[u] ? at : 0) * kv.dim_v, sub, kv.dim_v, live[u]);
+            if (position[u] >= 0 && !live[u] && p.logits && sub < heads)   // a position whose block is missing weighs nothing
                 p.logits[(static_cast<size_t>(b) * p.q_heads + head0 + sub) * p.logit_stride + position[u]] = -INFINITY;
-            live[u] = there;
         }
+        locate(base + kWarps * RPW * kRows);
         float x[kRows][G];
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
@@ -364,8 +373,8 @@ PagedView make_view(const void* k_pool, const void* v_pool, const int* table, co
 
 // The tensor-core kernel takes bf16, head_dim = head_dim_value = 128 or 64 and blocks of a multiple of 16 tokens; its
 // CTAs, two per SM, take equal ranges of all work.  The other one cuts every row into splits of whole blocks: as long as
-// two CTAs per SM allow (the ramp of a split is paid once), but at most 2048 positions, which evens out ragged
-// contexts, and at least 64.
+// two CTAs per SM allow (the ramp of a split is paid once), but at most 512 positions, which evens out ragged contexts (2048:
+// 195 instead of 157 us for 64 float32 sequences to 4096 tokens, 307 instead of 252 for eight of 8192), and at least 64.
 StepPlan step_plan(int dtype, int dim, int dim_v, int batch, int q_heads, int kv_heads, int tokens, int block_tokens, int num_blocks,
                    int wanted, bool wide) {
     StepPlan plan{};
@@ -386,7 +395,7 @@ StepPlan step_plan(int dtype, int dim, int dim_v, int batch, int q_heads, int kv
     int splits = wanted;
     if (splits <= 0) {
         splits = static_cast<int>(slots / heads < tokens / 64 ? slots / heads : tokens / 64);
-        if (splits < ceil_div(tokens, 2048)) splits = ceil_div(tokens, 2048);
+        if (splits < ceil_div(tokens, 512)) splits = ceil_div(tokens, 512);
     }
     if (splits > 128) splits = 128;
     if (splits > blocks) splits = blocks;
