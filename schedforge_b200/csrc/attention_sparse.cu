@@ -690,7 +690,7 @@ select_kernel(const __grid_constant__ SelectParams p) {
     const float err2 = reach < 1e37F ? 2.0F * p.error * reach + 1e-34F : INFINITY;
     const bool zeros = norm == 0.0F || size == 0.0F;   // (then every score is exactly zero)
     if (p.cached && k > n_forced) {
-        const bool settled = select_mask<kSelectThreads>(
+        const bool settled = select_mask<kSelectThreads, false>(
             sh, keys, n, k - n_forced,
             [&](uint32_t& low, uint32_t& high) {   // whatever the tolerance lets change places with the k-th (NaN, infinity: all)
                 const float from = score_of_key(low) - err2, to = score_of_key(high) + err2;

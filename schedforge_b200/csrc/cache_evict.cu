@@ -172,7 +172,7 @@ struct EvictParams {
 
 constexpr int kEvictThreads = 1024;
 
-// Lists the kept rows of a row too long, or with too many equal weights, for the bit mask: two walks in slot order,
+// Lists the kept rows of a row that is too long for the bit mask, or has more safe positions than the budget holds: two walks in slot order,
 // which rows are kept (ties go to the lower slot), then the ranks of freed slots and moved rows.
 template <int THREADS, class Safe>
 __device__ int evict_lists(const EvictParams& p, SelectShared& sh, const float* weights, const int* positions, float* weights_out,
@@ -268,7 +268,7 @@ evict_select_kernel(const __grid_constant__ EvictParams p) {
     bool settled = false;
     if (p.masked && n_safe <= k) {
         if (room > 0) {
-            settled = select_mask<kEvictThreads>(sh, keys, n, room, [](uint32_t&, uint32_t&) {}, [&](int j) -> uint64_t { return keys[sh.near[j]]; });
+            settled = select_mask<kEvictThreads, true>(sh, keys, n, room, [](uint32_t&, uint32_t&) {}, [&](int j) -> uint64_t { return keys[sh.near[j]]; });
         } else {
             for (int i0 = warp * 32; i0 < n; i0 += kEvictThreads) {
                 const unsigned word = __ballot_sync(0xffffffffu, i0 + lane < n && keys[i0 + lane] == kForced);
@@ -313,7 +313,6 @@ constexpr int kWideThreads = 512, kWideFrom = 16384;
 __global__ void __cluster_dims__(kWideCtas, 1, 1) __launch_bounds__(kWideThreads)
 evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
     __shared__ WideShared wide;
-    __shared__ SelectShared sh;        // (rows with too many equal weights only)
     __shared__ int newest_of[32];
     __shared__ int newest_here;
     auto cluster = cooperative_groups::this_cluster();
@@ -337,7 +336,8 @@ evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
         }
         return;
     }
-    extern __shared__ uint32_t keys[];   // of the stretch: the weights' keys (kForced for safe rows), then the positions
+    extern __shared__ __align__(16) uint32_t wide_keys[];
+    uint32_t* keys = wide_keys;          // of the stretch: the weights' keys (kForced for safe rows), then the positions
     const int stretch = wide_stretch(n), base = min(n, mine * stretch), count = min(stretch, n - base);
     int* at = reinterpret_cast<int*>(keys + p.wide_items);
     int newest = -1;
@@ -373,7 +373,7 @@ evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
     const int room = k - static_cast<int>(offsets_before(cluster, wide, n_safe, 0).all_a);
     bool settled = false;
     if (room > 0) {
-        settled = select_mask_wide<kWideThreads>(cluster, wide, keys, count, base, room, [](uint32_t&, uint32_t&) {},
+        settled = select_mask_wide<kWideThreads>(cluster, wide, keys, count, base, room,
                                                  [&](int j) -> uint64_t { return keys[wide.near[j] - base]; });
     } else if (room == 0) {
         for (int i0 = warp * 32; i0 < count; i0 += kWideThreads) {
@@ -383,9 +383,10 @@ evict_select_wide_kernel(const __grid_constant__ EvictParams p) {
         settled = true;
         __syncthreads();
     }
-    if (!settled) {        // (all CTAs of the cluster agree)
+    if (!settled) {        // more safe positions than the budget holds (all CTAs of the cluster agree)
         cluster.sync();    // the others' shared memory is not read any more
         if (mine != 0) return;
+        SelectShared& sh = *reinterpret_cast<SelectShared*>(wide_keys);   // (the keys are not needed any more)
         const auto safe = [&](int i) { return is_safe(positions[i]); };
         Threshold t{~0ull, 0};
         if (room > 0) t = select_threshold<kWideThreads>(sh, n, room, [&](int i) -> uint64_t { return safe(i) ? 0 : order_key(weights[i]); });
@@ -635,7 +636,7 @@ sfb_status sfb_k_paged_kv_evict(const sfb_evict_args* a, sfb_stream stream) {
         p.wide_items = wide_stretch(p.kv.limit);
         SFB_CUDA(cudaFuncSetAttribute(evict_select_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * static_cast<int>(sizeof(uint32_t)) * kWideItems));
         SFB_CUDA(launch_dependent(evict_select_wide_kernel, dim3(a->kv_heads * kWideCtas, a->batch), dim3(kWideThreads),
-                                  2 * sizeof(uint32_t) * static_cast<size_t>(p.wide_items), s, p));
+                                  std::max(2 * sizeof(uint32_t) * static_cast<size_t>(p.wide_items), sizeof(SelectShared)), s, p));
     } else {
         SFB_CUDA(launch_dependent(evict_select_kernel, dim3(a->kv_heads, a->batch), dim3(kEvictThreads), key_bytes, s, p));
     }

@@ -2,8 +2,9 @@
 //
 // Rows of up to kMaskItems keys of 32 bits (select_mask): the keys are counted in 2048 equal bins of their range, what
 // lies above the bin of the k-th is kept, and the few keys inside it are ranked against one another; the result is one
-// bit per key in shared memory.  Where too many keys share that bin, and for longer rows, keys of 64 bits are narrowed
-// bin by bin until the range holds one value (select_threshold: at most six passes).
+// bit per key in shared memory.  A bin with too many keys is cut into bins again, until it holds few or equal ones.  Keys known to
+// a tolerance of which too many are left, and longer rows, take keys of 64 bits that are narrowed bin by bin until
+// the range holds one value (select_threshold: at most six passes).
 // The order of the unsigned keys is the order wanted; a key of 0 does not take part.
 #pragma once
 
@@ -41,7 +42,7 @@ struct SelectShared {
     unsigned long long walk[32];
     uint64_t low, high;
     int rest, done;
-    unsigned words[kMaskWords];
+    unsigned words[kMaskWords], ties[kMaskWords];
     int near[kNearItems];
     uint64_t near_key[kNearItems];
     int near_count, kept_count;
@@ -129,14 +130,44 @@ __device__ Threshold select_threshold(SelectShared& sh, int n, int k, Key key) {
     return found;
 }
 
+// words |= the first `room` set bits of ties, counting on from `before`.
+template <int THREADS>
+__device__ __forceinline__ void take_first(unsigned* scan, const unsigned* ties, unsigned* words, int count, int room, int before) {
+    constexpr int kWarps = THREADS / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int w0 = 0; w0 < count; w0 += THREADS) {
+        const int w = w0 + threadIdx.x;
+        const unsigned bits = w < count ? ties[w] : 0u;
+        const int own = __popc(bits);
+        int incl = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        const unsigned mine = lane < kWarps ? scan[lane] : 0u;
+        const int take = room - (before + static_cast<int>(__reduce_add_sync(0xffffffffu, lane < warp ? mine : 0u)) + incl - own);
+        before += static_cast<int>(__reduce_add_sync(0xffffffffu, mine));
+        if (take > 0 && own > 0) {
+            unsigned rest = bits;
+            for (int i = 0; i < take && rest; ++i) rest &= rest - 1;
+            words[w] |= bits & ~rest;
+        }
+        __syncthreads();
+    }
+}
+
 constexpr uint32_t kForced = 0xffffffffu;   // a 32-bit key that is kept whatever the others are (no number's image)
 
 // Bits of the kept keys in sh.words: the forced ones and the k largest of the others (n <= kMaskItems; 1 <= k <= number of
 // other keys that are not 0).  keys: shared memory, complete after the callers' last barrier.  widen(low, high) may
 // extend the range of keys that are ranked, and rank(j) gives the final key of near item j (index sh.near[j]; called by
-// whole warps, all lanes of which return it): how keys known to a tolerance are ranked exactly where it matters.
-// Returns false, with nothing settled, where more than kNearItems keys are in that range.  All threads call it.
-template <int THREADS, class Widen, class Rank>
+// whole warps, all lanes of which return it): how keys known to a tolerance are ranked exactly where it matters.  EXACT: keys
+// are final, so that a range of one value is settled by index (one with more than kNearItems keys always is).  Otherwise
+// that many are not settled, and it returns false.  All threads call it.
+template <int THREADS, bool EXACT, class Widen, class Rank>
 __device__ bool select_mask(SelectShared& sh, const uint32_t* keys, int n, int k, Widen widen, Rank rank) {
     constexpr int kWarps = THREADS / 32, kPer = kSelectBins / THREADS;
     static_assert(kPer >= 1 && kWarps <= 32, "one or more bins a thread");
@@ -206,8 +237,13 @@ __device__ bool select_mask(SelectShared& sh, const uint32_t* keys, int n, int k
         const uint32_t v = i < n ? keys[i] : 0;
         const unsigned word = __ballot_sync(0xffffffffu, v > high);
         kept += __popc(word & __ballot_sync(0xffffffffu, v != kForced));
-        if (lane == 0) sh.words[i0 >> 5] = word;
-        if (v != 0 && v >= low && v <= high && v != kForced) {
+        const bool is_near = v != 0 && v >= low && v <= high && v != kForced;
+        const unsigned ties = __ballot_sync(0xffffffffu, is_near);
+        if (lane == 0) {
+            sh.words[i0 >> 5] = word;
+            sh.ties[i0 >> 5] = ties;
+        }
+        if (is_near) {
             const int at = atomicAdd(&sh.near_count, 1);
             if (at < kNearItems) sh.near[at] = i;
         }
@@ -215,6 +251,10 @@ __device__ bool select_mask(SelectShared& sh, const uint32_t* keys, int n, int k
     if (lane == 0 && kept) atomicAdd(&sh.kept_count, kept);
     __syncthreads();
     const int near = sh.near_count, room = k - sh.kept_count;
+    if (EXACT && low == high) {
+        take_first<THREADS>(sh.scan, sh.ties, sh.words, (n + 31) / 32, room, 0);
+        return true;
+    }
     if (near > kNearItems) return false;
     if (room >= near) {
         for (int j = threadIdx.x; j < near; j += THREADS) atomicOr(&sh.words[sh.near[j] >> 5], 1u << (sh.near[j] & 31));
@@ -257,17 +297,17 @@ struct alignas(16) WideShared {
     unsigned counts[2];           // for offsets_before
     int near[kNearItems], all[kNearItems];
     uint64_t near_key[kNearItems], all_key[kNearItems];
-    unsigned words[kWideItems / 32];
+    unsigned words[kWideItems / 32], ties[kWideItems / 32];
 };
 
 // Stretch of CTA `rank`: a multiple of 32 entries, all but the last of the same length.
 __host__ __device__ inline int wide_stretch(int n) { return ((n + kWideCtas - 1) / kWideCtas + 31) & ~31; }
 
-// keys: this CTA's n entries, which are numbers base, base + 1, ... of the row.  Otherwise as select_mask; k counts over the
+// keys: this CTA's n entries, final, which are numbers base, base + 1, ... of the row.  Otherwise as select_mask; k counts over the
 // whole row and is the same in all CTAs, and so is what is returned.
-template <int THREADS, class Widen, class Rank>
+template <int THREADS, class Rank>
 __device__ bool select_mask_wide(cooperative_groups::cluster_group& cluster, WideShared& sh, const uint32_t* keys, int n, int base, int k,
-                                 Widen widen, Rank rank) {
+                                 Rank rank) {
     constexpr int kWarps = THREADS / 32, kPer = kSelectBins / THREADS;
     static_assert(kPer == 4, "four bins a thread: one 16-byte read of each CTA");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = cluster.block_rank();
@@ -344,15 +384,19 @@ __device__ bool select_mask_wide(cooperative_groups::cluster_group& cluster, Wid
         bins[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
     }
-    widen(low, high);
     int kept = 0;
     for (int i0 = warp * 32; i0 < n; i0 += THREADS) {
         const int i = i0 + lane;
         const uint32_t v = i < n ? keys[i] : 0;
         const unsigned word = __ballot_sync(0xffffffffu, v > high);
         kept += __popc(word & __ballot_sync(0xffffffffu, v != kForced));
-        if (lane == 0) sh.words[i0 >> 5] = word;
-        if (v != 0 && v >= low && v <= high && v != kForced) {
+        const bool is_near = v != 0 && v >= low && v <= high && v != kForced;
+        const unsigned ties = __ballot_sync(0xffffffffu, is_near);
+        if (lane == 0) {
+            sh.words[i0 >> 5] = word;
+            sh.ties[i0 >> 5] = ties;
+        }
+        if (is_near) {
             const int at = atomicAdd(&sh.near_count, 1);
             if (at < kNearItems) sh.near[at] = base + i;
         }
@@ -368,6 +412,10 @@ __device__ bool select_mask_wide(cooperative_groups::cluster_group& cluster, Wid
         room -= *cluster.map_shared_rank(&sh.kept_count, c);
     }
     const int near = sh.near_count;
+    if (low == high) {
+        take_first<THREADS>(sh.scan, sh.ties, sh.words, (n + 31) / 32, room, before);
+        return true;
+    }
     if (all > kNearItems) return false;
     if (room >= all) {
         for (int j = threadIdx.x; j < near; j += THREADS) atomicOr(&sh.words[(sh.near[j] - base) >> 5], 1u << ((sh.near[j] - base) & 31));
