@@ -622,9 +622,11 @@ tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
 }
 
-// Joins the pieces of pairs that were cut: one warp per query row.
-template <int D>
-__global__ void __launch_bounds__(256)
+// Joins the pieces of pairs that were cut: one warp per query row, which reads up to kAtOnce pieces at the same time.  Eight
+// where all CTAs are on the GPU at once (8 rows, 5 pieces: 11.1 us with the attention, 11.7 with four), else four, with five CTAs
+// an SM instead of three (2048 CTAs of 2 to 4 pieces: 111.4 -> 109.1 us).
+template <int D, int kAtOnce>
+__global__ void __launch_bounds__(256, kAtOnce == 4 ? 5 : 1)
 tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
     constexpr int V = D / 32;
     const TreeParams& t = p.t;
@@ -641,8 +643,6 @@ tree_join_kernel(const __grid_constant__ TreeTcParams p, int rows_cta) {
     const int2 span = p.pair_span[pair];      // (not written where the sequence has no nodes; then the count is 0)
     if (node >= tree_node_count(t, b)) return;
     if (span.x == span.y) return;   // written by the attention kernel itself
-    // up to kAtOnce pieces are read at the same time
-    constexpr int kAtOnce = 8;
     const auto index = [&](int c) { return piece_of(c, c == span.x) * rows_cta + tile_row; };
     float2 ml[kAtOnce];
     float part[kAtOnce][V];
@@ -727,7 +727,9 @@ sfb_status launch_tc(const sfb_tree_args& a, const TcLayout& l, TreeTcParams& p,
     SFB_CUDA(cudaFuncSetAttribute(tree_tcgen05_kernel<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     SFB_CUDA(launch_dependent(tree_tcgen05_kernel<D, ROWS>, dim3(l.grid), dim3(kThreads), smem, stream, mq, mk, mv, mdk, mdv, p));
     SFB_TRY(check_launch("attention_tree_tcgen05"));
-    SFB_CUDA(launch_dependent(tree_join_kernel<D>, dim3(static_cast<unsigned>(l.pairs * (ROWS / 8))), dim3(256), 0, stream, p, ROWS));
+    const dim3 join(static_cast<unsigned>(l.pairs * (ROWS / 8)));
+    if (join.x <= 3u * static_cast<unsigned>(sm_count())) SFB_CUDA(launch_dependent(tree_join_kernel<D, 8>, join, dim3(256), 0, stream, p, ROWS));
+    else SFB_CUDA(launch_dependent(tree_join_kernel<D, 4>, join, dim3(256), 0, stream, p, ROWS));
     return check_launch("attention_tree_join");
 }
 
